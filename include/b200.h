@@ -341,6 +341,102 @@ b200_status b200_graph_compute(b200_context * ctx, const b200_tensor * tensors, 
 int b200_graph_supports(const b200_tensor * tensors, int64_t n, int64_t i);
 
 /* ------------------------------------------------------------------------------------------------------------
+ * Paged key/value cache: one layer's keys and values of many sequences in pages of one pool, written (and quantized)
+ * row by row, read back, and attended to. The reference keeps one dense F16 cache per request
+ * (src/common/qwen3-decoder.cpp:300-346) and attends to a view of it; this is the form for a program that serves many
+ * requests with one set of weights: sequence s's position p lies in page table[s][p / page_size], slot p % page_size.
+ *
+ * Layout of the cache's memory, arrays in this order, each starting at a multiple of 256 bytes (field_off):
+ *   F16:  k f16 [n_pages][n_kv_head][page_size][head_dim] | v likewise
+ *   Q8_0: k int8 [n_pages][n_kv_head][page_size][head_dim] | v likewise | k scales f16 [n_pages][n_kv_head][page_size]
+ *         [head_dim / 32] | v scales likewise; a value is its scale times the int8, and a row's blocks are quantized as
+ *         GGUF Q8_0 rows are (b200_quantize_rows), bit for bit. Blocks with non-finite values are unspecified.
+ *
+ * table: int32 [n_seq][max_pages] page numbers (entries past a sequence's length are not read); lens: int32 [n_seq], each
+ * sequence's positions INCLUDING the n_tok rows of the call, so row r of sequence s is position lens[s] - n_tok + r; a
+ * row whose position is negative does not exist (a batch of unequal prompts is aligned at its rows' end, and a length of 0
+ * is an empty place in the batch). Both are device memory. A length outside [0, max_pages * page_size] counts as 0 and a
+ * position whose page lies outside [0, n_pages) is left out; b200_synchronize() reports either as B200_ERR_RANGE (for a
+ * call on another stream: once that stream's work is done). Two rows of one call that name the same slot (a page shared by
+ * two sequences that both write to it) leave that slot's bytes unspecified.
+ *
+ * stream: a cudaStream_t of the context's device (cudaStreamLegacy for the default stream); NULL: the context's stream.
+ * These calls allocate nothing, use none of the context's scratch and may be captured in CUDA graphs.
+ * ------------------------------------------------------------------------------------------------------------ */
+typedef struct b200_kv_cache {
+    int32_t type;      /* B200_TYPE_F16 or B200_TYPE_Q8_0 */
+    int32_t device;
+    int32_t n_kv_head;
+    int32_t head_dim;  /* 64, 96, 128 or 256 */
+    int32_t page_size; /* positions per page: a multiple of 16, at most 4096 */
+    int32_t owned;     /* data was allocated by b200_kv_cache_alloc */
+    int64_t n_pages;
+    void * data;
+    size_t nbytes;
+    int64_t field_off[4]; /* byte offset of k, v, k scales, v scales in data */
+} b200_kv_cache;
+
+/* Bytes of a cache's memory; 0 for a type, head_dim, page_size or size that is not supported. */
+size_t b200_kv_cache_nbytes(int type, int64_t n_kv_head, int64_t head_dim, int64_t page_size, int64_t n_pages);
+/* Allocates a cache (zeroed). */
+b200_status b200_kv_cache_alloc(b200_context * ctx, int type, int64_t n_kv_head, int64_t head_dim, int64_t page_size, int64_t n_pages,
+                                b200_kv_cache * out);
+/* The same on the caller's device memory (16-byte aligned, at least b200_kv_cache_nbytes bytes, kept as it is). */
+b200_status b200_kv_cache_view(b200_context * ctx, int type, int64_t n_kv_head, int64_t head_dim, int64_t page_size, int64_t n_pages,
+                               void * data, size_t nbytes, b200_kv_cache * out);
+/* Frees what b200_kv_cache_alloc allocated (a view's memory stays). Waits for the device. */
+b200_status b200_kv_cache_free(b200_context * ctx, b200_kv_cache * cache);
+
+/* Writes n_tok rows per sequence: k, v float32 with row (s, r) at k + (s * n_tok + r) * ldk, heads [n_kv_head][head_dim]
+ * contiguous in it (ld >= n_kv_head * head_dim: a column range of a fused q|k|v product is written as it lies). */
+b200_status b200_kv_write(b200_context * ctx, void * stream, const b200_kv_cache * cache, const int32_t * table, int64_t max_pages,
+                          const int32_t * lens, int64_t n_seq, int64_t n_tok, const float * k, int64_t ldk, const float * v, int64_t ldv);
+/* Reads positions start[s] + r, r < n_tok, of each sequence (start int32 [n_seq] on the device, NULL: 0) that lie in
+ * [0, lens[s]) to k, v [n_seq][n_tok][n_kv_head][head_dim] of out_type B200_TYPE_F32 (exact) or B200_TYPE_F16 (rounded
+ * once); other rows are left as they were. Here lens is the sequences' lengths, independent of n_tok. */
+b200_status b200_kv_read(b200_context * ctx, void * stream, const b200_kv_cache * cache, const int32_t * table, int64_t max_pages,
+                         const int32_t * lens, const int32_t * start, int64_t n_seq, int64_t n_tok, int out_type, void * k, void * v);
+/* Attention of the n_tok (1 to 16) newest positions of each sequence, whose keys and values are already in the cache:
+ *   out[s][r][h] = sum_j softmax_j(scale * q[s][r][h] . k_j) v_j  over positions j <= lens[s] - n_tok + r,
+ * key/value head h / (n_head / n_kv_head). q float32 with row (s, r) at q + (s * n_tok + r) * ldq, heads [n_head][head_dim]
+ * contiguous in it; out float32 [n_seq][n_tok][n_head][head_dim]. Rows with no position to see (or whose scores are all
+ * -infinity) become zeros; what the cache holds past a row's last position does not reach it, NaN and infinities included.
+ * Unlike B200_OP_FLASH_ATTN (which rounds q to F16 as ggml does), q enters with 22 bits and sums are float32. workspace:
+ * device memory of b200_kv_attention_workspace bytes (256-byte aligned, contents arbitrary; NULL when that is 0), in use
+ * until the call's work is done: calls that may overlap on the GPU need one each. */
+size_t b200_kv_attention_workspace(b200_context * ctx, const b200_kv_cache * cache, int64_t max_pages, int64_t n_seq, int64_t n_tok,
+                                   int64_t n_head);
+b200_status b200_kv_attention(b200_context * ctx, void * stream, const b200_kv_cache * cache, const int32_t * table, int64_t max_pages,
+                              const int32_t * lens, int64_t n_seq, int64_t n_tok, int64_t n_head, const float * q, int64_t ldq, float scale,
+                              float * out, void * workspace, size_t workspace_bytes);
+
+/* ------------------------------------------------------------------------------------------------------------
+ * Expert router: the step between the router's product and b200_moe_ffn (softmax -> top_k -> get_rows -> renormalised
+ * weights in TextModel::experts, src/families/drama3/text-model.cpp:198-221), in the forms that mixture-of-experts models
+ * use. For each row of logits [T][n_expert]:
+ *   p = softmax(logits) or sigmoid(logits);  c = p + bias (bias float32 [n_expert], NULL: none);
+ *   with n_group > 1: experts lie in n_group equal runs, a group's score is the sum of its group_top (1 or 2) largest c,
+ *   and only the topk_group best groups' experts stay;
+ *   ids [T][top_k] = the top_k largest c, largest first; w [T][top_k] = their p, divided by their sum (renorm), times scale.
+ * p, c and their sums are double, rounded to float32 once in w; without bias and groups the experts are ordered by their
+ * logits. Ties go to the lowest index. A NaN logit or c counts as -infinity, a logit of -infinity has p = 0, +infinity shares the softmax with
+ * its equals; a sum of 0 gives weights 0.
+ * ------------------------------------------------------------------------------------------------------------ */
+enum { B200_ROUTER_SOFTMAX = 0, B200_ROUTER_SIGMOID = 1 };
+typedef struct b200_router {
+    int32_t n_expert;   /* 1 to 1024 */
+    int32_t top_k;      /* 1 to 32, at most the experts of topk_group groups */
+    int32_t score;      /* B200_ROUTER_* */
+    int32_t n_group;    /* 1, or a divisor of n_expert, at most 32 */
+    int32_t topk_group; /* 1 to n_group */
+    int32_t group_top;  /* 1 or 2 */
+    int32_t renorm;     /* != 0: divide by the sum of the chosen */
+    float scale;
+} b200_router;
+b200_status b200_moe_router(b200_context * ctx, void * stream, const b200_router * router, const float * logits, const float * bias,
+                            int64_t T, int32_t * ids, float * w);
+
+/* ------------------------------------------------------------------------------------------------------------
  * Host-buffer entry points (the end-to-end path a CPU caller takes: copies in, product, copy out, synchronous).
  * ------------------------------------------------------------------------------------------------------------ */
 b200_status b200_mul_mat_host(b200_context * ctx, const b200_weight * w, const float * x_host, int64_t M, float * dst_host);

@@ -37,6 +37,8 @@ EXPORTS = [
     "b200_ep_mailbox_alloc", "b200_ep_mailbox_open", "b200_ep_mailbox_close", "b200_ep_mailbox_free", "b200_ep_create",
     "b200_ep_destroy", "b200_ep_set_timeout", "b200_moe_ffn_ep", "b200_graph_compute", "b200_graph_supports",
     "b200_weight_prefetch_l2", "b200_ep_place",
+    "b200_kv_cache_nbytes", "b200_kv_cache_alloc", "b200_kv_cache_view", "b200_kv_cache_free", "b200_kv_write",
+    "b200_kv_read", "b200_kv_attention_workspace", "b200_kv_attention", "b200_moe_router",
 ]
 
 DEC_ATTN_Q, DEC_ATTN_K, DEC_ATTN_V, DEC_ATTN_O, DEC_FFN_GATE, DEC_FFN_UP, DEC_FFN_DOWN = range(7)
@@ -79,6 +81,28 @@ class Tensor(ctypes.Structure):
 I32 = 26
 (OP_NONE, OP_GET_ROWS, OP_MUL_MAT, OP_RMS_NORM, OP_MUL, OP_ADD, OP_ROPE, OP_SET_ROWS, OP_CPY, OP_CONT, OP_SOFT_MAX,
  OP_FLASH_ATTN, OP_SWIGLU, OP_ARGMAX, OP_SCALE, OP_FILL, OP_CONCAT) = range(17)
+
+
+class KvCacheStruct(ctypes.Structure):
+    """struct b200_kv_cache (include/b200.h)."""
+
+    _fields_ = [
+        ("type", ctypes.c_int32), ("device", ctypes.c_int32), ("n_kv_head", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32), ("owned", ctypes.c_int32), ("n_pages", ctypes.c_int64), ("data", ctypes.c_void_p),
+        ("nbytes", ctypes.c_size_t), ("field_off", ctypes.c_int64 * 4),
+    ]
+
+
+ROUTER_SOFTMAX, ROUTER_SIGMOID = 0, 1
+
+
+class Router(ctypes.Structure):
+    """struct b200_router (include/b200.h)."""
+
+    _fields_ = [
+        ("n_expert", ctypes.c_int32), ("top_k", ctypes.c_int32), ("score", ctypes.c_int32), ("n_group", ctypes.c_int32),
+        ("topk_group", ctypes.c_int32), ("group_top", ctypes.c_int32), ("renorm", ctypes.c_int32), ("scale", ctypes.c_float),
+    ]
 
 
 class EpPlan(ctypes.Structure):
@@ -135,6 +159,7 @@ def lib():
     L = ctypes.CDLL(LIB_PATH)
     vp, i64, i32, sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
     W = ctypes.POINTER(Weight)
+    KV = ctypes.POINTER(KvCacheStruct)
     sig = {
         "b200_device_count": (i32, []),
         "b200_device_info": (i32, [i32, ctypes.c_char_p, sz, ctypes.POINTER(sz), ctypes.POINTER(sz)]),
@@ -183,6 +208,15 @@ def lib():
         "b200_ep_place": (i32, [ctypes.c_int, ctypes.POINTER(sz), ctypes.c_int, ctypes.POINTER(ctypes.c_uint64), ctypes.c_int,
                                 ctypes.c_uint64, ctypes.POINTER(EpPlan)]),
         "b200_graph_supports": (i32, [ctypes.POINTER(Tensor), i64, i64]),
+        "b200_kv_cache_nbytes": (sz, [i32, i64, i64, i64, i64]),
+        "b200_kv_cache_alloc": (i32, [vp, i32, i64, i64, i64, i64, KV]),
+        "b200_kv_cache_view": (i32, [vp, i32, i64, i64, i64, i64, vp, sz, KV]),
+        "b200_kv_cache_free": (i32, [vp, KV]),
+        "b200_kv_write": (i32, [vp, vp, KV, vp, i64, vp, i64, i64, vp, i64, vp, i64]),
+        "b200_kv_read": (i32, [vp, vp, KV, vp, i64, vp, vp, i64, i64, i32, vp, vp]),
+        "b200_kv_attention_workspace": (sz, [vp, KV, i64, i64, i64, i64]),
+        "b200_kv_attention": (i32, [vp, vp, KV, vp, i64, vp, i64, i64, i64, vp, i64, ctypes.c_float, vp, vp, sz]),
+        "b200_moe_router": (i32, [vp, vp, ctypes.POINTER(Router), vp, vp, i64, vp, vp]),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)
@@ -398,6 +432,134 @@ class Context:
         self._sync_out()
         return out
 
+    # -- paged key/value cache and expert router (torch CUDA tensors; run on torch's current stream) ------------------
+    def _stream(self):
+        """torch's current stream of this device as a cudaStream_t (the default stream as cudaStreamLegacy, since NULL
+        means the context's own stream). These calls use nothing of the context's stream, so they run in torch's order."""
+        import torch
+
+        return torch.cuda.current_stream(self.device).cuda_stream or 1
+
+    def _arg(self, t, what, dtype, shape=None):
+        """The address of a contiguous CUDA tensor of this device, type and shape."""
+        if not t.is_cuda or t.device.index != self.device:
+            raise ValueError(f"{what}: expected a tensor on cuda:{self.device}, got one on {t.device}")
+        if t.dtype != dtype or (shape is not None and t.shape != shape) or not t.is_contiguous():
+            raise ValueError(f"{what}: expected a contiguous {dtype} tensor{'' if shape is None else f' of shape {tuple(shape)}'}, "
+                             f"got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+        return t.data_ptr()
+
+    def _row_arg(self, t, what, heads, dim):
+        """(address, row stride) of float32 rows [n_seq, n_tok, heads, dim] whose heads lie contiguous in each row and whose
+        rows lie at one stride (a slice of the columns of a wider product is taken as it is)."""
+        import torch
+
+        if not t.is_cuda or t.device.index != self.device:
+            raise ValueError(f"{what}: expected a tensor on cuda:{self.device}, got one on {t.device}")
+        if t.dtype != torch.float32 or t.dim() != 4 or t.shape[2] != heads or t.shape[3] != dim:
+            raise ValueError(f"{what}: expected float32 [n_seq, n_tok, {heads}, {dim}], got {t.dtype} {tuple(t.shape)}")
+        n_seq, n_tok = t.shape[:2]
+        s = t.stride()
+        ld = s[1] if n_tok > 1 else s[0] if n_seq > 1 else heads * dim
+        if t.numel() and (s[3] != 1 or (heads > 1 and s[2] != dim) or ld < heads * dim or (n_seq > 1 and s[0] != n_tok * ld)):
+            raise ValueError(f"{what}: the rows' heads are not contiguous or the rows lie at no single stride (strides {s})")
+        return t.data_ptr(), max(ld, heads * dim)
+
+    def kv_cache(self, qtype, n_kv_head, head_dim, page_size, n_pages, data=None):
+        """A paged key/value cache of type F16 or Q8_0 (b200_kv_cache); data: a CUDA uint8 tensor to lay it out in
+        (kept as it is), else its memory is allocated and zeroed."""
+        return KvCache(self, qtype, n_kv_head, head_dim, page_size, n_pages, data)
+
+    def _kv_open(self, cache, what):
+        if cache.ctx is not self or not cache.s.n_pages:
+            raise ValueError(f"{what}: the cache is closed or belongs to another context")
+
+    def _kv_places(self, cache, table, lens, n_seq, what):
+        import torch
+
+        if table.dim() != 2:
+            raise ValueError(f"{what}: expected a table [n_seq, max_pages], got {tuple(table.shape)}")
+        return self._arg(table, what + " table", torch.int32, (n_seq, table.shape[1])), table.shape[1], self._arg(lens, what + " lens", torch.int32, (n_seq,))
+
+    def kv_write(self, cache, k, v, table, lens):
+        """Writes rows k, v float32 [n_seq, n_tok, n_kv_head, head_dim] at positions lens[s] - n_tok + r (b200_kv_write);
+        table int32 [n_seq, max_pages], lens int32 [n_seq] (the lengths with these rows)."""
+        self._kv_open(cache, "kv_write")
+        kp, ldk = self._row_arg(k, "kv_write k", cache.s.n_kv_head, cache.s.head_dim)
+        vp, ldv = self._row_arg(v, "kv_write v", cache.s.n_kv_head, cache.s.head_dim)
+        n_seq, n_tok = k.shape[:2]
+        if v.shape != k.shape:
+            raise ValueError(f"kv_write: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+        tp, mp, lp = self._kv_places(cache, table, lens, n_seq, "kv_write")
+        self.check(self.L.b200_kv_write(self.h, self._stream(), cache.ref, tp, mp, lp, n_seq, n_tok, kp, ldk, vp, ldv))
+
+    def kv_read(self, cache, table, lens, n_tok=None, start=None, dtype=None, k=None, v=None):
+        """Positions start[s] + r (start int32 [n_seq], None: 0), r < n_tok, below lens[s] as float32 or float16 rows
+        [n_seq, n_tok, n_kv_head, head_dim] (b200_kv_read). k, v: tensors to fill, whose other rows stay as they are;
+        without them zeroed tensors are made."""
+        import torch
+
+        self._kv_open(cache, "kv_read")
+        n_seq = lens.shape[0]
+        if (k is None) != (v is None) or (k is None and n_tok is None):
+            raise ValueError("kv_read: give both k and v, or n_tok")
+        if k is None:
+            shape = (n_seq, n_tok, cache.s.n_kv_head, cache.s.head_dim)
+            k, v = (torch.zeros(shape, dtype=dtype or torch.float32, device=lens.device) for _ in range(2))
+        else:
+            n_tok = k.shape[1] if n_tok is None else n_tok
+            shape = (n_seq, n_tok, cache.s.n_kv_head, cache.s.head_dim)
+            if dtype is not None and dtype != k.dtype:
+                raise ValueError(f"kv_read: k is {k.dtype}, not {dtype}")
+        if k.dtype not in (torch.float32, torch.float16):
+            raise ValueError(f"kv_read: rows are float32 or float16, not {k.dtype}")
+        kp, vp = self._arg(k, "kv_read k", k.dtype, shape), self._arg(v, "kv_read v", k.dtype, shape)
+        sp = None if start is None else self._arg(start, "kv_read start", torch.int32, (n_seq,))
+        tp, mp, lp = self._kv_places(cache, table, lens, n_seq, "kv_read")
+        self.check(self.L.b200_kv_read(self.h, self._stream(), cache.ref, tp, mp, lp, sp, n_seq, n_tok, F16 if k.dtype == torch.float16 else F32, kp, vp))
+        return k, v
+
+    def kv_attention(self, cache, q, table, lens, scale, out=None):
+        """Attention of the n_tok newest positions of each sequence over the cache (b200_kv_attention): q float32
+        [n_seq, n_tok, n_head, head_dim] -> float32 of the same shape."""
+        import torch
+
+        self._kv_open(cache, "kv_attention")
+        if q.dim() != 4:
+            raise ValueError(f"kv_attention: expected q [n_seq, n_tok, n_head, head_dim], got {tuple(q.shape)}")
+        n_seq, n_tok, n_head, dim = q.shape
+        qp, ldq = self._row_arg(q, "kv_attention q", n_head, cache.s.head_dim)
+        tp, mp, lp = self._kv_places(cache, table, lens, n_seq, "kv_attention")
+        if out is None:
+            out = torch.empty((n_seq, n_tok, n_head, dim), dtype=torch.float32, device=q.device)
+        op = self._arg(out, "kv_attention out", torch.float32, q.shape)
+        size = self.L.b200_kv_attention_workspace(self.h, cache.ref, mp, n_seq, n_tok, n_head)
+        # the workspace comes from torch's allocator: reused in stream order, and a captured graph has its own
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        self.check(self.L.b200_kv_attention(self.h, self._stream(), cache.ref, tp, mp, lp, n_seq, n_tok, n_head, qp, ldq, scale, op,
+                                            ws.data_ptr() if size else None, size))
+        return out
+
+    def moe_router(self, logits, top_k, bias=None, score="softmax", n_group=1, topk_group=1, group_top=1, renorm=True, scale=1.0, ids=None,
+                   w=None):
+        """The experts of each row of logits float32 [T, n_expert] and their weights (b200_moe_router): ids int32 and w
+        float32 [T, top_k], as moe_ffn takes them. score: "softmax" or "sigmoid"; bias: float32 [n_expert]."""
+        import torch
+
+        if score not in ("softmax", "sigmoid"):
+            raise ValueError(f"moe_router: unknown score {score!r}")
+        if logits.dim() != 2:
+            raise ValueError(f"moe_router: expected logits [T, n_expert], got {tuple(logits.shape)}")
+        T, E = logits.shape
+        lp = self._arg(logits, "moe_router logits", torch.float32)
+        bp = None if bias is None else self._arg(bias, "moe_router bias", torch.float32, (E,))
+        r = Router(E, top_k, ROUTER_SIGMOID if score == "sigmoid" else ROUTER_SOFTMAX, n_group, topk_group, group_top, bool(renorm), scale)
+        ids = torch.empty((T, top_k), dtype=torch.int32, device=logits.device) if ids is None else ids
+        w = torch.empty((T, top_k), dtype=torch.float32, device=logits.device) if w is None else w
+        ip, wp = self._arg(ids, "moe_router ids", torch.int32, (T, top_k)), self._arg(w, "moe_router w", torch.float32, (T, top_k))
+        self.check(self.L.b200_moe_router(self.h, self._stream(), ctypes.byref(r), lp, bp, T, ip, wp))
+        return ids, w
+
     def mul_mat_host(self, w, x):
         """End-to-end host path: numpy float32 [M, K] -> numpy [M, N] (copies inside the call)."""
         import numpy as np
@@ -407,6 +569,41 @@ class Context:
         self.check(self.L.b200_mul_mat_host(self.h, ctypes.byref(w), x.ctypes.data_as(ctypes.c_void_p), x.shape[0],
                                             out.ctypes.data_as(ctypes.c_void_p)))
         return out
+
+
+class KvCache:
+    """A paged key/value cache (b200_kv_cache) of one layer: see Context.kv_cache, kv_write, kv_read, kv_attention."""
+
+    def __init__(self, ctx, qtype, n_kv_head, head_dim, page_size, n_pages, data=None):
+        self.ctx = ctx
+        self.s = KvCacheStruct()
+        self.ref = ctypes.byref(self.s)
+        self.data = data  # a view keeps its memory
+        if data is None:
+            ctx.check(ctx.L.b200_kv_cache_alloc(ctx.h, qtype, n_kv_head, head_dim, page_size, n_pages, self.ref))
+        else:
+            import torch
+
+            ctx.check(ctx.L.b200_kv_cache_view(ctx.h, qtype, n_kv_head, head_dim, page_size, n_pages, ctx._arg(data, "kv_cache data", torch.uint8),
+                                               data.numel(), self.ref))
+        ctx._children.add(self)
+
+    @property
+    def nbytes(self):
+        return self.s.nbytes
+
+    def close(self):
+        # the cache's memory is freed while its context is alive (the context closes its caches first)
+        if self.s.data and getattr(self.ctx, "h", None):
+            self.ctx.check(self.ctx.L.b200_kv_cache_free(self.ctx.h, self.ref))
+        self.s.data, self.s.n_pages = None, 0
+        self.data = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class Graph:

@@ -338,7 +338,8 @@ b200_status b200_synchronize(b200_context * ctx) {
         CK(ctx, cudaStreamSynchronize(ctx->stream));
         if (bits & B200_DEVERR_TIMEOUT) return fail(ctx, B200_ERR_TIMEOUT, "a bounded device wait gave up");
         if (bits & B200_DEVERR_EXPERT) return fail(ctx, B200_ERR_RANGE, "mul_mat_id: an expert id is outside [0, E)");
-        return fail(ctx, B200_ERR_RANGE, "get_rows: a row id is outside the table");
+        if (bits & B200_DEVERR_ROWS) return fail(ctx, B200_ERR_RANGE, "get_rows: a row id is outside the table");
+        return fail(ctx, B200_ERR_RANGE, "kv cache: a page number or a sequence length is outside its range");
     }
     return B200_OK;
 }

@@ -15,6 +15,7 @@
 #define B200_DEVERR_ROWS 1u     // GET_ROWS id out of range
 #define B200_DEVERR_EXPERT 2u   // MUL_MAT_ID id out of range
 #define B200_DEVERR_TIMEOUT 4u  // a bounded wait gave up
+#define B200_DEVERR_PAGE 8u     // a paged cache's page number or sequence length out of range
 
 // An expert-parallel group's view of every rank's mailbox (peer.cu): inbox [G][ceil(T_max / G)][H] float, final
 // [T_max][H] float, two arrival counters; peer[g] is rank g's mailbox mapped into this process (peer[rank] its own).
@@ -60,6 +61,22 @@ struct b200_context {
     // Expanded copies of K-quant weights used with many activation rows, by weight data pointer; dropped when the
     // weight is written or freed.
     std::unordered_map<const void *, KqExpansion> kq;
+};
+
+// Makes `device` current for a scope (a call on a context whose device is not the caller's current one).
+struct DeviceScope {
+    int prev = -1;
+    cudaError_t status;
+    explicit DeviceScope(int device) {
+        status = cudaGetDevice(&prev);
+        if (status == cudaSuccess && prev != device) status = cudaSetDevice(device);
+        else prev = -1;
+    }
+    ~DeviceScope() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+    DeviceScope(const DeviceScope &) = delete;
+    DeviceScope & operator=(const DeviceScope &) = delete;
 };
 
 namespace b200 {

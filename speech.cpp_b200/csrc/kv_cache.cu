@@ -1,0 +1,293 @@
+// kv_cache.cu — the paged key/value cache: its memory, and the kernels that write and read its rows
+// (b200_kv_cache_*, b200_kv_write, b200_kv_read, include/b200.h).
+//
+// The reference's cache is one dense F16 tensor per request, written with SET_ROWS (src/common/qwen3-decoder.cpp:300-346);
+// here sequences share a pool of pages, and Q8_0 halves the bytes that attention streams.
+//
+// Both kernels are copies with a conversion: one CTA per row (sequence, token), so the length and the page number are read
+// once, and its threads walk the row's k then v values four at a time, all of a row's heads contiguous on the float side
+// and 64 to 512 contiguous bytes per head on the page's side. They are bound by HBM (4 B per value on the float side, 2 or
+// 34/32 B in the cache), or by launch latency for the rows of a decode step.
+#include <cstdio>
+
+#include "kv.cuh"
+
+using namespace b200;
+
+namespace b200 {
+
+b200_status kv_fail(b200_context * ctx, b200_status s, const char * what, const char * why) {
+    const std::string text = std::string(what) + ": " + why;
+    if (ctx) ctx->last_error = text;
+    else set_thread_error(text.c_str());
+    return s;
+}
+
+b200_status kv_cuda(b200_context * ctx, cudaError_t e, const char * what) {
+    return e == cudaSuccess ? B200_OK : kv_fail(ctx, e == cudaErrorMemoryAllocation ? B200_ERR_ALLOC : B200_ERR_DEVICE, what, cudaGetErrorString(e));
+}
+
+b200_status kv_checked_view(b200_context * ctx, const char * what, const b200_kv_cache * c, const int32_t * table, int64_t max_pages,
+                            const int32_t * lens, int64_t n_seq, int64_t n_tok, KvView * out) {
+    if (!ctx) return kv_fail(ctx, B200_ERR_INVALID, what, "NULL context");
+    if (!c || !c->data || c->nbytes < b200_kv_cache_nbytes(c->type, c->n_kv_head, c->head_dim, c->page_size, c->n_pages) || c->nbytes == 0)
+        return kv_fail(ctx, B200_ERR_INVALID, what, "not a cache");
+    if (c->device != ctx->device) return kv_fail(ctx, B200_ERR_INVALID, what, "the cache lies on another device than the context");
+    if (n_seq < 0 || n_tok < 0 || max_pages < 0) return kv_fail(ctx, B200_ERR_INVALID, what, "a negative size");
+    if (n_seq > 0 && n_tok > 0 && (!lens || (max_pages > 0 && !table))) return kv_fail(ctx, B200_ERR_INVALID, what, "NULL table or lens");
+    if (max_pages > INT32_MAX / c->page_size) return kv_fail(ctx, B200_ERR_INVALID, what, "max_pages * page_size passes 2^31");
+    // one CTA per row (or fewer) in a one-dimensional grid
+    if (n_tok > 0 && n_seq > INT32_MAX / n_tok) return kv_fail(ctx, B200_ERR_INVALID, what, "n_seq * n_tok passes 2^31");
+    const uint8_t * base = (const uint8_t *) c->data;
+    out->k = base + c->field_off[0];
+    out->v = base + c->field_off[1];
+    out->kd = (const __half *) (base + c->field_off[2]);
+    out->vd = (const __half *) (base + c->field_off[3]);
+    out->n_kv_head = c->n_kv_head;
+    out->head_dim = c->head_dim;
+    out->page_size = c->page_size;
+    out->n_pages = c->n_pages;
+    out->table = table;
+    out->lens = lens;
+    out->max_pages = max_pages;
+    out->err = ctx->dev_err;
+    return B200_OK;
+}
+
+}  // namespace b200
+
+namespace {
+
+// Bytes of the arrays k (and v) and of the scales of k (and v); false when the cache is not one that is supported.
+bool kv_sizes(int type, int64_t heads, int64_t dim, int64_t page, int64_t pages, int64_t * values, int64_t * scales) {
+    if (type != B200_TYPE_F16 && type != B200_TYPE_Q8_0) return false;
+    if (dim != 64 && dim != 96 && dim != 128 && dim != 256) return false;
+    if (heads <= 0 || heads > 65535 || page <= 0 || page % 16 || page > 4096 || pages <= 0 || pages > INT32_MAX) return false;
+    const int64_t rows = heads * page;  // at most 2^28
+    if (pages > ((int64_t) 1 << 52) / (rows * dim)) return false;
+    *values = pages * rows * dim * (type == B200_TYPE_F16 ? 2 : 1);
+    *scales = type == B200_TYPE_F16 ? 0 : pages * rows * (dim / 32) * 2;
+    return true;
+}
+
+// Four float32 values at p (16-byte aligned when VEC).
+template <bool VEC>
+__device__ __forceinline__ float4 load4(const float * p) {
+    if constexpr (VEC) return *reinterpret_cast<const float4 *>(p);
+    return make_float4(p[0], p[1], p[2], p[3]);
+}
+
+__device__ __forceinline__ uint2 pack4(float4 v) {
+    const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+    return make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
+}
+
+// Row (s, r) of k and v to its slot. Q8_0: eight lanes hold a block's 32 values (quantize_q8_0_quad), so the warp's lanes
+// all take part in every step, those past the row's end on its last values without storing.
+template <bool Q8, bool VEC>
+__global__ void kv_write_kernel(KvView c, int64_t n_tok, const float * __restrict__ k, int64_t ldk, const float * __restrict__ v, int64_t ldv) {
+    const int64_t row = blockIdx.x, s = row / n_tok, r = row % n_tok;
+    const int64_t pos = kv_len(c, s, threadIdx.x == 0) - n_tok + r;
+    if (pos < 0) return;
+    const int page = kv_page(c, s, pos / c.page_size, threadIdx.x == 0);
+    if (page < 0) return;
+    const int slot = (int) (pos % c.page_size);
+    const int quads = c.n_kv_head * c.head_dim / 4;  // of k, and of v
+    for (int i0 = threadIdx.x & ~31; i0 < 2 * quads; i0 += blockDim.x) {
+        const int j = i0 + (threadIdx.x & 31);
+        const bool here = j < 2 * quads;
+        const int i = here ? j : 2 * quads - 1;
+        const bool is_v = i >= quads;
+        const int e = (is_v ? i - quads : i) * 4;  // element in the row
+        const int h = e / c.head_dim, d = e % c.head_dim;
+        const float4 x = load4<VEC>(is_v ? v + row * ldv + e : k + row * ldk + e);
+        const int64_t at = ((int64_t) page * c.n_kv_head + h) * c.page_size + slot;
+        uint8_t * to = const_cast<uint8_t *>(is_v ? c.v : c.k);
+        if constexpr (Q8) {
+            float df;
+            const uint32_t q = quantize_q8_0_quad(x, &df);
+            if (here) {
+                *reinterpret_cast<uint32_t *>(to + at * c.head_dim + d) = q;
+                if ((i & 7) == 0) const_cast<__half *>(is_v ? c.vd : c.kd)[at * (c.head_dim / 32) + d / 32] = __float2half_rn(df);
+            }
+        } else if (here) {
+            *reinterpret_cast<uint2 *>(to + (at * c.head_dim + d) * 2) = pack4(x);
+        }
+    }
+}
+
+// Position start[s] + r to row (s, r) of k and v.
+template <bool Q8, bool HALF, bool VEC>
+__global__ void kv_read_kernel(KvView c, const int32_t * __restrict__ start, int64_t n_tok, void * __restrict__ k, void * __restrict__ v) {
+    const int64_t row = blockIdx.x, s = row / n_tok, r = row % n_tok;
+    const int64_t len = kv_len(c, s, threadIdx.x == 0);
+    const int64_t pos = (start ? (int64_t) start[s] : 0) + r;
+    if (pos < 0 || pos >= len) return;
+    const int page = kv_page(c, s, pos / c.page_size, threadIdx.x == 0);
+    if (page < 0) return;
+    const int slot = (int) (pos % c.page_size);
+    const int quads = c.n_kv_head * c.head_dim / 4;
+    for (int i = threadIdx.x; i < 2 * quads; i += blockDim.x) {
+        const bool is_v = i >= quads;
+        const int e = (is_v ? i - quads : i) * 4;
+        const int h = e / c.head_dim, d = e % c.head_dim;
+        const int64_t at = ((int64_t) page * c.n_kv_head + h) * c.page_size + slot;
+        const uint8_t * from = is_v ? c.v : c.k;
+        const int64_t o = row * 4 * quads + e;
+        void * out = is_v ? v : k;
+        float4 x;
+        if constexpr (Q8) {
+            const char4 q = *reinterpret_cast<const char4 *>(from + at * c.head_dim + d);
+            const float f = __half2float((is_v ? c.vd : c.kd)[at * (c.head_dim / 32) + d / 32]);
+            x = make_float4(__fmul_rn(f, (float) q.x), __fmul_rn(f, (float) q.y), __fmul_rn(f, (float) q.z), __fmul_rn(f, (float) q.w));
+        } else {
+            const uint2 u = *reinterpret_cast<const uint2 *>(from + (at * c.head_dim + d) * 2);
+            const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
+            x = make_float4(a.x, a.y, b.x, b.y);
+        }
+        if constexpr (HALF) {
+            const uint2 u = pack4(x);
+            if constexpr (VEC) {
+                *reinterpret_cast<uint2 *>((__half *) out + o) = u;
+            } else {
+                uint16_t * p = (uint16_t *) out + o;
+                p[0] = (uint16_t) u.x, p[1] = (uint16_t) (u.x >> 16), p[2] = (uint16_t) u.y, p[3] = (uint16_t) (u.y >> 16);
+            }
+        } else if constexpr (VEC) {
+            *reinterpret_cast<float4 *>((float *) out + o) = x;
+        } else {
+            float * p = (float *) out + o;
+            p[0] = x.x, p[1] = x.y, p[2] = x.z, p[3] = x.w;
+        }
+    }
+}
+
+// Threads of a row's CTA: one per four values, at most 512.
+unsigned row_threads(const KvView & c) {
+    const int quads = c.n_kv_head * c.head_dim / 2;  // of k and v together
+    return (unsigned) (quads >= 512 ? 512 : (quads + 31) & ~31);
+}
+
+bool aligned(const void * p, size_t to) { return ((uintptr_t) p & (to - 1)) == 0; }
+
+}  // namespace
+
+extern "C" {
+
+size_t b200_kv_cache_nbytes(int type, int64_t n_kv_head, int64_t head_dim, int64_t page_size, int64_t n_pages) {
+    int64_t values, scales;
+    if (!kv_sizes(type, n_kv_head, head_dim, page_size, n_pages, &values, &scales)) return 0;
+    return (size_t) (2 * align256(values) + 2 * align256(scales));
+}
+
+b200_status b200_kv_cache_view(b200_context * ctx, int type, int64_t n_kv_head, int64_t head_dim, int64_t page_size, int64_t n_pages,
+                               void * data, size_t nbytes, b200_kv_cache * out) {
+    if (!out) return kv_fail(ctx, B200_ERR_INVALID, "kv_cache_view", "NULL argument");
+    std::memset(out, 0, sizeof *out);
+    if (!ctx || !data) return kv_fail(ctx, B200_ERR_INVALID, "kv_cache_view", "NULL argument");
+    int64_t values, scales;
+    if (!kv_sizes(type, n_kv_head, head_dim, page_size, n_pages, &values, &scales))
+        return kv_fail(ctx, B200_ERR_UNSUPPORTED, "kv_cache_view",
+                       "needs F16 or Q8_0, head_dim 64, 96, 128 or 256, page_size a multiple of 16 up to 4096");
+    if (!aligned(data, 16)) return kv_fail(ctx, B200_ERR_INVALID, "kv_cache_view", "data is not 16-byte aligned");
+    const size_t need = b200_kv_cache_nbytes(type, n_kv_head, head_dim, page_size, n_pages);
+    if (nbytes < need) return kv_fail(ctx, B200_ERR_INVALID, "kv_cache_view", "too few bytes");
+    out->type = type;
+    out->device = ctx->device;
+    out->n_kv_head = (int32_t) n_kv_head;
+    out->head_dim = (int32_t) head_dim;
+    out->page_size = (int32_t) page_size;
+    out->n_pages = n_pages;
+    out->data = data;
+    out->nbytes = need;
+    out->field_off[1] = align256(values);
+    out->field_off[2] = 2 * align256(values);
+    out->field_off[3] = 2 * align256(values) + align256(scales);
+    return B200_OK;
+}
+
+b200_status b200_kv_cache_alloc(b200_context * ctx, int type, int64_t n_kv_head, int64_t head_dim, int64_t page_size, int64_t n_pages,
+                                b200_kv_cache * out) {
+    if (!out) return kv_fail(ctx, B200_ERR_INVALID, "kv_cache_alloc", "NULL argument");
+    std::memset(out, 0, sizeof *out);
+    if (!ctx) return kv_fail(ctx, B200_ERR_INVALID, "kv_cache_alloc", "NULL argument");
+    const size_t need = b200_kv_cache_nbytes(type, n_kv_head, head_dim, page_size, n_pages);
+    if (!need)
+        return kv_fail(ctx, B200_ERR_UNSUPPORTED, "kv_cache_alloc",
+                       "needs F16 or Q8_0, head_dim 64, 96, 128 or 256, page_size a multiple of 16 up to 4096");
+    DeviceScope scope(ctx->device);
+    if (scope.status != cudaSuccess) return kv_cuda(ctx, scope.status, "kv_cache_alloc");
+    void * p = nullptr;
+    cudaError_t e = cudaMalloc(&p, need);
+    if (e != cudaSuccess) {
+        cudaGetLastError();  // an allocation that failed is reported here, not by the next launch
+        return kv_cuda(ctx, e, "kv_cache_alloc");
+    }
+    e = cudaMemsetAsync(p, 0, need, ctx->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);  // zero for calls on every stream
+    if (e != cudaSuccess) {
+        cudaFree(p);
+        return kv_cuda(ctx, e, "kv_cache_alloc");
+    }
+    const b200_status s = b200_kv_cache_view(ctx, type, n_kv_head, head_dim, page_size, n_pages, p, need, out);
+    if (s != B200_OK) cudaFree(p);
+    else out->owned = 1;
+    return s;
+}
+
+b200_status b200_kv_cache_free(b200_context * ctx, b200_kv_cache * cache) {
+    if (!ctx || !cache) return kv_fail(ctx, B200_ERR_INVALID, "kv_cache_free", "NULL argument");
+    DeviceScope scope(ctx->device);
+    cudaError_t e = scope.status;
+    if (e == cudaSuccess && cache->data && cache->owned) e = cudaFree(cache->data);
+    std::memset(cache, 0, sizeof *cache);
+    return kv_cuda(ctx, e, "kv_cache_free");
+}
+
+b200_status b200_kv_write(b200_context * ctx, void * stream, const b200_kv_cache * cache, const int32_t * table, int64_t max_pages,
+                          const int32_t * lens, int64_t n_seq, int64_t n_tok, const float * k, int64_t ldk, const float * v, int64_t ldv) {
+    KvView c;
+    const b200_status s = kv_checked_view(ctx, "kv_write", cache, table, max_pages, lens, n_seq, n_tok, &c);
+    if (s != B200_OK) return s;
+    if (n_seq == 0 || n_tok == 0) return B200_OK;
+    const int64_t width = (int64_t) c.n_kv_head * c.head_dim;
+    if (!k || !v || !aligned(k, 4) || !aligned(v, 4)) return kv_fail(ctx, B200_ERR_INVALID, "kv_write", "NULL or misaligned k or v");
+    if (ldk < width || ldv < width) return kv_fail(ctx, B200_ERR_INVALID, "kv_write", "a row stride is below n_kv_head * head_dim");
+    DeviceScope scope(ctx->device);
+    if (scope.status != cudaSuccess) return kv_cuda(ctx, scope.status, "kv_write");
+    const bool vec = aligned(k, 16) && aligned(v, 16) && ldk % 4 == 0 && ldv % 4 == 0;
+    const unsigned grid = (unsigned) (n_seq * n_tok), threads = row_threads(c);
+    cudaStream_t st = stream ? (cudaStream_t) stream : ctx->stream;
+    auto kern = cache->type == B200_TYPE_Q8_0 ? (vec ? kv_write_kernel<true, true> : kv_write_kernel<true, false>)
+                                              : (vec ? kv_write_kernel<false, true> : kv_write_kernel<false, false>);
+    kern<<<grid, threads, 0, st>>>(c, n_tok, k, ldk, v, ldv);
+    return kv_cuda(ctx, cudaGetLastError(), "kv_write");
+}
+
+b200_status b200_kv_read(b200_context * ctx, void * stream, const b200_kv_cache * cache, const int32_t * table, int64_t max_pages,
+                         const int32_t * lens, const int32_t * start, int64_t n_seq, int64_t n_tok, int out_type, void * k, void * v) {
+    KvView c;
+    const b200_status s = kv_checked_view(ctx, "kv_read", cache, table, max_pages, lens, n_seq, n_tok, &c);
+    if (s != B200_OK) return s;
+    if (out_type != B200_TYPE_F32 && out_type != B200_TYPE_F16) return kv_fail(ctx, B200_ERR_UNSUPPORTED, "kv_read", "rows are read as F32 or F16");
+    if (n_seq == 0 || n_tok == 0) return B200_OK;
+    const size_t elem = out_type == B200_TYPE_F16 ? 2 : 4;
+    if (!k || !v || !aligned(k, elem) || !aligned(v, elem)) return kv_fail(ctx, B200_ERR_INVALID, "kv_read", "NULL or misaligned k or v");
+    DeviceScope scope(ctx->device);
+    if (scope.status != cudaSuccess) return kv_cuda(ctx, scope.status, "kv_read");
+    const bool vec = aligned(k, 4 * elem) && aligned(v, 4 * elem);
+    const unsigned grid = (unsigned) (n_seq * n_tok), threads = row_threads(c);
+    cudaStream_t st = stream ? (cudaStream_t) stream : ctx->stream;
+    auto pick = [&](auto q8, auto half) {
+        constexpr bool Q8 = decltype(q8)::value, HALF = decltype(half)::value;
+        if (vec) kv_read_kernel<Q8, HALF, true><<<grid, threads, 0, st>>>(c, start, n_tok, k, v);
+        else kv_read_kernel<Q8, HALF, false><<<grid, threads, 0, st>>>(c, start, n_tok, k, v);
+    };
+    using std::true_type;
+    using std::false_type;
+    if (cache->type == B200_TYPE_Q8_0) elem == 2 ? pick(true_type{}, true_type{}) : pick(true_type{}, false_type{});
+    else elem == 2 ? pick(false_type{}, true_type{}) : pick(false_type{}, false_type{});
+    return kv_cuda(ctx, cudaGetLastError(), "kv_read");
+}
+
+}  // extern "C"
