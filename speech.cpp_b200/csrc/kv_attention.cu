@@ -1,8 +1,31 @@
 // kv_attention.cu — attention of a few new tokens per sequence over the paged key/value cache (b200_kv_attention).
 //
-// One CTA per (sequence, row, head) walks the positions that its row sees in chunks of one position per thread: scores from
-// a dot product per thread, a running maximum and sum (of exponentials to base e), and the output's dimensions one per
-// thread. All in float32.
+// Mathematics. The rows of one key/value head (its group of query heads, times the call's tokens) share every key and value,
+// so they are taken eight at a time: S = Q K^T and O = P V over 16 positions at a time, with a running maximum and sum per
+// row (o and l are rescaled by 2^(m_old - m_new) when a larger score appears; exponentials to base 2, their scale folded into
+// the scores'). Bytes decide: a position costs 4 D bytes (F16) or 2.125 D (Q8_0) of HBM and 4 D multiply-adds per row, so
+// the arithmetic has to cost next to nothing beside the stream of the cache.
+//
+// Float32 results from F16 matrix instructions. mma.m16n8k16 multiplies F16 exactly and adds in float32, but takes 16 rows
+// where there are at most eight: rows 0-7 of the tile hold the high half of the operand and rows 8-15 the low half (x = hi +
+// lo in F16, 22 bits; q scaled by a power of two per row first), and the two results of a row lie in the same lane's
+// registers, where one addition joins them. So q and the weights enter with 22 bits at the price of the padding. Q8_0's
+// values are whole numbers and exact in F16; their scales stay outside: a key block's multiplies its partial score, a value
+// block's multiplies the weight before it is split (times a power of two per 16 positions that keeps it in F16's range).
+// Each instruction's sum starts at zero and is added to the float32 result with an ordinary rounded addition (the
+// instruction's own accumulation truncates, which over thousands of positions would add up).
+//
+// Operands without shared memory. The k index of S = Q K^T may run through a row's dimensions in any order that both operands
+// share, and the n index of O = P V through any order that the output is written back in. They are chosen such that a lane's
+// fragment is 16 (F16 keys and values), 8 or 4 (Q8_0) contiguous bytes of a row: keys and values go from HBM to the matrix
+// instruction's registers with wide loads that use every byte of each sector, and the scores' registers are the weights'
+// fragment as they stand.
+//
+// Split. Sequences differ in length and there may be one of them, so the work is cut by positions: all (sequence, key/value
+// head, row tile) items laid end to end in chunks of 64 positions, and each CTA takes an equal run of chunks. A CTA's four
+// warps take turns at 16-position tiles of a run and join at its end. Items that lie within one CTA's run are finished by it;
+// of the others each CTA leaves a partial (m, l, o) in the workspace, and a second kernel, launched with programmatic
+// dependent launch, joins them.
 #include <cmath>
 
 #include "kv.cuh"
@@ -11,55 +34,504 @@ using namespace b200;
 
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kRows = 8;      // rows of a tile
+constexpr int kChunk = 64;    // positions of a chunk: one 16-position tile per warp
+constexpr float kShift = 15;  // weights are held times 2^15, so that their low halves reach 2^-39 of the largest
 
-__device__ __forceinline__ float value(const uint8_t * data, const __half * scales, int64_t row, int D, int d) {
-    if (scales) return __fmul_rn(__half2float(scales[row * (D / 32) + d / 32]), (float) reinterpret_cast<const int8_t *>(data)[row * D + d]);
-    return __half2float(reinterpret_cast<const __half *>(data)[row * D + d]);
+struct Geometry {
+    int n_tok, n_head, group, tiles;  // tiles: row tiles of a key/value head
+    int64_t items;                    // n_kv_head * tiles, per sequence
+    int64_t n_seq;
+    int64_t ctas;                     // CTAs among which the chunks are divided
+};
+
+// CTAs per SM, by what registers allow (__launch_bounds__ holds the compiler to it).
+template <bool Q8, int D>
+constexpr int ctas_per_sm() { return D == 256 ? 2 : 3; }
+
+int ctas_per_sm_of(bool q8, int D) { (void) q8; return D == 256 ? 2 : 3; }
+
+int64_t partial_floats(int D) { return (int64_t) kRows * (D + 2); }  // o [kRows][D], m [kRows], l [kRows]
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-__global__ void __launch_bounds__(kThreads) kv_attention_kernel(KvView c, bool q8, int n_tok, int n_head, const float * __restrict__ q,
-                                                                int64_t ldq, float scale, float * __restrict__ out) {
-    __shared__ float qs[256], p[kThreads], red[kThreads / 32];
-    __shared__ int64_t at[kThreads];
-    const int h = blockIdx.x % n_head;
-    const int64_t row = blockIdx.x / n_head, s = row / n_tok, r = row % n_tok;
-    const int D = c.head_dim, hk = h / (n_head / c.n_kv_head);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t seen = kv_len(c, s, tid == 0) - n_tok + r + 1;
-    for (int d = tid; d < D; d += kThreads) qs[d] = q[row * ldq + (int64_t) h * D + d];
-    float o[2] = {0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
-    for (int64_t j0 = 0; j0 < seen; j0 += kThreads) {
-        __syncthreads();
-        const int64_t j = j0 + tid;
-        const int page = j < seen ? kv_page(c, s, j / c.page_size, true) : -1;
-        const int64_t a = page < 0 ? -1 : ((int64_t) page * c.n_kv_head + hk) * c.page_size + j % c.page_size;
-        float score = -INFINITY;
-        if (a >= 0) {
-            score = 0.0f;
-            for (int d = 0; d < D; d++) score += qs[d] * value(c.k, q8 ? c.kd : nullptr, a, D, d);
-            score *= scale;
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// N 32-bit words from p (aligned to their size) when `there`, else zeros. The cache is read once: not kept in L1.
+template <int N>
+__device__ __forceinline__ void load(uint32_t (&w)[N], const void * p, bool there) {
+#pragma unroll
+    for (int i = 0; i < N; i++) w[i] = 0;
+    if (!there) return;
+    if constexpr (N == 4)
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
+    else if constexpr (N == 2) asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+    else asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+}
+
+// (x, y) as two F16 pairs, hi + lo.
+__device__ __forceinline__ void split(float x, float y, uint32_t & hi, uint32_t & lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+// Two of four bytes q + 128 (sel 0x4140: the first two, 0x4342: the last two) as F16 values q: 0x6400 | b is 1024 + b.
+__device__ __forceinline__ uint32_t halves(uint32_t biased, uint32_t sel) {
+    const uint32_t w = __byte_perm(biased, 0x64646464u, sel);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&w), __float2half2_rn(1152.0f));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+
+__device__ __forceinline__ float half_of(const uint32_t * w, int i) {
+    return __half2float(__ushort_as_half((uint16_t) (w[i >> 1] >> (16 * (i & 1)))));
+}
+
+// How the n index of O = P V runs through the dimensions: groups of 8 kRun dimensions, lane quad g holding kRun contiguous
+// ones of each.
+template <bool Q8, int D>
+struct Shape {
+    static constexpr int kBlocks = D / 32;
+    static constexpr int kRun = !Q8 && D % 64 == 0 ? 8 : 4;
+    static constexpr int kGroups = D / (8 * kRun);
+    static constexpr int kKeyWords = Q8 ? 2 : 4;           // a lane's words of a row's 32 dimensions
+    static constexpr int kValueWords = Q8 ? 1 : kRun / 2;  // a lane's words of a row's group
+};
+
+// The chunks before and in sequence s, and the chunks of all: block-wide over n_seq lengths (every thread gets the result).
+struct Scan {
+    int64_t before, own, total;
+};
+
+__device__ __forceinline__ int64_t chunks_of(const KvView & c, int64_t s, bool tell) { return (kv_len(c, s, tell) + kChunk - 1) / kChunk; }
+
+__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Chunks of sequences [0, n), summed by the block (red: one value per warp).
+__device__ __forceinline__ int64_t block_chunks(const KvView & c, int64_t n, int64_t * red) {
+    int64_t sum = 0;
+    for (int64_t s = threadIdx.x; s < n; s += kThreads) sum += chunks_of(c, s, blockIdx.x == 0);
+    sum = warp_sum64(sum);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) sum += red[w];
+    return sum;
+}
+
+// The sequence that holds chunk number `at` (of one item; chunk numbers count each sequence's chunks `items` times), and
+// where it starts. at < the total.
+__device__ __forceinline__ void find_sequence(const KvView & c, const Geometry & g, int64_t at, int64_t * red, int64_t & seq, int64_t & start) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t base = 0;
+    for (int64_t s0 = 0; s0 < g.n_seq; s0 += kThreads) {
+        const int64_t s = s0 + threadIdx.x;
+        const int64_t mine = s < g.n_seq ? chunks_of(c, s, false) * g.items : 0;
+        int64_t incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
         }
-        const float w = warp_max(score);
-        if (lane == 0) red[warp] = w;
         __syncthreads();
-        float top = m;
-        for (int i = 0; i < kThreads / 32; i++) top = fmaxf(top, red[i]);
-        const float base = top > -INFINITY ? top : 0.0f, keep = expf(m - base);
-        p[tid] = expf(score - base);
-        at[tid] = a;
-        m = top;
+        if (lane == 31) red[warp] = incl;
         __syncthreads();
-        o[0] *= keep, o[1] *= keep, l *= keep;
-        for (int i = 0; i < kThreads; i++) {
-            if (at[i] < 0) continue;
-            l += p[i];
-            for (int e = 0; e < 2; e++)
-                if (tid + e * kThreads < D) o[e] += p[i] * value(c.v, q8 ? c.vd : nullptr, at[i], D, tid + e * kThreads);
+        int64_t first = base, all = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            if (w < warp) first += red[w];
+            all += red[w];
         }
+        const int64_t begin = first + incl - mine;
+        if (mine > 0 && at >= begin && at < begin + mine) {
+            red[kWarps] = s;
+            red[kWarps + 1] = begin;
+        }
+        base += all;
+        if (at < base) break;  // the same for all threads
     }
-    for (int e = 0; e < 2; e++)
-        if (tid + e * kThreads < D) out[(row * n_head + h) * D + tid + e * kThreads] = l != 0.0f ? o[e] / l : 0.0f;
+    __syncthreads();
+    seq = red[kWarps];
+    start = red[kWarps + 1];
+}
+
+// Rows of a tile: row i is query head h * group + (tile * 8 + i) % group of token (tile * 8 + i) / group.
+struct Row {
+    int token, head;
+    bool there;
+};
+
+__device__ __forceinline__ Row row_of(const Geometry & g, int h, int tile, int i) {
+    const int n = tile * kRows + i;
+    return {n / g.group, h * g.group + n % g.group, n < g.n_tok * g.group};
+}
+
+template <bool Q8, int D>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
+    kv_attention_kernel(KvView c, Geometry g, const float * __restrict__ q, int64_t ldq, float scale, float * __restrict__ out, float * __restrict__ ws) {
+    using S = Shape<Q8, D>;
+    __shared__ __align__(16) uint32_t sq[D / 16][32][4];  // the query tile as fragments
+    __shared__ float so[kWarps][kRows][D + 4];            // the warps' results
+    __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
+    __shared__ int64_t red[kWarps + 2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int gq = lane >> 2, t = lane & 3;  // the fragment's group and thread in it
+    pdl_launch_dependents();
+
+    const int64_t total = block_chunks(c, g.n_seq, red) * g.items;
+    const int64_t share = (total + g.ctas - 1) / g.ctas;
+    int64_t at = blockIdx.x * share;
+    const int64_t end = at + share < total ? at + share : total;
+    if (at >= end) return;
+    int64_t seq, start;
+    find_sequence(c, g, at, red, seq, start);
+    int64_t len = kv_len(c, seq, false), chunks = (len + kChunk - 1) / kChunk;
+
+    while (at < end) {
+        while (at >= start + chunks * g.items) {  // the next sequence that has chunks
+            start += chunks * g.items;
+            seq++;
+            len = kv_len(c, seq, false);
+            chunks = (len + kChunk - 1) / kChunk;
+        }
+        const int64_t item = (at - start) / chunks, c0 = (at - start) % chunks;
+        const int64_t c1 = c0 + (end - at) < chunks ? c0 + (end - at) : chunks;
+        at += c1 - c0;
+        const int h = (int) (item / g.tiles), tile = (int) (item % g.tiles);
+        const Row row = row_of(g, h, tile, gq);
+
+        // ---- the query tile: each warp makes the fragments of its share of the k steps ----
+        // k step 2 j + b of lane (gq, t) holds dimensions 32 j + 8 t + 4 b .. + 3 of row gq: hi in registers 0 and 2, lo in
+        // 1 and 3. The row is scaled by 2^k to a largest magnitude in [2^14, 2^15).
+        float factor;  // what a raw score is multiplied by: scale log2(e) 2^-k
+        {
+            const float * src = q + (seq * g.n_tok + row.token) * ldq + (int64_t) row.head * D + 8 * t;
+            float x[D / 4], top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 4; i++) {
+                x[i] = row.there ? src[(i / 8) * 32 + i % 8] : 0.0f;
+                top = fmaxf(top, fabsf(x[i]));
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = (int) (__float_as_uint(top) >> 23);
+            const int k = e == 255 || top == 0.0f ? 0 : 141 - e < 126 ? 141 - e : 126;
+            const float up = __uint_as_float((uint32_t) (k + 127) << 23);
+            factor = scale * 1.4426950408889634f * __uint_as_float((uint32_t) (127 - k) << 23);
+#pragma unroll
+            for (int j = 0; j < D / 16; j++) {
+                if (j % kWarps != warp) continue;
+                uint32_t hi[2], lo[2];
+                split(x[4 * j] * up, x[4 * j + 1] * up, hi[0], lo[0]);
+                split(x[4 * j + 2] * up, x[4 * j + 3] * up, hi[1], lo[1]);
+                *reinterpret_cast<uint4 *>(sq[j][lane]) = make_uint4(hi[0], lo[0], hi[1], lo[1]);
+            }
+        }
+        __syncthreads();
+
+        // ---- this warp's tiles of positions [c0 * 64, c1 * 64) ----
+        const int64_t p_end = c1 * kChunk < len ? c1 * kChunk : len;
+        const int64_t all_see = len - g.n_tok + 1;  // positions below are seen by every row
+        const int64_t seen = row.there ? all_see + row.token : 0;
+        float o[S::kGroups][S::kRun][2] = {}, m = -INFINITY, l = 0.0f;
+        for (int64_t p0 = c0 * kChunk + warp * 16; p0 < p_end; p0 += kWarps * 16) {
+            const int page = kv_page(c, seq, p0 / c.page_size, lane == 0);
+            if (page < 0) continue;
+            const int here = p_end - p0 < 16 ? (int) (p_end - p0) : 16;  // positions of the tile
+            const int64_t r0 = ((int64_t) page * c.n_kv_head + h) * c.page_size + p0 % c.page_size;
+            const uint8_t * kp = c.k + (r0 + gq) * (Q8 ? D : 2 * D) + t * (Q8 ? 8 : 16);
+            const uint8_t * vp = c.v + (r0 + 2 * t) * (Q8 ? D : 2 * D) + gq * S::kRun * (Q8 ? 1 : 2);
+            uint32_t kw[2][S::kBlocks][S::kKeyWords], vw[4][S::kGroups][S::kValueWords];
+            uint32_t kd[2][Q8 ? S::kBlocks : 1], vd[2][Q8 ? S::kBlocks : 1];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int b = 0; b < S::kBlocks; b++)
+                    load(kw[i][b], kp + (int64_t) i * 8 * (Q8 ? D : 2 * D) + b * (Q8 ? 32 : 64), gq + 8 * i < here);
+            // positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9: the ones whose scores this lane holds
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int n = 0; n < S::kGroups; n++)
+                    load(vw[i][n], vp + (int64_t) ((i & 1) + 8 * (i >> 1)) * (Q8 ? D : 2 * D) + n * 8 * S::kRun * (Q8 ? 1 : 2),
+                         2 * t + (i & 1) + 8 * (i >> 1) < here);
+            if constexpr (Q8) {  // the scales of two neighbouring rows are kBlocks words
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const uint32_t * a = reinterpret_cast<const uint32_t *>(c.kd + (r0 + 2 * t + 8 * i) * S::kBlocks);
+                    const uint32_t * b = reinterpret_cast<const uint32_t *>(c.vd + (r0 + 2 * t + 8 * i) * S::kBlocks);
+#pragma unroll
+                    for (int n = 0; n < S::kBlocks; n++) {
+                        kd[i][n] = __ldg(a + n);
+                        vd[i][n] = __ldg(b + n);
+                    }
+                }
+            }
+
+            // ---- scores: s[2 i + j] is position 2 t + j + 8 i of row gq ----
+            float s[4];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                s[2 * i] = s[2 * i + 1] = 0.0f;
+#pragma unroll
+                for (int b = 0; b < S::kBlocks; b++) {
+                    const uint4 a0 = *reinterpret_cast<const uint4 *>(sq[2 * b][lane]), a1 = *reinterpret_cast<const uint4 *>(sq[2 * b + 1][lane]);
+                    const uint32_t f0[4] = {a0.x, a0.y, a0.z, a0.w}, f1[4] = {a1.x, a1.y, a1.z, a1.w};
+                    if constexpr (Q8) {
+                        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        const uint32_t w0 = kw[i][b][0] ^ 0x80808080u, w1 = kw[i][b][1] ^ 0x80808080u;
+                        mma(part, f0, halves(w0, 0x4140), halves(w0, 0x4342));
+                        mma(part, f1, halves(w1, 0x4140), halves(w1, 0x4342));
+                        s[2 * i] = fmaf(half_of(kd[i], b), part[0] + part[2], s[2 * i]);
+                        s[2 * i + 1] = fmaf(half_of(kd[i], S::kBlocks + b), part[1] + part[3], s[2 * i + 1]);
+                    } else {
+                        mma(sum, f0, kw[i][b][0], kw[i][b][1]);
+                        mma(sum, f1, kw[i][b][2], kw[i][b][3]);
+                    }
+                }
+                if constexpr (!Q8) {
+                    s[2 * i] = sum[0] + sum[2];
+                    s[2 * i + 1] = sum[1] + sum[3];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[i] *= factor;
+            const bool edge = p0 + here > all_see || here < 16;
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int j = 2 * t + (i & 1) + 8 * (i >> 1);
+                    if (j >= here || p0 + j >= seen) s[i] = -INFINITY;
+                }
+            }
+
+            // ---- weights: m is the running maximum less kShift (-infinity before any score) ----
+            float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float m_new = fmaxf(m, top - kShift);
+            const float base = m_new == -INFINITY ? 0.0f : m_new;
+            const float keep = ex2(m - base);
+            m = m_new;
+            float p[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[i] = ex2(s[i] - base);
+            l = fmaf(l, keep, (p[0] + p[1]) + (p[2] + p[3]));
+
+            // ---- o = o keep + P V ----
+            if constexpr (Q8) {
+#pragma unroll
+                for (int b = 0; b < S::kBlocks; b++) {
+                    float d[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) d[i] = half_of(vd[i >> 1], (i & 1) * S::kBlocks + b);
+                    if (here < 16) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (2 * t + (i & 1) + 8 * (i >> 1) >= here) d[i] = 0.0f;
+                    }
+                    float big = fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fabsf(d[3])));
+                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                    int e = (int) (__float_as_uint(big) >> 23);
+                    if (e == 0 || e == 255) e = 126;
+                    const float up = __uint_as_float((uint32_t) (253 - e) << 23), down = __uint_as_float((uint32_t) (e + 1) << 23);
+                    float w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) w[i] = edge && p[i] == 0.0f ? 0.0f : p[i] * (d[i] * up);
+                    uint32_t a[4];
+                    split(w[0], w[1], a[0], a[1]);
+                    split(w[2], w[3], a[2], a[3]);
+                    // two rows' four bytes each, interleaved: (row, row + 1) pairs of dimensions 0, 1 and 2, 3
+                    const uint32_t x0 = __byte_perm(vw[0][b][0], vw[1][b][0], 0x5140) ^ 0x80808080u;
+                    const uint32_t x1 = __byte_perm(vw[0][b][0], vw[1][b][0], 0x7362) ^ 0x80808080u;
+                    const uint32_t y0 = __byte_perm(vw[2][b][0], vw[3][b][0], 0x5140) ^ 0x80808080u;
+                    const uint32_t y1 = __byte_perm(vw[2][b][0], vw[3][b][0], 0x7362) ^ 0x80808080u;
+#pragma unroll
+                    for (int n = 0; n < 4; n++) {
+                        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        const uint32_t sel = n & 1 ? 0x4342 : 0x4140;
+                        mma(part, a, halves(n < 2 ? x0 : x1, sel), halves(n < 2 ? y0 : y1, sel));
+                        o[b][n][0] = fmaf(o[b][n][0], keep, (part[0] + part[2]) * down);
+                        o[b][n][1] = fmaf(o[b][n][1], keep, (part[1] + part[3]) * down);
+                    }
+                }
+            } else {
+                uint32_t a[4];
+                split(p[0], p[1], a[0], a[1]);
+                split(p[2], p[3], a[2], a[3]);
+                // Where rows see different positions, a value that is NaN or infinite must not meet the weight 0 of a row that
+                // does not see it: one product per token then, from the last, with the values behind its position zeroed.
+                const bool apart = edge && g.n_tok > 1;
+                const int first = apart ? tile * kRows / g.group : 0;
+                int token = apart ? min((tile * kRows + kRows - 1) / g.group, g.n_tok - 1) : 0;
+                for (; token >= first; token--) {
+                    if (apart) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (p0 + 2 * t + (i & 1) + 8 * (i >> 1) >= all_see + token) {
+#pragma unroll
+                                for (int n = 0; n < S::kGroups; n++)
+#pragma unroll
+                                    for (int w = 0; w < S::kValueWords; w++) vw[i][n][w] = 0;
+                            }
+                    }
+                    const bool mine = !apart || row.token == token;
+#pragma unroll
+                    for (int n = 0; n < S::kGroups; n++)
+#pragma unroll
+                        for (int r = 0; r < S::kRun; r++) {
+                            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            const uint32_t sel = r & 1 ? 0x7632 : 0x5410;
+                            mma(part, a, __byte_perm(vw[0][n][r / 2], vw[1][n][r / 2], sel), __byte_perm(vw[2][n][r / 2], vw[3][n][r / 2], sel));
+                            if (mine) {
+                                o[n][r][0] = fmaf(o[n][r][0], keep, part[0] + part[2]);
+                                o[n][r][1] = fmaf(o[n][r][1], keep, part[1] + part[3]);
+                            }
+                        }
+                }
+            }
+        }
+
+        // ---- join the warps ----
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (t == 0) {
+            sm[warp][gq] = m;
+            sl[warp][gq] = l;
+        }
+#pragma unroll
+        for (int n = 0; n < S::kGroups; n++)
+#pragma unroll
+            for (int r = 0; r < S::kRun; r++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) so[warp][gq][n * 8 * S::kRun + (2 * t + j) * S::kRun + r] = o[n][r][j];
+        __syncthreads();
+        {
+            const int i = tid / 16;  // a row per 16 threads
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) top = fmaxf(top, sm[w][i]);
+            const float base = top == -INFINITY ? 0.0f : top;
+            float f[kWarps], sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) {
+                f[w] = ex2(sm[w][i] - base);
+                sum = fmaf(sl[w][i], f[w], sum);
+            }
+            const Row mine = row_of(g, h, tile, i);
+            const bool whole = c0 == 0 && c1 == chunks;
+            float * to = whole ? out + ((seq * g.n_tok + mine.token) * g.n_head + mine.head) * D
+                               : ws + (2 * blockIdx.x + (c0 == 0 ? 1 : 0)) * (int64_t) (kRows * (D + 2)) + i * D;
+            const float inv = !whole ? 1.0f : sum != 0.0f ? 1.0f / sum : 0.0f;
+            if (!whole || mine.there) {
+                for (int d = tid & 15; d < D; d += 16) {
+                    float v = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < kWarps; w++) v = fmaf(so[w][i][d], f[w], v);
+                    to[d] = v * inv;
+                }
+            }
+            if (!whole && (tid & 15) == 0) {
+                float * ml = ws + (2 * blockIdx.x + (c0 == 0 ? 1 : 0)) * (int64_t) (kRows * (D + 2)) + kRows * D;
+                ml[i] = top;
+                ml[kRows + i] = sum;
+            }
+        }
+        __syncthreads();  // sq, so are written again by the next run
+    }
+}
+
+// Joins the partials of items that several CTAs worked on, and writes the zeros of empty sequences. One CTA per item.
+template <int D>
+__global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(KvView c, Geometry g, float * __restrict__ out, const float * __restrict__ ws) {
+    __shared__ int64_t red[kWarps + 2];
+    const int64_t seq = blockIdx.x / g.items, item = blockIdx.x % g.items;
+    const int h = (int) (item / g.tiles), tile = (int) (item % g.tiles), tid = threadIdx.x, i = tid / 16;
+    const int64_t total = block_chunks(c, g.n_seq, red) * g.items;
+    const int64_t share = (total + g.ctas - 1) / g.ctas;
+    const int64_t before = block_chunks(c, seq, red) * g.items;
+    const int64_t chunks = chunks_of(c, seq, false);
+    const Row mine = row_of(g, h, tile, i);
+    float * to = out + ((seq * g.n_tok + mine.token) * g.n_head + mine.head) * D;
+    pdl_wait();
+    if (chunks == 0) {
+        if (mine.there)
+            for (int d = tid & 15; d < D; d += 16) to[d] = 0.0f;
+        return;
+    }
+    const int64_t a = before + item * chunks, first = a / share, last = (a + chunks - 1) / share;
+    if (first == last || !mine.there) return;
+    auto part = [&](int64_t cta) { return ws + (2 * cta + (cta == first ? 1 : 0)) * (int64_t) (kRows * (D + 2)); };
+    float top = -INFINITY;
+    for (int64_t k = first; k <= last; k++) top = fmaxf(top, part(k)[kRows * D + i]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float v[D / 16] = {}, sum = 0.0f;
+    for (int64_t k = first; k <= last; k++) {
+        const float * src = part(k);
+        const float f = ex2(src[kRows * D + i] - base);
+        sum = fmaf(src[kRows * D + kRows + i], f, sum);
+#pragma unroll
+        for (int d = 0; d < D / 16; d++) v[d] = fmaf(src[i * D + (tid & 15) + 16 * d], f, v[d]);
+    }
+    const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int d = 0; d < D / 16; d++) to[(tid & 15) + 16 * d] = v[d] * inv;
+}
+
+Geometry geometry(const b200_context * ctx, const b200_kv_cache * c, int64_t max_pages, int64_t n_seq, int64_t n_tok, int64_t n_head) {
+    Geometry g;
+    g.n_tok = (int) n_tok;
+    g.n_head = (int) n_head;
+    g.group = (int) (n_head / c->n_kv_head);
+    g.tiles = (g.n_tok * g.group + kRows - 1) / kRows;
+    g.items = (int64_t) c->n_kv_head * g.tiles;
+    g.n_seq = n_seq;
+    g.ctas = (int64_t) ctx->num_sms * ctas_per_sm_of(c->type == B200_TYPE_Q8_0, c->head_dim);
+    const int64_t most = (max_pages * c->page_size + kChunk - 1) / kChunk * n_seq * g.items;  // chunks, if every length were the largest
+    if (g.ctas > most) g.ctas = most > 0 ? most : 1;
+    return g;
+}
+
+template <bool Q8, int D>
+cudaError_t launch(const KvView & c, const Geometry & g, const float * q, int64_t ldq, float scale, float * out, float * ws, cudaStream_t st) {
+    kv_attention_kernel<Q8, D><<<(unsigned) g.ctas, kThreads, 0, st>>>(c, g, q, ldq, scale, out, ws);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned) (g.n_seq * g.items), 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<D>, c, g, out, (const float *) ws);
+}
+
+bool fits(const b200_kv_cache * c, int64_t max_pages, int64_t n_seq, int64_t n_tok, int64_t n_head) {
+    return c && c->n_kv_head > 0 && c->page_size > 0 && max_pages >= 0 && n_seq > 0 && n_tok > 0 && n_tok <= 16 && n_head > 0 && n_head <= 65535 &&
+           n_head % c->n_kv_head == 0 && max_pages <= INT32_MAX / c->page_size && n_seq * n_tok <= INT32_MAX / n_head;
 }
 
 }  // namespace
@@ -68,8 +540,8 @@ extern "C" {
 
 size_t b200_kv_attention_workspace(b200_context * ctx, const b200_kv_cache * cache, int64_t max_pages, int64_t n_seq, int64_t n_tok,
                                    int64_t n_head) {
-    (void) ctx, (void) cache, (void) max_pages, (void) n_seq, (void) n_tok, (void) n_head;
-    return 0;
+    if (!ctx || !fits(cache, max_pages, n_seq, n_tok, n_head)) return 0;
+    return (size_t) (2 * geometry(ctx, cache, max_pages, n_seq, n_tok, n_head).ctas * partial_floats(cache->head_dim)) * sizeof(float);
 }
 
 b200_status b200_kv_attention(b200_context * ctx, void * stream, const b200_kv_cache * cache, const int32_t * table, int64_t max_pages,
@@ -82,18 +554,29 @@ b200_status b200_kv_attention(b200_context * ctx, void * stream, const b200_kv_c
     if (n_tok > 16) return kv_fail(ctx, B200_ERR_UNSUPPORTED, what, "more than 16 tokens per sequence");
     if (n_head <= 0 || n_head > 65535 || n_head % c.n_kv_head) return kv_fail(ctx, B200_ERR_INVALID, what, "n_head is not a multiple of n_kv_head");
     if (n_seq == 0 || n_tok == 0) return B200_OK;
-    if (n_seq * n_tok > INT32_MAX / n_head) return kv_fail(ctx, B200_ERR_INVALID, what, "n_seq * n_tok * n_head passes 2^31");
+    if (!fits(cache, max_pages, n_seq, n_tok, n_head)) return kv_fail(ctx, B200_ERR_INVALID, what, "n_seq * n_tok * n_head passes 2^31");
     if (ldq < n_head * c.head_dim) return kv_fail(ctx, B200_ERR_INVALID, what, "the row stride is below n_head * head_dim");
     if (!q || !out || ((uintptr_t) q & 3) || ((uintptr_t) out & 3)) return kv_fail(ctx, B200_ERR_INVALID, what, "NULL or misaligned q or out");
-    const size_t need = b200_kv_attention_workspace(ctx, cache, max_pages, n_seq, n_tok, n_head);
-    if (need && (!workspace || workspace_bytes < need || ((uintptr_t) workspace & 255)))
+    const Geometry g = geometry(ctx, cache, max_pages, n_seq, n_tok, n_head);
+    if (!workspace || workspace_bytes < 2 * (size_t) (g.ctas * partial_floats(c.head_dim)) * sizeof(float) || ((uintptr_t) workspace & 255))
         return kv_fail(ctx, B200_ERR_INVALID, what, "the workspace is missing, misaligned or too small");
     DeviceScope scope(ctx->device);
     if (scope.status != cudaSuccess) return kv_cuda(ctx, scope.status, what);
     cudaStream_t st = stream ? (cudaStream_t) stream : ctx->stream;
-    kv_attention_kernel<<<(unsigned) (n_seq * n_tok * n_head), kThreads, 0, st>>>(c, cache->type == B200_TYPE_Q8_0, (int) n_tok, (int) n_head, q, ldq,
-                                                                                scale, out);
-    return kv_cuda(ctx, cudaGetLastError(), what);
+    auto go = [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        return cache->type == B200_TYPE_Q8_0 ? launch<true, D>(c, g, q, ldq, scale, out, (float *) workspace, st)
+                                             : launch<false, D>(c, g, q, ldq, scale, out, (float *) workspace, st);
+    };
+    cudaError_t e = cudaErrorInvalidValue;
+    switch (c.head_dim) {
+    case 64: e = go(std::integral_constant<int, 64>{}); break;
+    case 96: e = go(std::integral_constant<int, 96>{}); break;
+    case 128: e = go(std::integral_constant<int, 128>{}); break;
+    case 256: e = go(std::integral_constant<int, 256>{}); break;
+    default: break;
+    }
+    return kv_cuda(ctx, e, what);
 }
 
 }  // extern "C"
