@@ -36,6 +36,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
+constexpr int kJoinWarps = 8;
 constexpr int kRows = 8;      // rows of a tile
 constexpr int kChunk = 64;    // positions of a chunk: one 16-position tile per warp
 constexpr float kShift = 15;  // weights are held times 2^15, so that their low halves reach 2^-39 of the largest
@@ -53,7 +54,7 @@ constexpr int ctas_per_sm() { return D == 256 ? 2 : 3; }
 
 int ctas_per_sm_of(bool q8, int D) { (void) q8; return D == 256 ? 2 : 3; }
 
-int64_t partial_floats(int D) { return (int64_t) kRows * (D + 2); }  // o [kRows][D], m [kRows], l [kRows]
+constexpr int64_t partial_floats(int D) { return (int64_t) kRows * (D + 2); }  // o [kRows][D], m [kRows], l [kRows]
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -108,11 +109,6 @@ struct Shape {
     static constexpr int kGroups = D / (8 * kRun);
     static constexpr int kKeyWords = Q8 ? 2 : 4;           // a lane's words of a row's 32 dimensions
     static constexpr int kValueWords = Q8 ? 1 : kRun / 2;  // a lane's words of a row's group
-};
-
-// The chunks before and in sequence s, and the chunks of all: block-wide over n_seq lengths (every thread gets the result).
-struct Scan {
-    int64_t before, own, total;
 };
 
 __device__ __forceinline__ int64_t chunks_of(const KvView & c, int64_t s, bool tell) { return (kv_len(c, s, tell) + kChunk - 1) / kChunk; }
@@ -441,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
             const Row mine = row_of(g, h, tile, i);
             const bool whole = c0 == 0 && c1 == chunks;
             float * to = whole ? out + ((seq * g.n_tok + mine.token) * g.n_head + mine.head) * D
-                               : ws + (2 * blockIdx.x + (c0 == 0 ? 1 : 0)) * (int64_t) (kRows * (D + 2)) + i * D;
+                               : ws + (2 * blockIdx.x + (c0 == 0 ? 1 : 0)) * partial_floats(D) + i * D;
             const float inv = !whole ? 1.0f : sum != 0.0f ? 1.0f / sum : 0.0f;
             if (!whole || mine.there) {
                 for (int d = tid & 15; d < D; d += 16) {
@@ -452,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
                 }
             }
             if (!whole && (tid & 15) == 0) {
-                float * ml = ws + (2 * blockIdx.x + (c0 == 0 ? 1 : 0)) * (int64_t) (kRows * (D + 2)) + kRows * D;
+                float * ml = ws + (2 * blockIdx.x + (c0 == 0 ? 1 : 0)) * partial_floats(D) + kRows * D;
                 ml[i] = top;
                 ml[kRows + i] = sum;
             }
@@ -461,41 +457,100 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
     }
 }
 
-// Joins the partials of items that several CTAs worked on, and writes the zeros of empty sequences. One CTA per item.
+// Joins the partials of items that several CTAs worked on, and writes the zeros of empty sequences. One CTA per row of an
+// item: a warp takes every kJoinWarps-th partial, a lane D / 32 dimensions, and the warps join in shared memory.
 template <int D>
-__global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(KvView c, Geometry g, float * __restrict__ out, const float * __restrict__ ws) {
-    __shared__ int64_t red[kWarps + 2];
-    const int64_t seq = blockIdx.x / g.items, item = blockIdx.x % g.items;
-    const int h = (int) (item / g.tiles), tile = (int) (item % g.tiles), tid = threadIdx.x, i = tid / 16;
-    const int64_t total = block_chunks(c, g.n_seq, red) * g.items;
-    const int64_t share = (total + g.ctas - 1) / g.ctas;
-    const int64_t before = block_chunks(c, seq, red) * g.items;
+__global__ void __launch_bounds__(32 * kJoinWarps) kv_attention_join_kernel(KvView c, Geometry g, float * __restrict__ out, const float * __restrict__ ws) {
+    __shared__ int64_t red[2 * kJoinWarps];
+    __shared__ float so[kJoinWarps][D], sm[kJoinWarps], sl[kJoinWarps];
+    const int i = blockIdx.x % kRows, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t seq = blockIdx.x / kRows / g.items, item = blockIdx.x / kRows % g.items;
+    const Row mine = row_of(g, (int) (item / g.tiles), (int) (item % g.tiles), i);
+    if (!mine.there) return;
+    int64_t sums[2] = {0, 0};  // the chunks of an item in all sequences, and in those before this one
+    for (int64_t s = tid; s < g.n_seq; s += 32 * kJoinWarps) {
+        const int64_t n = chunks_of(c, s, false);
+        sums[0] += n;
+        if (s < seq) sums[1] += n;
+    }
+    sums[0] = warp_sum64(sums[0]);
+    sums[1] = warp_sum64(sums[1]);
+    if (lane == 0) {
+        red[2 * warp] = sums[0];
+        red[2 * warp + 1] = sums[1];
+    }
     const int64_t chunks = chunks_of(c, seq, false);
-    const Row mine = row_of(g, h, tile, i);
+    __syncthreads();
+    int64_t total = 0, a = 0;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; w++) {
+        total += red[2 * w];
+        a += red[2 * w + 1];
+    }
+    total *= g.items;
+    a = a * g.items + item * chunks;
     float * to = out + ((seq * g.n_tok + mine.token) * g.n_head + mine.head) * D;
     pdl_wait();
     if (chunks == 0) {
-        if (mine.there)
-            for (int d = tid & 15; d < D; d += 16) to[d] = 0.0f;
+        for (int d = tid; d < D; d += 32 * kJoinWarps) to[d] = 0.0f;
         return;
     }
-    const int64_t a = before + item * chunks, first = a / share, last = (a + chunks - 1) / share;
-    if (first == last || !mine.there) return;
-    auto part = [&](int64_t cta) { return ws + (2 * cta + (cta == first ? 1 : 0)) * (int64_t) (kRows * (D + 2)); };
-    float top = -INFINITY;
-    for (int64_t k = first; k <= last; k++) top = fmaxf(top, part(k)[kRows * D + i]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float v[D / 16] = {}, sum = 0.0f;
-    for (int64_t k = first; k <= last; k++) {
-        const float * src = part(k);
-        const float f = ex2(src[kRows * D + i] - base);
-        sum = fmaf(src[kRows * D + kRows + i], f, sum);
+    const int64_t share = (total + g.ctas - 1) / g.ctas;
+    const int first = (int) (a / share), last = (int) ((a + chunks - 1) / share);
+    if (first == last) return;
+    constexpr int kStep = 4;  // partials of a warp in flight
+    float v[D / 32] = {}, m = -INFINITY, l = 0.0f;
+    for (int k0 = first + warp; k0 <= last; k0 += kStep * kJoinWarps) {
+        float pm[kStep], pl[kStep], po[kStep][D / 32];
 #pragma unroll
-        for (int d = 0; d < D / 16; d++) v[d] = fmaf(src[i * D + (tid & 15) + 16 * d], f, v[d]);
+        for (int n = 0; n < kStep; n++) {
+            const int k = k0 + n * kJoinWarps;
+            const float * src = ws + (2 * k + (k == first ? 1 : 0)) * partial_floats(D);
+            pm[n] = k <= last ? src[kRows * D + i] : -INFINITY;
+            pl[n] = k <= last ? src[kRows * D + kRows + i] : 0.0f;
+#pragma unroll
+            for (int d = 0; d < D / 32; d++) po[n][d] = k <= last ? src[i * D + lane + 32 * d] : 0.0f;
+        }
+        float top = m;
+#pragma unroll
+        for (int n = 0; n < kStep; n++) top = fmaxf(top, pm[n]);
+        const float base = top == -INFINITY ? 0.0f : top, keep = ex2(m - base);
+        m = top;
+        l *= keep;
+#pragma unroll
+        for (int d = 0; d < D / 32; d++) v[d] *= keep;
+#pragma unroll
+        for (int n = 0; n < kStep; n++) {
+            const float f = ex2(pm[n] - base);
+            l = fmaf(pl[n], f, l);
+#pragma unroll
+            for (int d = 0; d < D / 32; d++) v[d] = fmaf(po[n][d], f, v[d]);
+        }
+    }
+    if (lane == 0) {
+        sm[warp] = m;
+        sl[warp] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < D / 32; d++) so[warp][lane + 32 * d] = v[d];
+    __syncthreads();
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; w++) top = fmaxf(top, sm[w]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float f[kJoinWarps], sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; w++) {
+        f[w] = ex2(sm[w] - base);
+        sum = fmaf(sl[w], f[w], sum);
     }
     const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+    for (int d = tid; d < D; d += 32 * kJoinWarps) {
+        float o = 0.0f;
 #pragma unroll
-    for (int d = 0; d < D / 16; d++) to[(tid & 15) + 16 * d] = v[d] * inv;
+        for (int w = 0; w < kJoinWarps; w++) o = fmaf(so[w][d], f[w], o);
+        to[d] = o * inv;
+    }
 }
 
 Geometry geometry(const b200_context * ctx, const b200_kv_cache * c, int64_t max_pages, int64_t n_seq, int64_t n_tok, int64_t n_head) {
@@ -518,8 +573,8 @@ cudaError_t launch(const KvView & c, const Geometry & g, const float * q, int64_
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned) (g.n_seq * g.items), 1, 1);
-    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.gridDim = dim3((unsigned) (g.n_seq * g.items * kRows), 1, 1);
+    cfg.blockDim = dim3(32 * kJoinWarps, 1, 1);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -531,7 +586,7 @@ cudaError_t launch(const KvView & c, const Geometry & g, const float * q, int64_
 
 bool fits(const b200_kv_cache * c, int64_t max_pages, int64_t n_seq, int64_t n_tok, int64_t n_head) {
     return c && c->n_kv_head > 0 && c->page_size > 0 && max_pages >= 0 && n_seq > 0 && n_tok > 0 && n_tok <= 16 && n_head > 0 && n_head <= 65535 &&
-           n_head % c->n_kv_head == 0 && max_pages <= INT32_MAX / c->page_size && n_seq * n_tok <= INT32_MAX / n_head;
+           n_head % c->n_kv_head == 0 && max_pages <= INT32_MAX / c->page_size && n_seq * n_tok <= INT32_MAX / kRows / n_head;
 }
 
 }  // namespace
@@ -554,7 +609,7 @@ b200_status b200_kv_attention(b200_context * ctx, void * stream, const b200_kv_c
     if (n_tok > 16) return kv_fail(ctx, B200_ERR_UNSUPPORTED, what, "more than 16 tokens per sequence");
     if (n_head <= 0 || n_head > 65535 || n_head % c.n_kv_head) return kv_fail(ctx, B200_ERR_INVALID, what, "n_head is not a multiple of n_kv_head");
     if (n_seq == 0 || n_tok == 0) return B200_OK;
-    if (!fits(cache, max_pages, n_seq, n_tok, n_head)) return kv_fail(ctx, B200_ERR_INVALID, what, "n_seq * n_tok * n_head passes 2^31");
+    if (!fits(cache, max_pages, n_seq, n_tok, n_head)) return kv_fail(ctx, B200_ERR_INVALID, what, "n_seq * n_tok * n_head passes 2^28");
     if (ldq < n_head * c.head_dim) return kv_fail(ctx, B200_ERR_INVALID, what, "the row stride is below n_head * head_dim");
     if (!q || !out || ((uintptr_t) q & 3) || ((uintptr_t) out & 3)) return kv_fail(ctx, B200_ERR_INVALID, what, "NULL or misaligned q or out");
     const Geometry g = geometry(ctx, cache, max_pages, n_seq, n_tok, n_head);

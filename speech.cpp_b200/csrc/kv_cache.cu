@@ -4,10 +4,10 @@
 // The reference's cache is one dense F16 tensor per request, written with SET_ROWS (src/common/qwen3-decoder.cpp:300-346);
 // here sequences share a pool of pages, and Q8_0 halves the bytes that attention streams.
 //
-// Both kernels are copies with a conversion: one CTA per row (sequence, token), so the length and the page number are read
-// once, and its threads walk the row's k then v values four at a time, all of a row's heads contiguous on the float side
-// and 64 to 512 contiguous bytes per head on the page's side. They are bound by HBM (4 B per value on the float side, 2 or
-// 34/32 B in the cache), or by launch latency for the rows of a decode step.
+// Both kernels are copies with a conversion, bound by HBM (4 B per value on the float side, 2 or 34/32 B in the cache), or by
+// launch latency for the rows of a decode step. A row's length and page number are a chain of dependent loads before its
+// first value, so many rows have to be under way: a warp or more per row, its threads walking the row's k then v values four
+// at a time with four such pieces in flight.
 #include <cstdio>
 
 #include "kv.cuh"
@@ -82,90 +82,159 @@ __device__ __forceinline__ uint2 pack4(float4 v) {
     return make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
 }
 
+// How rows are given to threads: `per_row` threads (32 to 512) for a row, 256 / per_row rows (or one) in a CTA.
+struct RowSplit {
+    int per_row;
+    int64_t rows;
+};
+
+constexpr int kUnroll = 4;  // four-value pieces of a row that a thread has in flight
+
+// The row of this thread (-1: none) and its place among the row's threads, a multiple of 32 to the warp.
+__device__ __forceinline__ int64_t my_row(const RowSplit & p, int & i0) {
+    const int64_t row = blockIdx.x * (int64_t) (blockDim.x / p.per_row) + threadIdx.x / p.per_row;
+    i0 = threadIdx.x % p.per_row;
+    return row < p.rows ? row : -1;
+}
+
 // Row (s, r) of k and v to its slot. Q8_0: eight lanes hold a block's 32 values (quantize_q8_0_quad), so the warp's lanes
 // all take part in every step, those past the row's end on its last values without storing.
-template <bool Q8, bool VEC>
-__global__ void kv_write_kernel(KvView c, int64_t n_tok, const float * __restrict__ k, int64_t ldk, const float * __restrict__ v, int64_t ldv) {
-    const int64_t row = blockIdx.x, s = row / n_tok, r = row % n_tok;
-    const int64_t pos = kv_len(c, s, threadIdx.x == 0) - n_tok + r;
+template <bool Q8, bool VEC, int D>
+__global__ void __launch_bounds__(512) kv_write_kernel(KvView c, RowSplit p, int64_t n_tok, const float * __restrict__ k, int64_t ldk,
+                                                       const float * __restrict__ v, int64_t ldv) {
+    int i0;
+    const int64_t row = my_row(p, i0);
+    if (row < 0) return;  // whole warps: per_row is a multiple of 32
+    const int64_t s = row / n_tok, r = row % n_tok;
+    const int64_t pos = kv_len(c, s, i0 == 0) - n_tok + r;
     if (pos < 0) return;
-    const int page = kv_page(c, s, pos / c.page_size, threadIdx.x == 0);
+    const int page = kv_page(c, s, pos / c.page_size, i0 == 0);
     if (page < 0) return;
-    const int slot = (int) (pos % c.page_size);
-    const int quads = c.n_kv_head * c.head_dim / 4;  // of k, and of v
-    for (int i0 = threadIdx.x & ~31; i0 < 2 * quads; i0 += blockDim.x) {
-        const int j = i0 + (threadIdx.x & 31);
-        const bool here = j < 2 * quads;
-        const int i = here ? j : 2 * quads - 1;
-        const bool is_v = i >= quads;
-        const int e = (is_v ? i - quads : i) * 4;  // element in the row
-        const int h = e / c.head_dim, d = e % c.head_dim;
-        const float4 x = load4<VEC>(is_v ? v + row * ldv + e : k + row * ldk + e);
-        const int64_t at = ((int64_t) page * c.n_kv_head + h) * c.page_size + slot;
-        uint8_t * to = const_cast<uint8_t *>(is_v ? c.v : c.k);
-        if constexpr (Q8) {
-            float df;
-            const uint32_t q = quantize_q8_0_quad(x, &df);
-            if (here) {
-                *reinterpret_cast<uint32_t *>(to + at * c.head_dim + d) = q;
-                if ((i & 7) == 0) const_cast<__half *>(is_v ? c.vd : c.kd)[at * (c.head_dim / 32) + d / 32] = __float2half_rn(df);
+    const int64_t at0 = (int64_t) page * c.n_kv_head * c.page_size + pos % c.page_size;  // head 0's row in the arrays
+    const int quads = c.n_kv_head * (D / 4);  // of k, and of v
+    const float * kr = k + row * ldk, * vr = v + row * ldv;
+    for (int j0 = i0; (j0 & ~31) < 2 * quads; j0 += kUnroll * p.per_row) {
+        float4 x[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; u++) {
+            const int j = j0 + u * p.per_row, i = j < 2 * quads ? j : 2 * quads - 1;
+            if ((j & ~31) >= 2 * quads) break;  // the whole warp
+            x[u] = load4<VEC>(i >= quads ? vr + (i - quads) * 4 : kr + i * 4);
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; u++) {
+            const int j = j0 + u * p.per_row;
+            if ((j & ~31) >= 2 * quads) break;
+            const bool here = j < 2 * quads;
+            const int i = here ? j : 2 * quads - 1;
+            const bool is_v = i >= quads;
+            const int e = (is_v ? i - quads : i) * 4, h = e / D, d = e % D;
+            const int64_t at = at0 + (int64_t) h * c.page_size;
+            uint8_t * to = const_cast<uint8_t *>(is_v ? c.v : c.k);
+            if constexpr (Q8) {
+                float df;
+                const uint32_t q = quantize_q8_0_quad(x[u], &df);
+                if (here) {
+                    *reinterpret_cast<uint32_t *>(to + at * D + d) = q;
+                    if ((i & 7) == 0) const_cast<__half *>(is_v ? c.vd : c.kd)[at * (D / 32) + d / 32] = __float2half_rn(df);
+                }
+            } else if (here) {
+                *reinterpret_cast<uint2 *>(to + (at * D + d) * 2) = pack4(x[u]);
             }
-        } else if (here) {
-            *reinterpret_cast<uint2 *>(to + (at * c.head_dim + d) * 2) = pack4(x);
         }
     }
 }
 
 // Position start[s] + r to row (s, r) of k and v.
-template <bool Q8, bool HALF, bool VEC>
-__global__ void kv_read_kernel(KvView c, const int32_t * __restrict__ start, int64_t n_tok, void * __restrict__ k, void * __restrict__ v) {
-    const int64_t row = blockIdx.x, s = row / n_tok, r = row % n_tok;
-    const int64_t len = kv_len(c, s, threadIdx.x == 0);
+template <bool Q8, bool HALF, bool VEC, int D>
+__global__ void __launch_bounds__(512) kv_read_kernel(KvView c, RowSplit p, const int32_t * __restrict__ start, int64_t n_tok, void * __restrict__ k,
+                                                      void * __restrict__ v) {
+    int i0;
+    const int64_t row = my_row(p, i0);
+    if (row < 0) return;
+    const int64_t s = row / n_tok, r = row % n_tok;
     const int64_t pos = (start ? (int64_t) start[s] : 0) + r;
-    if (pos < 0 || pos >= len) return;
-    const int page = kv_page(c, s, pos / c.page_size, threadIdx.x == 0);
+    if (pos < 0 || pos >= kv_len(c, s, i0 == 0)) return;
+    const int page = kv_page(c, s, pos / c.page_size, i0 == 0);
     if (page < 0) return;
-    const int slot = (int) (pos % c.page_size);
-    const int quads = c.n_kv_head * c.head_dim / 4;
-    for (int i = threadIdx.x; i < 2 * quads; i += blockDim.x) {
-        const bool is_v = i >= quads;
-        const int e = (is_v ? i - quads : i) * 4;
-        const int h = e / c.head_dim, d = e % c.head_dim;
-        const int64_t at = ((int64_t) page * c.n_kv_head + h) * c.page_size + slot;
-        const uint8_t * from = is_v ? c.v : c.k;
-        const int64_t o = row * 4 * quads + e;
-        void * out = is_v ? v : k;
-        float4 x;
-        if constexpr (Q8) {
-            const char4 q = *reinterpret_cast<const char4 *>(from + at * c.head_dim + d);
-            const float f = __half2float((is_v ? c.vd : c.kd)[at * (c.head_dim / 32) + d / 32]);
-            x = make_float4(__fmul_rn(f, (float) q.x), __fmul_rn(f, (float) q.y), __fmul_rn(f, (float) q.z), __fmul_rn(f, (float) q.w));
-        } else {
-            const uint2 u = *reinterpret_cast<const uint2 *>(from + (at * c.head_dim + d) * 2);
-            const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
-            x = make_float4(a.x, a.y, b.x, b.y);
-        }
-        if constexpr (HALF) {
-            const uint2 u = pack4(x);
-            if constexpr (VEC) {
-                *reinterpret_cast<uint2 *>((__half *) out + o) = u;
+    const int64_t at0 = (int64_t) page * c.n_kv_head * c.page_size + pos % c.page_size;
+    const int quads = c.n_kv_head * (D / 4);
+    for (int j0 = i0; j0 < 2 * quads; j0 += kUnroll * p.per_row) {
+        uint2 raw[kUnroll];
+        __half scale[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; u++) {
+            const int i = j0 + u * p.per_row;
+            if (i >= 2 * quads) break;
+            const bool is_v = i >= quads;
+            const int e = (is_v ? i - quads : i) * 4, h = e / D, d = e % D;
+            const int64_t at = at0 + (int64_t) h * c.page_size;
+            const uint8_t * from = is_v ? c.v : c.k;
+            if constexpr (Q8) {
+                raw[u].x = *reinterpret_cast<const uint32_t *>(from + at * D + d);
+                scale[u] = (is_v ? c.vd : c.kd)[at * (D / 32) + d / 32];
             } else {
-                uint16_t * p = (uint16_t *) out + o;
-                p[0] = (uint16_t) u.x, p[1] = (uint16_t) (u.x >> 16), p[2] = (uint16_t) u.y, p[3] = (uint16_t) (u.y >> 16);
+                raw[u] = *reinterpret_cast<const uint2 *>(from + (at * D + d) * 2);
             }
-        } else if constexpr (VEC) {
-            *reinterpret_cast<float4 *>((float *) out + o) = x;
-        } else {
-            float * p = (float *) out + o;
-            p[0] = x.x, p[1] = x.y, p[2] = x.z, p[3] = x.w;
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; u++) {
+            const int i = j0 + u * p.per_row;
+            if (i >= 2 * quads) break;
+            float4 x;
+            if constexpr (Q8) {
+                const char4 q = *reinterpret_cast<const char4 *>(&raw[u].x);
+                const float f = __half2float(scale[u]);
+                x = make_float4(__fmul_rn(f, (float) q.x), __fmul_rn(f, (float) q.y), __fmul_rn(f, (float) q.z), __fmul_rn(f, (float) q.w));
+            } else {
+                const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&raw[u].x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&raw[u].y));
+                x = make_float4(a.x, a.y, b.x, b.y);
+            }
+            const int64_t o = row * 4 * quads + (i >= quads ? i - quads : i) * 4;
+            void * out = i >= quads ? v : k;
+            if constexpr (HALF) {
+                const uint2 w = pack4(x);
+                if constexpr (VEC) {
+                    *reinterpret_cast<uint2 *>((__half *) out + o) = w;
+                } else {
+                    uint16_t * to = (uint16_t *) out + o;
+                    to[0] = (uint16_t) w.x, to[1] = (uint16_t) (w.x >> 16), to[2] = (uint16_t) w.y, to[3] = (uint16_t) (w.y >> 16);
+                }
+            } else if constexpr (VEC) {
+                *reinterpret_cast<float4 *>((float *) out + o) = x;
+            } else {
+                float * to = (float *) out + o;
+                to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
+            }
         }
     }
 }
 
-// Threads of a row's CTA: one per four values, at most 512.
-unsigned row_threads(const KvView & c) {
-    const int quads = c.n_kv_head * c.head_dim / 2;  // of k and v together
-    return (unsigned) (quads >= 512 ? 512 : (quads + 31) & ~31);
+// Threads per row: enough that all rows together fill the GPU's 2048 threads per SM, at most one per four values of the row,
+// a power of two from 32 to 512.
+RowSplit split_rows(const b200_context * ctx, const KvView & c, int64_t rows) {
+    const int64_t fill = (int64_t) ctx->num_sms * 2048, most = c.n_kv_head * c.head_dim / 2;
+    int n = 32;
+    while (n < 512 && n < most && rows * n < fill) n *= 2;
+    return {n, rows};
+}
+
+unsigned split_threads(const RowSplit & p) { return p.per_row < 256 ? 256 : (unsigned) p.per_row; }
+
+unsigned split_grid(const RowSplit & p) {
+    const int64_t rows = split_threads(p) / p.per_row;
+    return (unsigned) ((p.rows + rows - 1) / rows);
+}
+
+// Calls f with D as a constant.
+template <class F>
+void with_dim(int D, F f) {
+    switch (D) {
+    case 64: f(std::integral_constant<int, 64>{}); break;
+    case 96: f(std::integral_constant<int, 96>{}); break;
+    case 128: f(std::integral_constant<int, 128>{}); break;
+    default: f(std::integral_constant<int, 256>{}); break;
+    }
 }
 
 bool aligned(const void * p, size_t to) { return ((uintptr_t) p & (to - 1)) == 0; }
@@ -256,11 +325,14 @@ b200_status b200_kv_write(b200_context * ctx, void * stream, const b200_kv_cache
     DeviceScope scope(ctx->device);
     if (scope.status != cudaSuccess) return kv_cuda(ctx, scope.status, "kv_write");
     const bool vec = aligned(k, 16) && aligned(v, 16) && ldk % 4 == 0 && ldv % 4 == 0;
-    const unsigned grid = (unsigned) (n_seq * n_tok), threads = row_threads(c);
+    const RowSplit p = split_rows(ctx, c, n_seq * n_tok);
     cudaStream_t st = stream ? (cudaStream_t) stream : ctx->stream;
-    auto kern = cache->type == B200_TYPE_Q8_0 ? (vec ? kv_write_kernel<true, true> : kv_write_kernel<true, false>)
-                                              : (vec ? kv_write_kernel<false, true> : kv_write_kernel<false, false>);
-    kern<<<grid, threads, 0, st>>>(c, n_tok, k, ldk, v, ldv);
+    with_dim(c.head_dim, [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        auto kern = cache->type == B200_TYPE_Q8_0 ? (vec ? kv_write_kernel<true, true, D> : kv_write_kernel<true, false, D>)
+                                                  : (vec ? kv_write_kernel<false, true, D> : kv_write_kernel<false, false, D>);
+        kern<<<split_grid(p), split_threads(p), 0, st>>>(c, p, n_tok, k, ldk, v, ldv);
+    });
     return kv_cuda(ctx, cudaGetLastError(), "kv_write");
 }
 
@@ -276,17 +348,20 @@ b200_status b200_kv_read(b200_context * ctx, void * stream, const b200_kv_cache 
     DeviceScope scope(ctx->device);
     if (scope.status != cudaSuccess) return kv_cuda(ctx, scope.status, "kv_read");
     const bool vec = aligned(k, 4 * elem) && aligned(v, 4 * elem);
-    const unsigned grid = (unsigned) (n_seq * n_tok), threads = row_threads(c);
+    const RowSplit p = split_rows(ctx, c, n_seq * n_tok);
     cudaStream_t st = stream ? (cudaStream_t) stream : ctx->stream;
-    auto pick = [&](auto q8, auto half) {
-        constexpr bool Q8 = decltype(q8)::value, HALF = decltype(half)::value;
-        if (vec) kv_read_kernel<Q8, HALF, true><<<grid, threads, 0, st>>>(c, start, n_tok, k, v);
-        else kv_read_kernel<Q8, HALF, false><<<grid, threads, 0, st>>>(c, start, n_tok, k, v);
-    };
-    using std::true_type;
-    using std::false_type;
-    if (cache->type == B200_TYPE_Q8_0) elem == 2 ? pick(true_type{}, true_type{}) : pick(true_type{}, false_type{});
-    else elem == 2 ? pick(false_type{}, true_type{}) : pick(false_type{}, false_type{});
+    with_dim(c.head_dim, [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        auto pick = [&](auto q8, auto half) {
+            constexpr bool Q8 = decltype(q8)::value, HALF = decltype(half)::value;
+            auto kern = vec ? kv_read_kernel<Q8, HALF, true, D> : kv_read_kernel<Q8, HALF, false, D>;
+            kern<<<split_grid(p), split_threads(p), 0, st>>>(c, p, start, n_tok, k, v);
+        };
+        using std::false_type;
+        using std::true_type;
+        if (cache->type == B200_TYPE_Q8_0) elem == 2 ? pick(true_type{}, true_type{}) : pick(true_type{}, false_type{});
+        else elem == 2 ? pick(false_type{}, true_type{}) : pick(false_type{}, false_type{});
+    });
     return kv_cuda(ctx, cudaGetLastError(), "kv_read");
 }
 

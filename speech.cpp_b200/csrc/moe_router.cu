@@ -1,8 +1,14 @@
 // moe_router.cu — the expert router (b200_moe_router): scores, group choice, top-k and weights of each row of logits.
 //
-// One warp per row; lane l holds experts l, l + 32, ... and each round takes the best expert that is left. Scores that are
-// compared across experts (with a bias or groups) are double, since a sum with a bias rounded to float32 would reorder
-// experts that are nearly equal.
+// One warp per row; lane l holds experts l, l + 32, ... as 32-bit keys whose unsigned order is the values' order, and each
+// round of the top-k is a maximum over the lane's keys and one reduction instruction over the warp (another finds the lowest
+// expert with that key). Which experts are chosen has to be right where they are nearly equal:
+//  - without bias and groups the logits themselves are the keys, which decides exactly;
+//  - otherwise scores are computed in float32 first, with a bound on their error, and the row is accepted if every
+//    comparison that decides (neighbours among the chosen and the next one, the last group kept and the first one left) is
+//    wider than that. The few rows that are not, and rows with anything non-finite, are done again in double.
+// The weights of the chosen, one per lane, are double either way. Reading the logits takes 4 B per expert; the rounds' some
+// 30 to 60 instructions each decide the time (about 10 us per 16384 rows of 256 experts against 2.7 us of HBM).
 #include <cmath>
 
 #include "kv.cuh"
@@ -11,10 +17,29 @@ using namespace b200;
 
 namespace {
 
+constexpr int kWarps = 4;
+constexpr unsigned kAll = 0xffffffffu;
+
 struct RouterParams {
     int E, top_k, score, n_group, topk_group, group_top, renorm;
     float scale;
+    // groups in the float32 pass: `lanes` lanes (a power of two, n_group * lanes <= 32) for each, the scores of a group
+    // `pitch` floats apart in shared memory so that a step's lanes read different banks
+    int lanes, pitch;
+    unsigned inv;  // expert e's group is e * inv >> 21 (e < 1024)
 };
+
+__device__ __forceinline__ int group_of(const RouterParams & a, int e) { return (int) ((unsigned) e * a.inv >> 21); }
+
+// Unsigned order of the keys = order of the values (NaN: not allowed). 0 is below every value's key.
+__device__ __forceinline__ unsigned key_of(float x) {
+    const unsigned u = __float_as_uint(x + 0.0f);  // -0 as 0
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ float value_of(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
+// ---- the row in double ------------------------------------------------------------------------------------------------
 
 // (a, i) before (b, j): larger first, ties to the lower index.
 __device__ __forceinline__ bool before(double a, int i, double b, int j) { return a > b || (a == b && i < j); }
@@ -22,53 +47,43 @@ __device__ __forceinline__ bool before(double a, int i, double b, int j) { retur
 __device__ __forceinline__ void warp_best(double & v, int & i) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const double ov = __shfl_xor_sync(0xffffffffu, v, o);
-        const int oi = __shfl_xor_sync(0xffffffffu, i, o);
+        const double ov = __shfl_xor_sync(kAll, v, o);
+        const int oi = __shfl_xor_sync(kAll, i, o);
         if (before(ov, oi, v, i)) v = ov, i = oi;
     }
 }
 
-// EPL: experts per lane.
+__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x; }
+
+// The numerator of a softmax term (or a sigmoid) of logit x in double; top: the row's largest logit.
+__device__ __forceinline__ double term(const RouterParams & a, float x, float top) {
+    if (x == -INFINITY) return 0.0;
+    if (a.score == B200_ROUTER_SIGMOID) return 1.0 / (1.0 + exp(-(double) x));
+    return x == top ? 1.0 : exp((double) x - (double) top);
+}
+
+// The experts of one row: lane k gets the k-th chosen. For rows that float32 does not decide.
 template <int EPL>
-__global__ void __launch_bounds__(128) moe_router_kernel(RouterParams a, const float * __restrict__ logits, const float * __restrict__ bias,
-                                                         int64_t T, int32_t * __restrict__ ids, float * __restrict__ w) {
+__device__ __noinline__ int choose_exactly(const RouterParams & a, const float * __restrict__ logits, const float * __restrict__ bias, float top) {
     const int lane = threadIdx.x & 31;
-    const int64_t t = blockIdx.x * (int64_t) (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (t >= T) return;
     const double ninf = -INFINITY;
-    double p[EPL], c[EPL];
-    float top = -INFINITY;
+    double c[EPL], sum = 0.0;
 #pragma unroll
     for (int i = 0; i < EPL; i++) {
         const int e = i * 32 + lane;
-        float x = e < a.E ? logits[t * a.E + e] : -INFINITY;
-        if (x != x) x = -INFINITY;
-        p[i] = x;
-        top = fmaxf(top, x);
-    }
-    top = warp_max(top);
-    double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < EPL; i++) {
-        const double x = p[i];
-        const bool order = !bias && a.n_group == 1;  // the logits' order is the scores'
-        if (a.score == B200_ROUTER_SIGMOID) p[i] = x == ninf ? 0.0 : 1.0 / (1.0 + exp(-x));
-        else p[i] = x == ninf ? 0.0 : x == (double) top ? 1.0 : exp(x - (double) top);
-        sum += p[i];
-        c[i] = order ? x : p[i];
+        c[i] = e < a.E ? term(a, clean(logits[e]), top) : 0.0;
+        sum += c[i];
     }
     sum = warp_sum_d(sum);
+    unsigned taken = 0;  // bit i: this lane's expert i is out (past the last one, in a group that is not kept, or chosen)
 #pragma unroll
     for (int i = 0; i < EPL; i++) {
         const int e = i * 32 + lane;
-        if (a.score == B200_ROUTER_SOFTMAX) p[i] = sum > 0.0 ? p[i] / sum : 0.0;
-        if (bias || a.n_group > 1) c[i] = e < a.E ? (bias ? p[i] + (double) bias[e] : p[i]) : ninf;
+        if (a.score == B200_ROUTER_SOFTMAX) c[i] = sum > 0.0 ? c[i] / sum : 0.0;
+        if (e >= a.E) taken |= 1u << i, c[i] = ninf;
+        else if (bias) c[i] += (double) bias[e];
         if (c[i] != c[i]) c[i] = ninf;
     }
-    unsigned taken = 0;  // bit i: this lane's expert i is out (past the last one, in a group that is not kept, or chosen)
-#pragma unroll
-    for (int i = 0; i < EPL; i++)
-        if (i * 32 + lane >= a.E) taken |= 1u << i;
     if (a.n_group > 1) {
         const int size = a.E / a.n_group;
         double mine = 0.0;  // lane g: group g's score
@@ -81,7 +96,7 @@ __global__ void __launch_bounds__(128) moe_router_kernel(RouterParams a, const f
 #pragma unroll
                 for (int i = 0; i < EPL; i++) {
                     const int e = i * 32 + lane;
-                    if (e < a.E && e / size == g && e != skip && before(c[i], e, v, at)) v = c[i], at = e;
+                    if (e < a.E && group_of(a, e) == g && e != skip && before(c[i], e, v, at)) v = c[i], at = e;
                 }
                 warp_best(v, at);
                 score += v;
@@ -91,21 +106,21 @@ __global__ void __launch_bounds__(128) moe_router_kernel(RouterParams a, const f
         }
         unsigned kept = 0;
         for (int n = 0; n < a.topk_group; n++) {
-            double v = lane < a.n_group && !(kept >> lane & 1) ? mine : ninf;
-            int at = lane < a.n_group && !(kept >> lane & 1) ? lane : 32 + lane;
+            const bool open = lane < a.n_group && !(kept >> lane & 1);
+            double v = open ? mine : ninf;
+            int at = open ? lane : 32 + lane;
             warp_best(v, at);
             kept |= 1u << at;
         }
 #pragma unroll
         for (int i = 0; i < EPL; i++) {
             const int e = i * 32 + lane;
-            if (e < a.E && !(kept >> (e / size) & 1)) taken |= 1u << i;
+            if (e < a.E && !(kept >> group_of(a, e) & 1)) taken |= 1u << i;
         }
     }
-    double mine = 0.0, total = 0.0;  // lane k: the score of the k-th chosen
     int id = 0;
     for (int k = 0; k < a.top_k; k++) {
-        double v = ninf, ps = 0.0;
+        double v = ninf;
         int at = INT32_MAX;
 #pragma unroll
         for (int i = 0; i < EPL; i++)
@@ -113,13 +128,158 @@ __global__ void __launch_bounds__(128) moe_router_kernel(RouterParams a, const f
         warp_best(v, at);
 #pragma unroll
         for (int i = 0; i < EPL; i++)
-            if (at == i * 32 + lane) ps = p[i], taken |= 1u << i;
-        ps = __shfl_sync(0xffffffffu, ps, at & 31);
-        total += ps;
-        if (lane == k) mine = ps, id = at;
+            if (at == i * 32 + lane) taken |= 1u << i;
+        if (lane == k) id = at;
     }
-    if (lane < a.top_k) {
-        if (a.renorm) mine = total > 0.0 ? mine / total : 0.0;
+    return id;
+}
+
+// ---- rows by keys -----------------------------------------------------------------------------------------------------
+
+// The `rounds` largest of the warp's keys (0: out), ties to the lowest expert: lane k gets the k-th's expert and key.
+template <int EPL>
+__device__ __forceinline__ void largest(unsigned (&key)[EPL], int rounds, int & id, unsigned & found) {
+    const int lane = threadIdx.x & 31;
+    for (int k = 0; k < rounds; k++) {
+        unsigned best = key[0];
+#pragma unroll
+        for (int i = 1; i < EPL; i++) best = max(best, key[i]);
+        const unsigned top = __reduce_max_sync(kAll, best);
+        unsigned at = 0xffffffffu;
+#pragma unroll
+        for (int i = EPL - 1; i >= 0; i--)
+            if (key[i] == top) at = i * 32 + lane;
+        at = __reduce_min_sync(kAll, at);
+#pragma unroll
+        for (int i = 0; i < EPL; i++)
+            if (at == i * 32u + lane) key[i] = 0;
+        if (lane == k) id = (int) at, found = top;
+    }
+}
+
+// The larger pair of (a1 >= a2) and (b1 >= b2).
+__device__ __forceinline__ void merge2(float & a1, float & a2, float b1, float b2) {
+    a2 = fmaxf(fminf(a1, b1), fmaxf(a2, b2));
+    a1 = fmaxf(a1, b1);
+}
+
+// EPL: experts per lane. BY_LOGIT: no bias and no groups.
+template <int EPL, bool BY_LOGIT>
+__global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a, const float * __restrict__ logits, const float * __restrict__ bias,
+                                                                 int64_t T, int32_t * __restrict__ ids, float * __restrict__ w) {
+    extern __shared__ float shared[];  // groups: each warp's scores, [n_group][pitch]
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t t = blockIdx.x * (int64_t) kWarps + warp;
+    if (t >= T) return;
+    const float * row = logits + t * a.E;
+    float x[EPL], top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < EPL; i++) {
+        x[i] = i * 32 + lane < a.E ? clean(row[i * 32 + lane]) : -INFINITY;
+        top = fmaxf(top, x[i]);
+    }
+    top = value_of(__reduce_max_sync(kAll, key_of(top)));
+
+    int id = 0;
+    if constexpr (BY_LOGIT) {
+        unsigned key[EPL], found = 0;
+#pragma unroll
+        for (int i = 0; i < EPL; i++) key[i] = i * 32 + lane < a.E ? key_of(x[i]) : 0;
+        largest<EPL>(key, a.top_k, id, found);
+    } else {
+        // float32 scores; `off` bounds the error of each. __expf(-d) is within 2 + 1.173 d units of its last place, so within
+        // 2^-22 absolutely; a sigmoid is that, a rounded sum and a quotient of two units: below 2^-20. A softmax's sum adds up
+        // to 32 terms per lane and five times over the warp (37 roundings, below 2^-18.7) of terms that are off by some 2^-20.7
+        // of the sum at most: below 2^-17 of the largest term. The sum with the bias rounds once more.
+        float sum = 0.0f, c[EPL], far = 0.0f;
+        bool finite = true;
+#pragma unroll
+        for (int i = 0; i < EPL; i++) {
+            const bool there = i * 32 + lane < a.E;
+            finite = finite && (!there || fabsf(x[i]) < INFINITY);
+            c[i] = a.score == B200_ROUTER_SIGMOID ? __fdividef(1.0f, 1.0f + __expf(-x[i])) : __expf(x[i] - top);
+            sum += there ? c[i] : 0.0f;
+        }
+        const float inv = a.score == B200_ROUTER_SOFTMAX ? __fdividef(1.0f, warp_sum(sum)) : 1.0f;
+        unsigned key[EPL];
+#pragma unroll
+        for (int i = 0; i < EPL; i++) {
+            const int e = i * 32 + lane;
+            c[i] *= inv;
+            if (bias && e < a.E) c[i] += bias[e];
+            finite = finite && (e >= a.E || fabsf(c[i]) < INFINITY);
+            if (e < a.E) far = fmaxf(far, fabsf(c[i]));
+            key[i] = e < a.E ? key_of(c[i]) : 0;
+        }
+        far = value_of(__reduce_max_sync(kAll, key_of(far)));
+        const float off = (a.score == B200_ROUTER_SIGMOID ? 0x1p-20f : 0x1p-17f * inv) + 0x1p-23f * far;
+        bool sure = __all_sync(kAll, finite);
+        if (sure && a.n_group > 1) {
+            const int size = a.E / a.n_group;
+            float * mine = shared + warp * a.n_group * a.pitch;
+#pragma unroll
+            for (int i = 0; i < EPL; i++) {
+                const int e = i * 32 + lane;
+                const int of = group_of(a, e);
+                if (e < a.E) mine[of * a.pitch + e - of * size] = c[i];
+            }
+            __syncwarp();
+            const int g = lane / a.lanes;
+            float b1 = -INFINITY, b2 = -INFINITY;
+            if (g < a.n_group)
+                for (int n = lane % a.lanes; n < size; n += a.lanes) merge2(b1, b2, mine[g * a.pitch + n], -INFINITY);
+            for (int o = a.lanes >> 1; o > 0; o >>= 1) {
+                const float o1 = __shfl_xor_sync(kAll, b1, o), o2 = __shfl_xor_sync(kAll, b2, o);
+                merge2(b1, b2, o1, o2);
+            }
+            __syncwarp();
+            const float score = a.group_top == 2 && size > 1 ? b1 + b2 : b1;
+            // lane n: group n's score, and how many are before it
+            const float s = __shfl_sync(kAll, score, lane < a.n_group ? lane * a.lanes : 0);
+            int ahead = 0;
+            for (int n = 0; n < a.n_group; n++) {
+                const float other = __shfl_sync(kAll, s, n);
+                ahead += other > s || (other == s && n < lane);
+            }
+            const bool in = lane < a.n_group && ahead < a.topk_group;
+            const unsigned kept = __ballot_sync(kAll, in);
+            if (a.topk_group < a.n_group) {
+                const float low = value_of(__reduce_min_sync(kAll, in ? key_of(s) : kAll));
+                const float high = value_of(__reduce_max_sync(kAll, lane < a.n_group && !in ? key_of(s) : 0));
+                sure = low - high > 4.0f * off + 0x1p-22f * fmaxf(fabsf(low), fabsf(high));
+            }
+#pragma unroll
+            for (int i = 0; i < EPL; i++) {
+                const int e = i * 32 + lane;
+                if (e < a.E && !(kept >> group_of(a, e) & 1)) key[i] = 0;
+            }
+        }
+        if (sure) {
+            // one more than the chosen, to see that it lies apart (key 0: there is none)
+            unsigned found = 0;
+            const int left = a.E / a.n_group * a.topk_group, rounds = a.top_k < 32 && a.top_k < left ? a.top_k + 1 : a.top_k;
+            largest<EPL>(key, rounds, id, found);
+            const unsigned next = __shfl_down_sync(kAll, found, 1);
+            const bool apart = lane + 1 >= rounds || value_of(found) - value_of(next) > 2.0f * off;
+            sure = __all_sync(kAll, apart) && (rounds > a.top_k || a.top_k == left);
+        }
+        if (!sure) id = choose_exactly<EPL>(a, row, bias, top);
+    }
+
+    // ---- weights: lane k's is the k-th chosen expert's ----
+    const bool chosen = lane < a.top_k;
+    double mine = chosen ? term(a, clean(row[id]), top) : 0.0;
+    if (a.renorm) {
+        const double total = warp_sum_d(mine);
+        mine = total > 0.0 ? mine / total : 0.0;
+    } else if (a.score == B200_ROUTER_SOFTMAX) {
+        double total = 0.0;
+#pragma unroll
+        for (int i = 0; i < EPL; i++) total += term(a, x[i], top);
+        total = warp_sum_d(total);
+        mine = total > 0.0 ? mine / total : 0.0;
+    }
+    if (chosen) {
         ids[t * a.top_k + lane] = id;
         w[t * a.top_k + lane] = __double2float_rn(mine * (double) a.scale);
     }
@@ -143,14 +303,28 @@ extern "C" b200_status b200_moe_router(b200_context * ctx, void * stream, const 
     if (T > (int64_t) INT32_MAX) return kv_fail(ctx, B200_ERR_INVALID, what, "more than 2^31 rows");
     DeviceScope scope(ctx->device);
     if (scope.status != cudaSuccess) return kv_cuda(ctx, scope.status, what);
-    const RouterParams a{r->n_expert, r->top_k, r->score, r->n_group, r->topk_group, r->group_top, r->renorm, r->scale};
+    RouterParams a{r->n_expert, r->top_k, r->score, r->n_group, r->topk_group, r->group_top, r->renorm, r->scale, 1, 0, 0};
+    size_t smem = 0;
+    if (a.n_group > 1) {
+        const int size = a.E / a.n_group;
+        a.inv = ((1u << 21) + size - 1) / size;  // e * (inv * size - 2^21) < 2^10 2^10, so the quotient is exact
+        while (2 * a.lanes * a.n_group <= 32) a.lanes *= 2;
+        a.pitch = size + (a.lanes - size % 32 + 32) % 32;  // pitch mod 32 = lanes: lane l of a step reads bank l + const
+        smem = (size_t) kWarps * a.n_group * a.pitch * sizeof(float);  // at most 4 * (1024 + 32 * 31) * 4 B < 32 KB
+    }
     cudaStream_t st = stream ? (cudaStream_t) stream : ctx->stream;
-    const unsigned grid = (unsigned) ((T + 3) / 4);
+    const unsigned grid = (unsigned) ((T + kWarps - 1) / kWarps);
+    const bool by_logit = !bias && a.n_group == 1;
+    auto go = [&](auto epl) {
+        constexpr int EPL = decltype(epl)::value;
+        auto kern = by_logit ? moe_router_kernel<EPL, true> : moe_router_kernel<EPL, false>;
+        kern<<<grid, 32 * kWarps, smem, st>>>(a, logits, bias, T, ids, w);
+    };
     const int epl = (a.E + 31) / 32;
-    if (epl <= 2) moe_router_kernel<2><<<grid, 128, 0, st>>>(a, logits, bias, T, ids, w);
-    else if (epl <= 4) moe_router_kernel<4><<<grid, 128, 0, st>>>(a, logits, bias, T, ids, w);
-    else if (epl <= 8) moe_router_kernel<8><<<grid, 128, 0, st>>>(a, logits, bias, T, ids, w);
-    else if (epl <= 16) moe_router_kernel<16><<<grid, 128, 0, st>>>(a, logits, bias, T, ids, w);
-    else moe_router_kernel<32><<<grid, 128, 0, st>>>(a, logits, bias, T, ids, w);
+    if (epl <= 2) go(std::integral_constant<int, 2>{});
+    else if (epl <= 4) go(std::integral_constant<int, 4>{});
+    else if (epl <= 8) go(std::integral_constant<int, 8>{});
+    else if (epl <= 16) go(std::integral_constant<int, 16>{});
+    else go(std::integral_constant<int, 32>{});
     return kv_cuda(ctx, cudaGetLastError(), what);
 }
