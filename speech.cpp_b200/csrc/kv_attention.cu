@@ -39,7 +39,7 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kJoinWarps = 8;
 constexpr int kRows = 8;      // rows of a tile
 constexpr int kChunk = 64;    // positions of a chunk: one 16-position tile per warp
-constexpr float kShift = 15;  // weights are held times 2^15, so that their low halves reach 2^-39 of the largest
+constexpr float kShift = 14;  // weights are held times 2^14, so that their low halves reach 2^-38 of the largest
 
 struct Geometry {
     int n_tok, n_head, group, tiles;  // tiles: row tiles of a key/value head
@@ -68,16 +68,37 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// N 32-bit words from p (aligned to their size) when `there`, else zeros. The cache is read once: not kept in L1.
+// N 32-bit words from p (aligned to their size; N = 3, 8: to one and four words). The cache is read once: not kept in L1.
 template <int N>
-__device__ __forceinline__ void load(uint32_t (&w)[N], const void * p, bool there) {
+__device__ __forceinline__ void load(uint32_t (&w)[N], const uint8_t * p) {
+    if constexpr (N == 4 || N == 8) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+            asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
+                         : "l"(p + 4 * i));
+    } else if constexpr (N == 2) {
+        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(w[i]) : "l"(p + 4 * i));
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void zero(uint32_t (&w)[N]) {
 #pragma unroll
     for (int i = 0; i < N; i++) w[i] = 0;
-    if (!there) return;
-    if constexpr (N == 4)
-        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
-    else if constexpr (N == 2) asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
-    else asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+}
+
+__device__ __forceinline__ __half2 h2(uint32_t w) { return *reinterpret_cast<const __half2 *>(&w); }
+__device__ __forceinline__ uint32_t u32(__half2 h) { return *reinterpret_cast<const uint32_t *>(&h); }
+
+// Half numbers i and j of two rows' scales (kept together in w) as a pair.
+template <int I, int J, int N>
+__device__ __forceinline__ uint32_t pair_of(const uint32_t (&w)[N]) {
+    constexpr uint32_t sel = (I & 1 ? 0x32u : 0x10u) | (J & 1 ? 0x7600u : 0x5400u);
+    return __byte_perm(w[I / 2], w[J / 2], sel);
 }
 
 // (x, y) as two F16 pairs, hi + lo.
@@ -85,15 +106,13 @@ __device__ __forceinline__ void split(float x, float y, uint32_t & hi, uint32_t 
     const __half2 h = __floats2half2_rn(x, y);
     const float2 f = __half22float2(h);
     const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
+    hi = u32(h);
+    lo = u32(l);
 }
 
 // Two of four bytes q + 128 (sel 0x4140: the first two, 0x4342: the last two) as F16 values q: 0x6400 | b is 1024 + b.
 __device__ __forceinline__ uint32_t halves(uint32_t biased, uint32_t sel) {
-    const uint32_t w = __byte_perm(biased, 0x64646464u, sel);
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&w), __float2half2_rn(1152.0f));
-    return *reinterpret_cast<const uint32_t *>(&r);
+    return u32(__hsub2(h2(__byte_perm(biased, 0x64646464u, sel)), __float2half2_rn(1152.0f)));
 }
 
 __device__ __forceinline__ float half_of(const uint32_t * w, int i) {
@@ -244,43 +263,53 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
         __syncthreads();
 
         // ---- this warp's tiles of positions [c0 * 64, c1 * 64) ----
-        const int64_t p_end = c1 * kChunk < len ? c1 * kChunk : len;
-        const int64_t all_see = len - g.n_tok + 1;  // positions below are seen by every row
-        const int64_t seen = row.there ? all_see + row.token : 0;
+        constexpr int kRowBytes = Q8 ? D : 2 * D;
+        const int p_end = (int) (c1 * kChunk < len ? c1 * kChunk : len);
+        const int all_see = (int) len - g.n_tok + 1;  // positions below are seen by every row
+        const int seen = row.there ? all_see + row.token : 0;
+        const int64_t page_bytes = (int64_t) c.n_kv_head * c.page_size * kRowBytes;
+        const int64_t head_bytes = (int64_t) h * c.page_size * kRowBytes;
+        const uint8_t * kl = c.k + head_bytes + gq * kRowBytes + t * (Q8 ? 8 : 16);                      // this lane's bytes of page 0
+        const uint8_t * vl = c.v + head_bytes + 2 * t * kRowBytes + gq * S::kRun * (Q8 ? 1 : 2);
+        const uint8_t * kdl = reinterpret_cast<const uint8_t *>(c.kd) + head_bytes / 16 + t * (D / 8);  // a row's scales: D / 16 bytes
+        const uint8_t * vdl = reinterpret_cast<const uint8_t *>(c.vd) + head_bytes / 16 + t * (D / 8);
+        const int page_step = kChunk / c.page_size, slot_step = kChunk % c.page_size;
         float o[S::kGroups][S::kRun][2] = {}, m = -INFINITY, l = 0.0f;
-        for (int64_t p0 = c0 * kChunk + warp * 16; p0 < p_end; p0 += kWarps * 16) {
-            const int page = kv_page(c, seq, p0 / c.page_size, lane == 0);
+        int p0 = (int) c0 * kChunk + warp * 16;
+        int in_table = p0 / c.page_size, slot = p0 % c.page_size;
+        for (; p0 < p_end; p0 += kChunk) {
+            const int page = kv_page(c, seq, in_table, lane == 0);
+            const int64_t at = page * page_bytes + slot * kRowBytes;
+            in_table += page_step;
+            slot += slot_step;
+            if (slot >= c.page_size) slot -= c.page_size, in_table++;
             if (page < 0) continue;
-            const int here = p_end - p0 < 16 ? (int) (p_end - p0) : 16;  // positions of the tile
-            const int64_t r0 = ((int64_t) page * c.n_kv_head + h) * c.page_size + p0 % c.page_size;
-            const uint8_t * kp = c.k + (r0 + gq) * (Q8 ? D : 2 * D) + t * (Q8 ? 8 : 16);
-            const uint8_t * vp = c.v + (r0 + 2 * t) * (Q8 ? D : 2 * D) + gq * S::kRun * (Q8 ? 1 : 2);
+            const int here = p_end - p0;  // positions of the tile: 16 or more, or its end
+            const bool edge = p0 + 16 > all_see || here < 16;
             uint32_t kw[2][S::kBlocks][S::kKeyWords], vw[4][S::kGroups][S::kValueWords];
             uint32_t kd[2][Q8 ? S::kBlocks : 1], vd[2][Q8 ? S::kBlocks : 1];
+            // keys of positions gq, gq + 8; values of positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9, whose scores this lane holds
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
-                for (int b = 0; b < S::kBlocks; b++)
-                    load(kw[i][b], kp + (int64_t) i * 8 * (Q8 ? D : 2 * D) + b * (Q8 ? 32 : 64), gq + 8 * i < here);
-            // positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9: the ones whose scores this lane holds
+                for (int b = 0; b < S::kBlocks; b++) {
+                    if (edge && gq + 8 * i >= here) zero(kw[i][b]);
+                    else load(kw[i][b], kl + at + i * 8 * kRowBytes + b * (Q8 ? 32 : 64));
+                }
+            if constexpr (Q8) {  // the scales of two neighbouring rows are kBlocks words; the tile's rows all lie in its page
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    load(kd[i], kdl + at / 16 + i * (D / 2));
+                    load(vd[i], vdl + at / 16 + i * (D / 2));
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int n = 0; n < S::kGroups; n++)
-                    load(vw[i][n], vp + (int64_t) ((i & 1) + 8 * (i >> 1)) * (Q8 ? D : 2 * D) + n * 8 * S::kRun * (Q8 ? 1 : 2),
-                         2 * t + (i & 1) + 8 * (i >> 1) < here);
-            if constexpr (Q8) {  // the scales of two neighbouring rows are kBlocks words
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const uint32_t * a = reinterpret_cast<const uint32_t *>(c.kd + (r0 + 2 * t + 8 * i) * S::kBlocks);
-                    const uint32_t * b = reinterpret_cast<const uint32_t *>(c.vd + (r0 + 2 * t + 8 * i) * S::kBlocks);
-#pragma unroll
-                    for (int n = 0; n < S::kBlocks; n++) {
-                        kd[i][n] = __ldg(a + n);
-                        vd[i][n] = __ldg(b + n);
-                    }
+                for (int n = 0; n < S::kGroups; n++) {
+                    if (edge && 2 * t + (i & 1) + 8 * (i >> 1) >= here) zero(vw[i][n]);
+                    else load(vw[i][n], vl + at + ((i & 1) + 8 * (i >> 1)) * kRowBytes + n * 8 * S::kRun * (Q8 ? 1 : 2));
                 }
-            }
 
             // ---- scores: s[2 i + j] is position 2 t + j + 8 i of row gq ----
             float s[4];
@@ -311,7 +340,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) s[i] *= factor;
-            const bool edge = p0 + here > all_see || here < 16;
             if (edge) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -334,29 +362,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
             l = fmaf(l, keep, (p[0] + p[1]) + (p[2] + p[3]));
 
             // ---- o = o keep + P V ----
+            uint32_t pf[4];  // the weights' fragment: hi, lo of positions 2 t, 2 t + 1, then of 2 t + 8, 2 t + 9
+            split(p[0], p[1], pf[0], pf[1]);
+            split(p[2], p[3], pf[2], pf[3]);
             if constexpr (Q8) {
-#pragma unroll
-                for (int b = 0; b < S::kBlocks; b++) {
-                    float d[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) d[i] = half_of(vd[i >> 1], (i & 1) * S::kBlocks + b);
-                    if (here < 16) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (2 * t + (i & 1) + 8 * (i >> 1) >= here) d[i] = 0.0f;
-                    }
-                    float big = fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fabsf(d[3])));
-                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-                    int e = (int) (__float_as_uint(big) >> 23);
-                    if (e == 0 || e == 255) e = 126;
-                    const float up = __uint_as_float((uint32_t) (253 - e) << 23), down = __uint_as_float((uint32_t) (e + 1) << 23);
-                    float w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) w[i] = edge && p[i] == 0.0f ? 0.0f : p[i] * (d[i] * up);
-                    uint32_t a[4];
-                    split(w[0], w[1], a[0], a[1]);
-                    split(w[2], w[3], a[2], a[3]);
+                // one block of 32 dimensions: weights times scales (fragment a), times 2^k and back where `down` is not 1
+                auto block = [&](int b, const uint32_t(&a)[4], auto scaled, float down) {
                     // two rows' four bytes each, interleaved: (row, row + 1) pairs of dimensions 0, 1 and 2, 3
                     const uint32_t x0 = __byte_perm(vw[0][b][0], vw[1][b][0], 0x5140) ^ 0x80808080u;
                     const uint32_t x1 = __byte_perm(vw[0][b][0], vw[1][b][0], 0x7362) ^ 0x80808080u;
@@ -367,43 +378,89 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
                         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                         const uint32_t sel = n & 1 ? 0x4342 : 0x4140;
                         mma(part, a, halves(n < 2 ? x0 : x1, sel), halves(n < 2 ? y0 : y1, sel));
-                        o[b][n][0] = fmaf(o[b][n][0], keep, (part[0] + part[2]) * down);
-                        o[b][n][1] = fmaf(o[b][n][1], keep, (part[1] + part[3]) * down);
+                        part[0] += part[2];
+                        part[1] += part[3];
+                        if constexpr (decltype(scaled)::value) part[0] *= down, part[1] *= down;
+                        o[b][n][0] = fmaf(o[b][n][0], keep, part[0]);
+                        o[b][n][1] = fmaf(o[b][n][1], keep, part[1]);
+                    }
+                };
+                // Scales between 2^-14 and 2 (nearly always all of them) multiply the weights' halves in F16 pairs: the
+                // product's rounding error is exact in F16 and goes to the low half. The weights being up to 2^14 and the low
+                // halves reaching 2^-24, nothing overflows and what is lost is below 2^-24 of the largest weight's product.
+                uint32_t low = vd[0][0], high = vd[0][0];
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int b = 0; b < S::kBlocks; b++) low = __vminu2(low, vd[i][b]), high = __vmaxu2(high, vd[i][b]);
+                const bool plain = (low & 0xffffu) >= 0x0400u && low >= 0x04000000u && (high & 0xffffu) < 0x4000u && high < 0x40000000u;
+                if (__all_sync(0xffffffffu, plain)) {
+                    auto go = [&](auto index) {
+                        constexpr int b = decltype(index)::value;
+                        if constexpr (b < S::kBlocks) {
+                            const __half2 d0 = h2(pair_of<b, S::kBlocks + b>(vd[0])), d1 = h2(pair_of<b, S::kBlocks + b>(vd[1]));
+                            const __half2 w0 = __hmul2_rn(h2(pf[0]), d0), w1 = __hmul2_rn(h2(pf[2]), d1);
+                            const uint32_t a[4] = {u32(w0), u32(__hfma2(h2(pf[1]), d0, __hfma2(h2(pf[0]), d0, __hneg2(w0)))), u32(w1),
+                                                   u32(__hfma2(h2(pf[3]), d1, __hfma2(h2(pf[2]), d1, __hneg2(w1))))};
+                            block(b, a, std::false_type{}, 1.0f);
+                        }
+                    };
+                    go(std::integral_constant<int, 0>{}), go(std::integral_constant<int, 1>{}), go(std::integral_constant<int, 2>{});
+                    go(std::integral_constant<int, 3>{}), go(std::integral_constant<int, 4>{}), go(std::integral_constant<int, 5>{});
+                    go(std::integral_constant<int, 6>{}), go(std::integral_constant<int, 7>{});
+                } else {
+                    // any scales: the product in float32, times a power of two that brings the tile's largest scale below 1
+#pragma unroll
+                    for (int b = 0; b < S::kBlocks; b++) {
+                        float d[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            d[i] = 2 * t + (i & 1) + 8 * (i >> 1) < here ? half_of(vd[i >> 1], (i & 1) * S::kBlocks + b) : 0.0f;
+                        float big = fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fabsf(d[3])));
+                        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                        int e = (int) (__float_as_uint(big) >> 23);
+                        if (e == 0 || e == 255) e = 126;
+                        const float up = __uint_as_float((uint32_t) (253 - e) << 23), down = __uint_as_float((uint32_t) (e + 1) << 23);
+                        float w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) w[i] = edge && p[i] == 0.0f ? 0.0f : p[i] * (d[i] * up);
+                        uint32_t a[4];
+                        split(w[0], w[1], a[0], a[1]);
+                        split(w[2], w[3], a[2], a[3]);
+                        block(b, a, std::true_type{}, down);
                     }
                 }
             } else {
-                uint32_t a[4];
-                split(p[0], p[1], a[0], a[1]);
-                split(p[2], p[3], a[2], a[3]);
-                // Where rows see different positions, a value that is NaN or infinite must not meet the weight 0 of a row that
-                // does not see it: one product per token then, from the last, with the values behind its position zeroed.
-                const bool apart = edge && g.n_tok > 1;
-                const int first = apart ? tile * kRows / g.group : 0;
-                int token = apart ? min((tile * kRows + kRows - 1) / g.group, g.n_tok - 1) : 0;
-                for (; token >= first; token--) {
-                    if (apart) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (p0 + 2 * t + (i & 1) + 8 * (i >> 1) >= all_see + token) {
-#pragma unroll
-                                for (int n = 0; n < S::kGroups; n++)
-#pragma unroll
-                                    for (int w = 0; w < S::kValueWords; w++) vw[i][n][w] = 0;
-                            }
-                    }
-                    const bool mine = !apart || row.token == token;
+                auto product = [&](bool mine) {
 #pragma unroll
                     for (int n = 0; n < S::kGroups; n++)
 #pragma unroll
                         for (int r = 0; r < S::kRun; r++) {
                             float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                             const uint32_t sel = r & 1 ? 0x7632 : 0x5410;
-                            mma(part, a, __byte_perm(vw[0][n][r / 2], vw[1][n][r / 2], sel), __byte_perm(vw[2][n][r / 2], vw[3][n][r / 2], sel));
+                            mma(part, pf, __byte_perm(vw[0][n][r / 2], vw[1][n][r / 2], sel), __byte_perm(vw[2][n][r / 2], vw[3][n][r / 2], sel));
                             if (mine) {
                                 o[n][r][0] = fmaf(o[n][r][0], keep, part[0] + part[2]);
                                 o[n][r][1] = fmaf(o[n][r][1], keep, part[1] + part[3]);
                             }
                         }
+                };
+                if (edge && g.n_tok > 1) {
+                    // Where rows see different positions, a value that is NaN or infinite must not meet the weight 0 of a row
+                    // that does not see it: one product per token, from the last, with the values behind its position zeroed.
+                    const int first = tile * kRows / g.group;
+                    for (int token = min((tile * kRows + kRows - 1) / g.group, g.n_tok - 1); token >= first; token--) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (p0 + 2 * t + (i & 1) + 8 * (i >> 1) >= all_see + token) {
+#pragma unroll
+                                for (int n = 0; n < S::kGroups; n++) zero(vw[i][n]);
+                            }
+                        product(row.token == token);
+                    }
+                } else {
+                    product(true);
                 }
             }
         }
@@ -586,7 +643,7 @@ cudaError_t launch(const KvView & c, const Geometry & g, const float * q, int64_
 
 bool fits(const b200_kv_cache * c, int64_t max_pages, int64_t n_seq, int64_t n_tok, int64_t n_head) {
     return c && c->n_kv_head > 0 && c->page_size > 0 && max_pages >= 0 && n_seq > 0 && n_tok > 0 && n_tok <= 16 && n_head > 0 && n_head <= 65535 &&
-           n_head % c->n_kv_head == 0 && max_pages <= INT32_MAX / c->page_size && n_seq * n_tok <= INT32_MAX / kRows / n_head;
+           n_head % c->n_kv_head == 0 && max_pages <= (1 << 30) / c->page_size && n_seq * n_tok <= INT32_MAX / kRows / n_head;
 }
 
 }  // namespace

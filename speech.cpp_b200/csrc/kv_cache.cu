@@ -35,7 +35,7 @@ b200_status kv_checked_view(b200_context * ctx, const char * what, const b200_kv
     if (c->device != ctx->device) return kv_fail(ctx, B200_ERR_INVALID, what, "the cache lies on another device than the context");
     if (n_seq < 0 || n_tok < 0 || max_pages < 0) return kv_fail(ctx, B200_ERR_INVALID, what, "a negative size");
     if (n_seq > 0 && n_tok > 0 && (!lens || (max_pages > 0 && !table))) return kv_fail(ctx, B200_ERR_INVALID, what, "NULL table or lens");
-    if (max_pages > INT32_MAX / c->page_size) return kv_fail(ctx, B200_ERR_INVALID, what, "max_pages * page_size passes 2^31");
+    if (max_pages > (1 << 30) / c->page_size) return kv_fail(ctx, B200_ERR_INVALID, what, "max_pages * page_size passes 2^30");
     // one CTA per row (or fewer) in a one-dimensional grid
     if (n_tok > 0 && n_seq > INT32_MAX / n_tok) return kv_fail(ctx, B200_ERR_INVALID, what, "n_seq * n_tok passes 2^31");
     const uint8_t * base = (const uint8_t *) c->data;
