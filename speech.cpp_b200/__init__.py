@@ -248,6 +248,8 @@ def _ptr(t):
 class Context:
     """One B200 device, one stream, a scratch pool (b200_context)."""
 
+    _raw_stream = None
+
     def __init__(self, device=0):
         self.L = lib()
         self.device = device
@@ -433,37 +435,46 @@ class Context:
         return out
 
     # -- paged key/value cache and expert router (torch CUDA tensors; run on torch's current stream) ------------------
+    # A decode step calls these once per layer, so their checks read each attribute of a tensor once and build texts only for
+    # an error.
     def _stream(self):
         """torch's current stream of this device as a cudaStream_t (the default stream as cudaStreamLegacy, since NULL
         means the context's own stream). These calls use nothing of the context's stream, so they run in torch's order."""
-        import torch
+        if self._raw_stream is None:
+            import torch
 
-        return torch.cuda.current_stream(self.device).cuda_stream or 1
+            # the handle alone, where torch has it: a Stream object costs a microsecond more per call
+            self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+        return self._raw_stream(self.device) or 1
 
-    def _arg(self, t, what, dtype, shape=None):
-        """The address of a contiguous CUDA tensor of this device, type and shape."""
-        if not t.is_cuda or t.device.index != self.device:
+    def _refuse(self, t, what, wanted):
+        if not t.is_cuda or t.get_device() != self.device:
             raise ValueError(f"{what}: expected a tensor on cuda:{self.device}, got one on {t.device}")
-        if t.dtype != dtype or (shape is not None and t.shape != shape) or not t.is_contiguous():
-            raise ValueError(f"{what}: expected a contiguous {dtype} tensor{'' if shape is None else f' of shape {tuple(shape)}'}, "
-                             f"got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+        raise ValueError(f"{what}: expected {wanted}, got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+
+    def _arg(self, t, what, dtype, shape):
+        """The address of a contiguous CUDA tensor of this device, type and shape."""
+        if not t.is_cuda or t.get_device() != self.device or t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+            self._refuse(t, what, f"a contiguous {dtype} tensor of shape {tuple(shape)}")
         return t.data_ptr()
 
-    def _row_arg(self, t, what, heads, dim):
+    def _row_arg(self, t, what, shape):
         """(address, row stride) of float32 rows [n_seq, n_tok, heads, dim] whose heads lie contiguous in each row and whose
         rows lie at one stride (a slice of the columns of a wider product is taken as it is)."""
         import torch
 
-        if not t.is_cuda or t.device.index != self.device:
-            raise ValueError(f"{what}: expected a tensor on cuda:{self.device}, got one on {t.device}")
-        if t.dtype != torch.float32 or t.dim() != 4 or t.shape[2] != heads or t.shape[3] != dim:
-            raise ValueError(f"{what}: expected float32 [n_seq, n_tok, {heads}, {dim}], got {t.dtype} {tuple(t.shape)}")
-        n_seq, n_tok = t.shape[:2]
-        s = t.stride()
-        ld = s[1] if n_tok > 1 else s[0] if n_seq > 1 else heads * dim
-        if t.numel() and (s[3] != 1 or (heads > 1 and s[2] != dim) or ld < heads * dim or (n_seq > 1 and s[0] != n_tok * ld)):
-            raise ValueError(f"{what}: the rows' heads are not contiguous or the rows lie at no single stride (strides {s})")
-        return t.data_ptr(), max(ld, heads * dim)
+        n_seq, n_tok, heads, dim = shape
+        width = heads * dim
+        if t.dtype == torch.float32 and t.shape == shape and t.is_cuda and t.get_device() == self.device:
+            if t.is_contiguous():
+                return t.data_ptr(), width
+            s = t.stride()
+            ld = s[1] if n_tok > 1 else s[0]
+            if s[3] == 1 and (heads == 1 or s[2] == dim) and ld >= width and (n_seq == 1 or s[0] == n_tok * ld):
+                return t.data_ptr(), ld
+            if n_seq == 1 and n_tok == 1 and s[3] == 1 and (heads == 1 or s[2] == dim):  # one row: it has no stride
+                return t.data_ptr(), width
+        self._refuse(t, what, f"float32 {tuple(shape)} with contiguous heads and one row stride")
 
     def kv_cache(self, qtype, n_kv_head, head_dim, page_size, n_pages, data=None):
         """A paged key/value cache of type F16 or Q8_0 (b200_kv_cache); data: a CUDA uint8 tensor to lay it out in
@@ -471,26 +482,27 @@ class Context:
         return KvCache(self, qtype, n_kv_head, head_dim, page_size, n_pages, data)
 
     def _kv_open(self, cache, what):
-        if cache.ctx is not self or not cache.s.n_pages:
+        if cache.ctx is not self or not cache.open:
             raise ValueError(f"{what}: the cache is closed or belongs to another context")
 
-    def _kv_places(self, cache, table, lens, n_seq, what):
+    def _kv_places(self, table, lens, n_seq, what):
+        """(table's address, its width, the lengths' address)."""
         import torch
 
         if table.dim() != 2:
-            raise ValueError(f"{what}: expected a table [n_seq, max_pages], got {tuple(table.shape)}")
-        return self._arg(table, what + " table", torch.int32, (n_seq, table.shape[1])), table.shape[1], self._arg(lens, what + " lens", torch.int32, (n_seq,))
+            self._refuse(table, what + " table", "int32 [n_seq, max_pages]")
+        width = table.shape[1]
+        return self._arg(table, what, torch.int32, (n_seq, width)), width, self._arg(lens, what, torch.int32, (n_seq,))
 
     def kv_write(self, cache, k, v, table, lens):
         """Writes rows k, v float32 [n_seq, n_tok, n_kv_head, head_dim] at positions lens[s] - n_tok + r (b200_kv_write);
         table int32 [n_seq, max_pages], lens int32 [n_seq] (the lengths with these rows)."""
         self._kv_open(cache, "kv_write")
-        kp, ldk = self._row_arg(k, "kv_write k", cache.s.n_kv_head, cache.s.head_dim)
-        vp, ldv = self._row_arg(v, "kv_write v", cache.s.n_kv_head, cache.s.head_dim)
         n_seq, n_tok = k.shape[:2]
-        if v.shape != k.shape:
-            raise ValueError(f"kv_write: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
-        tp, mp, lp = self._kv_places(cache, table, lens, n_seq, "kv_write")
+        shape = (n_seq, n_tok, cache.n_kv_head, cache.head_dim)
+        kp, ldk = self._row_arg(k, "kv_write k", shape)
+        vp, ldv = self._row_arg(v, "kv_write v", shape)
+        tp, mp, lp = self._kv_places(table, lens, n_seq, "kv_write table and lens")
         self.check(self.L.b200_kv_write(self.h, self._stream(), cache.ref, tp, mp, lp, n_seq, n_tok, kp, ldk, vp, ldv))
 
     def kv_read(self, cache, table, lens, n_tok=None, start=None, dtype=None, k=None, v=None):
@@ -504,19 +516,20 @@ class Context:
         if (k is None) != (v is None) or (k is None and n_tok is None):
             raise ValueError("kv_read: give both k and v, or n_tok")
         if k is None:
-            shape = (n_seq, n_tok, cache.s.n_kv_head, cache.s.head_dim)
+            shape = (n_seq, n_tok, cache.n_kv_head, cache.head_dim)
             k, v = (torch.zeros(shape, dtype=dtype or torch.float32, device=lens.device) for _ in range(2))
         else:
             n_tok = k.shape[1] if n_tok is None else n_tok
-            shape = (n_seq, n_tok, cache.s.n_kv_head, cache.s.head_dim)
-            if dtype is not None and dtype != k.dtype:
-                raise ValueError(f"kv_read: k is {k.dtype}, not {dtype}")
-        if k.dtype not in (torch.float32, torch.float16):
-            raise ValueError(f"kv_read: rows are float32 or float16, not {k.dtype}")
-        kp, vp = self._arg(k, "kv_read k", k.dtype, shape), self._arg(v, "kv_read v", k.dtype, shape)
+            shape = (n_seq, n_tok, cache.n_kv_head, cache.head_dim)
+        kind = k.dtype
+        if dtype is not None and dtype != kind:
+            raise ValueError(f"kv_read: k is {kind}, not {dtype}")
+        if kind != torch.float32 and kind != torch.float16:
+            raise ValueError(f"kv_read: rows are float32 or float16, not {kind}")
+        kp, vp = self._arg(k, "kv_read k", kind, shape), self._arg(v, "kv_read v", kind, shape)
         sp = None if start is None else self._arg(start, "kv_read start", torch.int32, (n_seq,))
-        tp, mp, lp = self._kv_places(cache, table, lens, n_seq, "kv_read")
-        self.check(self.L.b200_kv_read(self.h, self._stream(), cache.ref, tp, mp, lp, sp, n_seq, n_tok, F16 if k.dtype == torch.float16 else F32, kp, vp))
+        tp, mp, lp = self._kv_places(table, lens, n_seq, "kv_read table and lens")
+        self.check(self.L.b200_kv_read(self.h, self._stream(), cache.ref, tp, mp, lp, sp, n_seq, n_tok, F16 if kind == torch.float16 else F32, kp, vp))
         return k, v
 
     def kv_attention(self, cache, q, table, lens, scale, out=None):
@@ -525,15 +538,20 @@ class Context:
         import torch
 
         self._kv_open(cache, "kv_attention")
-        if q.dim() != 4:
-            raise ValueError(f"kv_attention: expected q [n_seq, n_tok, n_head, head_dim], got {tuple(q.shape)}")
-        n_seq, n_tok, n_head, dim = q.shape
-        qp, ldq = self._row_arg(q, "kv_attention q", n_head, cache.s.head_dim)
-        tp, mp, lp = self._kv_places(cache, table, lens, n_seq, "kv_attention")
+        shape = q.shape
+        if len(shape) != 4:
+            raise ValueError(f"kv_attention: expected q [n_seq, n_tok, n_head, head_dim], got {tuple(shape)}")
+        n_seq, n_tok, n_head = shape[:3]
+        qp, ldq = self._row_arg(q, "kv_attention q", (n_seq, n_tok, n_head, cache.head_dim))
+        tp, mp, lp = self._kv_places(table, lens, n_seq, "kv_attention table and lens")
         if out is None:
-            out = torch.empty((n_seq, n_tok, n_head, dim), dtype=torch.float32, device=q.device)
-        op = self._arg(out, "kv_attention out", torch.float32, q.shape)
-        size = self.L.b200_kv_attention_workspace(self.h, cache.ref, mp, n_seq, n_tok, n_head)
+            out = torch.empty(shape, dtype=torch.float32, device=q.device)
+            op = out.data_ptr()
+        else:
+            op = self._arg(out, "kv_attention out", torch.float32, shape)
+        size = cache.workspaces.get((mp, n_seq, n_tok, n_head))
+        if size is None:
+            size = cache.workspaces[mp, n_seq, n_tok, n_head] = self.L.b200_kv_attention_workspace(self.h, cache.ref, mp, n_seq, n_tok, n_head)
         # the workspace comes from torch's allocator: reused in stream order, and a captured graph has its own
         ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
         self.check(self.L.b200_kv_attention(self.h, self._stream(), cache.ref, tp, mp, lp, n_seq, n_tok, n_head, qp, ldq, scale, op,
@@ -550,13 +568,14 @@ class Context:
             raise ValueError(f"moe_router: unknown score {score!r}")
         if logits.dim() != 2:
             raise ValueError(f"moe_router: expected logits [T, n_expert], got {tuple(logits.shape)}")
-        T, E = logits.shape
-        lp = self._arg(logits, "moe_router logits", torch.float32)
+        T, E = shape = logits.shape
+        lp = self._arg(logits, "moe_router logits", torch.float32, shape)
         bp = None if bias is None else self._arg(bias, "moe_router bias", torch.float32, (E,))
         r = Router(E, top_k, ROUTER_SIGMOID if score == "sigmoid" else ROUTER_SOFTMAX, n_group, topk_group, group_top, bool(renorm), scale)
-        ids = torch.empty((T, top_k), dtype=torch.int32, device=logits.device) if ids is None else ids
-        w = torch.empty((T, top_k), dtype=torch.float32, device=logits.device) if w is None else w
-        ip, wp = self._arg(ids, "moe_router ids", torch.int32, (T, top_k)), self._arg(w, "moe_router w", torch.float32, (T, top_k))
+        chosen = (T, top_k)
+        ids = torch.empty(chosen, dtype=torch.int32, device=logits.device) if ids is None else ids
+        w = torch.empty(chosen, dtype=torch.float32, device=logits.device) if w is None else w
+        ip, wp = self._arg(ids, "moe_router ids", torch.int32, chosen), self._arg(w, "moe_router w", torch.float32, chosen)
         self.check(self.L.b200_moe_router(self.h, self._stream(), ctypes.byref(r), lp, bp, T, ip, wp))
         return ids, w
 
@@ -578,14 +597,18 @@ class KvCache:
         self.ctx = ctx
         self.s = KvCacheStruct()
         self.ref = ctypes.byref(self.s)
+        self.open = False
         self.data = data  # a view keeps its memory
+        self.workspaces = {}  # b200_kv_attention_workspace by (max_pages, n_seq, n_tok, n_head)
         if data is None:
             ctx.check(ctx.L.b200_kv_cache_alloc(ctx.h, qtype, n_kv_head, head_dim, page_size, n_pages, self.ref))
         else:
             import torch
 
-            ctx.check(ctx.L.b200_kv_cache_view(ctx.h, qtype, n_kv_head, head_dim, page_size, n_pages, ctx._arg(data, "kv_cache data", torch.uint8),
-                                               data.numel(), self.ref))
+            at = ctx._arg(data, "kv_cache data", torch.uint8, data.shape)
+            ctx.check(ctx.L.b200_kv_cache_view(ctx.h, qtype, n_kv_head, head_dim, page_size, n_pages, at, data.numel(), self.ref))
+        self.n_kv_head, self.head_dim = self.s.n_kv_head, self.s.head_dim
+        self.open = True
         ctx._children.add(self)
 
     @property
@@ -594,9 +617,9 @@ class KvCache:
 
     def close(self):
         # the cache's memory is freed while its context is alive (the context closes its caches first)
-        if self.s.data and getattr(self.ctx, "h", None):
+        if self.open and getattr(self.ctx, "h", None):
             self.ctx.check(self.ctx.L.b200_kv_cache_free(self.ctx.h, self.ref))
-        self.s.data, self.s.n_pages = None, 0
+        self.open = False
         self.data = None
 
     def __del__(self):

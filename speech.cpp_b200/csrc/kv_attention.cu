@@ -26,6 +26,8 @@
 // warps take turns at 16-position tiles of a run and join at its end. Items that lie within one CTA's run are finished by it;
 // of the others each CTA leaves a partial (m, l, o) in the workspace, and a second kernel, launched with programmatic
 // dependent launch, joins them.
+#include <cooperative_groups.h>
+
 #include <cmath>
 
 #include "kv.cuh"
@@ -39,13 +41,15 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kJoinWarps = 8;
 constexpr int kRows = 8;      // rows of a tile
 constexpr int kChunk = 64;    // positions of a chunk: one 16-position tile per warp
+constexpr int kItemChunks = 8;  // chunks per CTA up to which the work is cut by items
 constexpr float kShift = 14;  // weights are held times 2^14, so that their low halves reach 2^-38 of the largest
 
 struct Geometry {
     int n_tok, n_head, group, tiles;  // tiles: row tiles of a key/value head
     int64_t items;                    // n_kv_head * tiles, per sequence
     int64_t n_seq;
-    int64_t ctas;                     // CTAs among which the chunks are divided
+    int64_t ctas;                     // CTAs among which the chunks are divided, or
+    int cluster;                      // CTAs that share an item (0: the work is cut by positions)
 };
 
 // CTAs per SM, by what registers allow (__launch_bounds__ holds the compiler to it).
@@ -199,16 +203,302 @@ __device__ __forceinline__ Row row_of(const Geometry & g, int h, int tile, int i
     return {n / g.group, h * g.group + n % g.group, n < g.n_tok * g.group};
 }
 
+// What a CTA holds while it works on one item.
+template <int D>
+struct Shared {
+    __align__(16) uint32_t sq[D / 16][32][4];  // the query tile as fragments
+    float so[kWarps][kRows][D + 4];            // the warps' results
+    float sm[kWarps][kRows], sl[kWarps][kRows];
+};
+
+// Chunks [c0, c1) of one item: the warps' m, l and o are left in shared memory (synchronised).
+template <bool Q8, int D>
+__device__ __forceinline__ void attend(const KvView & c, const Geometry & g, const float * __restrict__ q, int64_t ldq, float scale, Shared<D> & sh,
+                                       int64_t seq, int64_t len, int h, int tile, int64_t c0, int64_t c1) {
+    using S = Shape<Q8, D>;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int gq = lane >> 2, t = lane & 3;  // the fragment's group and thread in it
+    const Row row = row_of(g, h, tile, gq);
+
+    // ---- the query tile: each warp makes the fragments of its share of the k steps ----
+    // k step 2 j + b of lane (gq, t) holds dimensions 32 j + 8 t + 4 b .. + 3 of row gq: hi in registers 0 and 2, lo in
+    // 1 and 3. The row is scaled by 2^k to a largest magnitude in [2^14, 2^15).
+    float factor;  // what a raw score is multiplied by: scale log2(e) 2^-k
+    {
+        const float * src = q + (seq * g.n_tok + row.token) * ldq + (int64_t) row.head * D + 8 * t;
+        float x[D / 4], top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 4; i++) {
+            x[i] = row.there ? src[(i / 8) * 32 + i % 8] : 0.0f;
+            top = fmaxf(top, fabsf(x[i]));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = (int) (__float_as_uint(top) >> 23);
+        const int k = e == 255 || top == 0.0f ? 0 : 141 - e < 126 ? 141 - e : 126;
+        const float up = __uint_as_float((uint32_t) (k + 127) << 23);
+        factor = scale * 1.4426950408889634f * __uint_as_float((uint32_t) (127 - k) << 23);
+#pragma unroll
+        for (int j = 0; j < D / 16; j++) {
+            if (j % kWarps != warp) continue;
+            uint32_t hi[2], lo[2];
+            split(x[4 * j] * up, x[4 * j + 1] * up, hi[0], lo[0]);
+            split(x[4 * j + 2] * up, x[4 * j + 3] * up, hi[1], lo[1]);
+            *reinterpret_cast<uint4 *>(sh.sq[j][lane]) = make_uint4(hi[0], lo[0], hi[1], lo[1]);
+        }
+    }
+    __syncthreads();
+
+    // ---- this warp's tiles of positions [c0 * 64, c1 * 64) ----
+    constexpr int kRowBytes = Q8 ? D : 2 * D;
+    const int p_end = (int) (c1 * kChunk < len ? c1 * kChunk : len);
+    const int all_see = (int) len - g.n_tok + 1;  // positions below are seen by every row
+    const int seen = row.there ? all_see + row.token : 0;
+    const int64_t page_bytes = (int64_t) c.n_kv_head * c.page_size * kRowBytes;
+    const int64_t head_bytes = (int64_t) h * c.page_size * kRowBytes;
+    const uint8_t * kl = c.k + head_bytes + gq * kRowBytes + t * (Q8 ? 8 : 16);                      // this lane's bytes of page 0
+    const uint8_t * vl = c.v + head_bytes + 2 * t * kRowBytes + gq * S::kRun * (Q8 ? 1 : 2);
+    const uint8_t * kdl = reinterpret_cast<const uint8_t *>(c.kd) + head_bytes / 16 + t * (D / 8);  // a row's scales: D / 16 bytes
+    const uint8_t * vdl = reinterpret_cast<const uint8_t *>(c.vd) + head_bytes / 16 + t * (D / 8);
+    const int page_step = kChunk / c.page_size, slot_step = kChunk % c.page_size;
+    float o[S::kGroups][S::kRun][2] = {}, m = -INFINITY, l = 0.0f;
+    int p0 = (int) c0 * kChunk + warp * 16;
+    int in_table = p0 / c.page_size, slot = p0 % c.page_size;
+    for (; p0 < p_end; p0 += kChunk) {
+        const int page = kv_page(c, seq, in_table, lane == 0);
+        const int64_t at = page * page_bytes + slot * kRowBytes;
+        in_table += page_step;
+        slot += slot_step;
+        if (slot >= c.page_size) slot -= c.page_size, in_table++;
+        if (page < 0) continue;
+        const int here = p_end - p0;  // positions of the tile: 16 or more, or its end
+        const bool edge = p0 + 16 > all_see || here < 16;
+        uint32_t kw[2][S::kBlocks][S::kKeyWords], vw[4][S::kGroups][S::kValueWords];
+        uint32_t kd[2][Q8 ? S::kBlocks : 1], vd[2][Q8 ? S::kBlocks : 1];
+        // keys of positions gq, gq + 8; values of positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9, whose scores this lane holds
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int b = 0; b < S::kBlocks; b++) {
+                if (edge && gq + 8 * i >= here) zero(kw[i][b]);
+                else load(kw[i][b], kl + at + i * 8 * kRowBytes + b * (Q8 ? 32 : 64));
+            }
+        if constexpr (Q8) {  // the scales of two neighbouring rows are kBlocks words; the tile's rows all lie in its page
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                load(kd[i], kdl + at / 16 + i * (D / 2));
+                load(vd[i], vdl + at / 16 + i * (D / 2));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int n = 0; n < S::kGroups; n++) {
+                if (edge && 2 * t + (i & 1) + 8 * (i >> 1) >= here) zero(vw[i][n]);
+                else load(vw[i][n], vl + at + ((i & 1) + 8 * (i >> 1)) * kRowBytes + n * 8 * S::kRun * (Q8 ? 1 : 2));
+            }
+
+        // ---- scores: s[2 i + j] is position 2 t + j + 8 i of row gq ----
+        float s[4];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            s[2 * i] = s[2 * i + 1] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < S::kBlocks; b++) {
+                const uint4 a0 = *reinterpret_cast<const uint4 *>(sh.sq[2 * b][lane]), a1 = *reinterpret_cast<const uint4 *>(sh.sq[2 * b + 1][lane]);
+                const uint32_t f0[4] = {a0.x, a0.y, a0.z, a0.w}, f1[4] = {a1.x, a1.y, a1.z, a1.w};
+                if constexpr (Q8) {
+                    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    const uint32_t w0 = kw[i][b][0] ^ 0x80808080u, w1 = kw[i][b][1] ^ 0x80808080u;
+                    mma(part, f0, halves(w0, 0x4140), halves(w0, 0x4342));
+                    mma(part, f1, halves(w1, 0x4140), halves(w1, 0x4342));
+                    s[2 * i] = fmaf(half_of(kd[i], b), part[0] + part[2], s[2 * i]);
+                    s[2 * i + 1] = fmaf(half_of(kd[i], S::kBlocks + b), part[1] + part[3], s[2 * i + 1]);
+                } else {
+                    mma(sum, f0, kw[i][b][0], kw[i][b][1]);
+                    mma(sum, f1, kw[i][b][2], kw[i][b][3]);
+                }
+            }
+            if constexpr (!Q8) {
+                s[2 * i] = sum[0] + sum[2];
+                s[2 * i + 1] = sum[1] + sum[3];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[i] *= factor;
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int j = 2 * t + (i & 1) + 8 * (i >> 1);
+                if (j >= here || p0 + j >= seen) s[i] = -INFINITY;
+            }
+        }
+
+        // ---- weights: m is the running maximum less kShift (-infinity before any score) ----
+        float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float m_new = fmaxf(m, top - kShift);
+        const float base = m_new == -INFINITY ? 0.0f : m_new;
+        const float keep = ex2(m - base);
+        m = m_new;
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) p[i] = ex2(s[i] - base);
+        l = fmaf(l, keep, (p[0] + p[1]) + (p[2] + p[3]));
+
+        // ---- o = o keep + P V ----
+        uint32_t pf[4];  // the weights' fragment: hi, lo of positions 2 t, 2 t + 1, then of 2 t + 8, 2 t + 9
+        split(p[0], p[1], pf[0], pf[1]);
+        split(p[2], p[3], pf[2], pf[3]);
+        if constexpr (Q8) {
+            // one block of 32 dimensions: weights times scales (fragment a), times 2^k and back where `down` is not 1
+            auto block = [&](int b, const uint32_t(&a)[4], auto scaled, float down) {
+                // two rows' four bytes each, interleaved: (row, row + 1) pairs of dimensions 0, 1 and 2, 3
+                const uint32_t x0 = __byte_perm(vw[0][b][0], vw[1][b][0], 0x5140) ^ 0x80808080u;
+                const uint32_t x1 = __byte_perm(vw[0][b][0], vw[1][b][0], 0x7362) ^ 0x80808080u;
+                const uint32_t y0 = __byte_perm(vw[2][b][0], vw[3][b][0], 0x5140) ^ 0x80808080u;
+                const uint32_t y1 = __byte_perm(vw[2][b][0], vw[3][b][0], 0x7362) ^ 0x80808080u;
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    const uint32_t sel = n & 1 ? 0x4342 : 0x4140;
+                    mma(part, a, halves(n < 2 ? x0 : x1, sel), halves(n < 2 ? y0 : y1, sel));
+                    part[0] += part[2];
+                    part[1] += part[3];
+                    if constexpr (decltype(scaled)::value) part[0] *= down, part[1] *= down;
+                    o[b][n][0] = fmaf(o[b][n][0], keep, part[0]);
+                    o[b][n][1] = fmaf(o[b][n][1], keep, part[1]);
+                }
+            };
+            // Scales between 2^-14 and 2 (nearly always all of them) multiply the weights' halves in F16 pairs: the
+            // product's rounding error is exact in F16 and goes to the low half. The weights being up to 2^14 and the low
+            // halves reaching 2^-24, nothing overflows and what is lost is below 2^-24 of the largest weight's product.
+            uint32_t low = vd[0][0], high = vd[0][0];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int b = 0; b < S::kBlocks; b++) low = __vminu2(low, vd[i][b]), high = __vmaxu2(high, vd[i][b]);
+            const bool plain = (low & 0xffffu) >= 0x0400u && low >= 0x04000000u && (high & 0xffffu) < 0x4000u && high < 0x40000000u;
+            if (__all_sync(0xffffffffu, plain)) {
+                auto go = [&](auto index) {
+                    constexpr int b = decltype(index)::value;
+                    if constexpr (b < S::kBlocks) {
+                        const __half2 d0 = h2(pair_of<b, S::kBlocks + b>(vd[0])), d1 = h2(pair_of<b, S::kBlocks + b>(vd[1]));
+                        const __half2 w0 = __hmul2_rn(h2(pf[0]), d0), w1 = __hmul2_rn(h2(pf[2]), d1);
+                        const uint32_t a[4] = {u32(w0), u32(__hfma2(h2(pf[1]), d0, __hfma2(h2(pf[0]), d0, __hneg2(w0)))), u32(w1),
+                                               u32(__hfma2(h2(pf[3]), d1, __hfma2(h2(pf[2]), d1, __hneg2(w1))))};
+                        block(b, a, std::false_type{}, 1.0f);
+                    }
+                };
+                go(std::integral_constant<int, 0>{}), go(std::integral_constant<int, 1>{}), go(std::integral_constant<int, 2>{});
+                go(std::integral_constant<int, 3>{}), go(std::integral_constant<int, 4>{}), go(std::integral_constant<int, 5>{});
+                go(std::integral_constant<int, 6>{}), go(std::integral_constant<int, 7>{});
+            } else {
+                // any scales: the product in float32, times a power of two that brings the tile's largest scale below 1
+#pragma unroll
+                for (int b = 0; b < S::kBlocks; b++) {
+                    float d[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        d[i] = 2 * t + (i & 1) + 8 * (i >> 1) < here ? half_of(vd[i >> 1], (i & 1) * S::kBlocks + b) : 0.0f;
+                    float big = fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fabsf(d[3])));
+                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                    int e = (int) (__float_as_uint(big) >> 23);
+                    if (e == 0 || e == 255) e = 126;
+                    const float up = __uint_as_float((uint32_t) (253 - e) << 23), down = __uint_as_float((uint32_t) (e + 1) << 23);
+                    float w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) w[i] = edge && p[i] == 0.0f ? 0.0f : p[i] * (d[i] * up);
+                    uint32_t a[4];
+                    split(w[0], w[1], a[0], a[1]);
+                    split(w[2], w[3], a[2], a[3]);
+                    block(b, a, std::true_type{}, down);
+                }
+            }
+        } else {
+            auto product = [&](bool mine) {
+#pragma unroll
+                for (int n = 0; n < S::kGroups; n++)
+#pragma unroll
+                    for (int r = 0; r < S::kRun; r++) {
+                        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        const uint32_t sel = r & 1 ? 0x7632 : 0x5410;
+                        mma(part, pf, __byte_perm(vw[0][n][r / 2], vw[1][n][r / 2], sel), __byte_perm(vw[2][n][r / 2], vw[3][n][r / 2], sel));
+                        if (mine) {
+                            o[n][r][0] = fmaf(o[n][r][0], keep, part[0] + part[2]);
+                            o[n][r][1] = fmaf(o[n][r][1], keep, part[1] + part[3]);
+                        }
+                    }
+            };
+            if (edge && g.n_tok > 1) {
+                // Where rows see different positions, a value that is NaN or infinite must not meet the weight 0 of a row
+                // that does not see it: one product per token, from the last, with the values behind its position zeroed.
+                const int first = tile * kRows / g.group;
+                for (int token = min((tile * kRows + kRows - 1) / g.group, g.n_tok - 1); token >= first; token--) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (p0 + 2 * t + (i & 1) + 8 * (i >> 1) >= all_see + token) {
+#pragma unroll
+                            for (int n = 0; n < S::kGroups; n++) zero(vw[i][n]);
+                        }
+                    product(row.token == token);
+                }
+            } else {
+                product(true);
+            }
+        }
+    }
+
+    // ---- join the warps ----
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (t == 0) {
+        sh.sm[warp][gq] = m;
+        sh.sl[warp][gq] = l;
+    }
+#pragma unroll
+    for (int n = 0; n < S::kGroups; n++)
+#pragma unroll
+        for (int r = 0; r < S::kRun; r++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) sh.so[warp][gq][n * 8 * S::kRun + (2 * t + j) * S::kRun + r] = o[n][r][j];
+    __syncthreads();
+}
+
+// The CTA's sum of the warps' results for one row: the factors of the warps, and m and l.
+template <int D>
+struct Joined {
+    float f[kWarps], m, l;
+    __device__ __forceinline__ Joined(const Shared<D> & sh, int i) {
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) m = fmaxf(m, sh.sm[w][i]);
+        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            f[w] = ex2(sh.sm[w][i] - base);
+            l = fmaf(sh.sl[w][i], f[w], l);
+        }
+    }
+    __device__ __forceinline__ float value(const Shared<D> & sh, int i, int d) const {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) v = fmaf(sh.so[w][i][d], f[w], v);
+        return v;
+    }
+};
+
+// The work cut by positions: CTA b takes chunks [b share, (b + 1) share) of all items' chunks.
 template <bool Q8, int D>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
     kv_attention_kernel(KvView c, Geometry g, const float * __restrict__ q, int64_t ldq, float scale, float * __restrict__ out, float * __restrict__ ws) {
-    using S = Shape<Q8, D>;
-    __shared__ __align__(16) uint32_t sq[D / 16][32][4];  // the query tile as fragments
-    __shared__ float so[kWarps][kRows][D + 4];            // the warps' results
-    __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
+    __shared__ Shared<D> sh;
     __shared__ int64_t red[kWarps + 2];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int gq = lane >> 2, t = lane & 3;  // the fragment's group and thread in it
+    const int tid = threadIdx.x;
     pdl_launch_dependents();
 
     const int64_t total = block_chunks(c, g.n_seq, red) * g.items;
@@ -231,287 +521,63 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
         const int64_t c1 = c0 + (end - at) < chunks ? c0 + (end - at) : chunks;
         at += c1 - c0;
         const int h = (int) (item / g.tiles), tile = (int) (item % g.tiles);
-        const Row row = row_of(g, h, tile, gq);
+        attend<Q8, D>(c, g, q, ldq, scale, sh, seq, len, h, tile, c0, c1);
 
-        // ---- the query tile: each warp makes the fragments of its share of the k steps ----
-        // k step 2 j + b of lane (gq, t) holds dimensions 32 j + 8 t + 4 b .. + 3 of row gq: hi in registers 0 and 2, lo in
-        // 1 and 3. The row is scaled by 2^k to a largest magnitude in [2^14, 2^15).
-        float factor;  // what a raw score is multiplied by: scale log2(e) 2^-k
-        {
-            const float * src = q + (seq * g.n_tok + row.token) * ldq + (int64_t) row.head * D + 8 * t;
-            float x[D / 4], top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < D / 4; i++) {
-                x[i] = row.there ? src[(i / 8) * 32 + i % 8] : 0.0f;
-                top = fmaxf(top, fabsf(x[i]));
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = (int) (__float_as_uint(top) >> 23);
-            const int k = e == 255 || top == 0.0f ? 0 : 141 - e < 126 ? 141 - e : 126;
-            const float up = __uint_as_float((uint32_t) (k + 127) << 23);
-            factor = scale * 1.4426950408889634f * __uint_as_float((uint32_t) (127 - k) << 23);
-#pragma unroll
-            for (int j = 0; j < D / 16; j++) {
-                if (j % kWarps != warp) continue;
-                uint32_t hi[2], lo[2];
-                split(x[4 * j] * up, x[4 * j + 1] * up, hi[0], lo[0]);
-                split(x[4 * j + 2] * up, x[4 * j + 3] * up, hi[1], lo[1]);
-                *reinterpret_cast<uint4 *>(sq[j][lane]) = make_uint4(hi[0], lo[0], hi[1], lo[1]);
+        const int i = tid / 16;  // a row per 16 threads
+        const Joined<D> all(sh, i);
+        const Row row = row_of(g, h, tile, i);
+        if (c0 == 0 && c1 == chunks) {  // the whole item
+            const float inv = all.l != 0.0f ? 1.0f / all.l : 0.0f;
+            if (row.there)
+                for (int d = tid & 15; d < D; d += 16) out[((seq * g.n_tok + row.token) * g.n_head + row.head) * D + d] = all.value(sh, i, d) * inv;
+        } else {  // the CTA's first partial (of an item begun before it) or its last
+            float * to = ws + (2 * blockIdx.x + (c0 == 0 ? 1 : 0)) * partial_floats(D);
+            for (int d = tid & 15; d < D; d += 16) to[i * D + d] = all.value(sh, i, d);
+            if ((tid & 15) == 0) {
+                to[kRows * D + i] = all.m;
+                to[kRows * D + kRows + i] = all.l;
             }
         }
-        __syncthreads();
-
-        // ---- this warp's tiles of positions [c0 * 64, c1 * 64) ----
-        constexpr int kRowBytes = Q8 ? D : 2 * D;
-        const int p_end = (int) (c1 * kChunk < len ? c1 * kChunk : len);
-        const int all_see = (int) len - g.n_tok + 1;  // positions below are seen by every row
-        const int seen = row.there ? all_see + row.token : 0;
-        const int64_t page_bytes = (int64_t) c.n_kv_head * c.page_size * kRowBytes;
-        const int64_t head_bytes = (int64_t) h * c.page_size * kRowBytes;
-        const uint8_t * kl = c.k + head_bytes + gq * kRowBytes + t * (Q8 ? 8 : 16);                      // this lane's bytes of page 0
-        const uint8_t * vl = c.v + head_bytes + 2 * t * kRowBytes + gq * S::kRun * (Q8 ? 1 : 2);
-        const uint8_t * kdl = reinterpret_cast<const uint8_t *>(c.kd) + head_bytes / 16 + t * (D / 8);  // a row's scales: D / 16 bytes
-        const uint8_t * vdl = reinterpret_cast<const uint8_t *>(c.vd) + head_bytes / 16 + t * (D / 8);
-        const int page_step = kChunk / c.page_size, slot_step = kChunk % c.page_size;
-        float o[S::kGroups][S::kRun][2] = {}, m = -INFINITY, l = 0.0f;
-        int p0 = (int) c0 * kChunk + warp * 16;
-        int in_table = p0 / c.page_size, slot = p0 % c.page_size;
-        for (; p0 < p_end; p0 += kChunk) {
-            const int page = kv_page(c, seq, in_table, lane == 0);
-            const int64_t at = page * page_bytes + slot * kRowBytes;
-            in_table += page_step;
-            slot += slot_step;
-            if (slot >= c.page_size) slot -= c.page_size, in_table++;
-            if (page < 0) continue;
-            const int here = p_end - p0;  // positions of the tile: 16 or more, or its end
-            const bool edge = p0 + 16 > all_see || here < 16;
-            uint32_t kw[2][S::kBlocks][S::kKeyWords], vw[4][S::kGroups][S::kValueWords];
-            uint32_t kd[2][Q8 ? S::kBlocks : 1], vd[2][Q8 ? S::kBlocks : 1];
-            // keys of positions gq, gq + 8; values of positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9, whose scores this lane holds
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int b = 0; b < S::kBlocks; b++) {
-                    if (edge && gq + 8 * i >= here) zero(kw[i][b]);
-                    else load(kw[i][b], kl + at + i * 8 * kRowBytes + b * (Q8 ? 32 : 64));
-                }
-            if constexpr (Q8) {  // the scales of two neighbouring rows are kBlocks words; the tile's rows all lie in its page
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    load(kd[i], kdl + at / 16 + i * (D / 2));
-                    load(vd[i], vdl + at / 16 + i * (D / 2));
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int n = 0; n < S::kGroups; n++) {
-                    if (edge && 2 * t + (i & 1) + 8 * (i >> 1) >= here) zero(vw[i][n]);
-                    else load(vw[i][n], vl + at + ((i & 1) + 8 * (i >> 1)) * kRowBytes + n * 8 * S::kRun * (Q8 ? 1 : 2));
-                }
-
-            // ---- scores: s[2 i + j] is position 2 t + j + 8 i of row gq ----
-            float s[4];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                s[2 * i] = s[2 * i + 1] = 0.0f;
-#pragma unroll
-                for (int b = 0; b < S::kBlocks; b++) {
-                    const uint4 a0 = *reinterpret_cast<const uint4 *>(sq[2 * b][lane]), a1 = *reinterpret_cast<const uint4 *>(sq[2 * b + 1][lane]);
-                    const uint32_t f0[4] = {a0.x, a0.y, a0.z, a0.w}, f1[4] = {a1.x, a1.y, a1.z, a1.w};
-                    if constexpr (Q8) {
-                        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        const uint32_t w0 = kw[i][b][0] ^ 0x80808080u, w1 = kw[i][b][1] ^ 0x80808080u;
-                        mma(part, f0, halves(w0, 0x4140), halves(w0, 0x4342));
-                        mma(part, f1, halves(w1, 0x4140), halves(w1, 0x4342));
-                        s[2 * i] = fmaf(half_of(kd[i], b), part[0] + part[2], s[2 * i]);
-                        s[2 * i + 1] = fmaf(half_of(kd[i], S::kBlocks + b), part[1] + part[3], s[2 * i + 1]);
-                    } else {
-                        mma(sum, f0, kw[i][b][0], kw[i][b][1]);
-                        mma(sum, f1, kw[i][b][2], kw[i][b][3]);
-                    }
-                }
-                if constexpr (!Q8) {
-                    s[2 * i] = sum[0] + sum[2];
-                    s[2 * i + 1] = sum[1] + sum[3];
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) s[i] *= factor;
-            if (edge) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int j = 2 * t + (i & 1) + 8 * (i >> 1);
-                    if (j >= here || p0 + j >= seen) s[i] = -INFINITY;
-                }
-            }
-
-            // ---- weights: m is the running maximum less kShift (-infinity before any score) ----
-            float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float m_new = fmaxf(m, top - kShift);
-            const float base = m_new == -INFINITY ? 0.0f : m_new;
-            const float keep = ex2(m - base);
-            m = m_new;
-            float p[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) p[i] = ex2(s[i] - base);
-            l = fmaf(l, keep, (p[0] + p[1]) + (p[2] + p[3]));
-
-            // ---- o = o keep + P V ----
-            uint32_t pf[4];  // the weights' fragment: hi, lo of positions 2 t, 2 t + 1, then of 2 t + 8, 2 t + 9
-            split(p[0], p[1], pf[0], pf[1]);
-            split(p[2], p[3], pf[2], pf[3]);
-            if constexpr (Q8) {
-                // one block of 32 dimensions: weights times scales (fragment a), times 2^k and back where `down` is not 1
-                auto block = [&](int b, const uint32_t(&a)[4], auto scaled, float down) {
-                    // two rows' four bytes each, interleaved: (row, row + 1) pairs of dimensions 0, 1 and 2, 3
-                    const uint32_t x0 = __byte_perm(vw[0][b][0], vw[1][b][0], 0x5140) ^ 0x80808080u;
-                    const uint32_t x1 = __byte_perm(vw[0][b][0], vw[1][b][0], 0x7362) ^ 0x80808080u;
-                    const uint32_t y0 = __byte_perm(vw[2][b][0], vw[3][b][0], 0x5140) ^ 0x80808080u;
-                    const uint32_t y1 = __byte_perm(vw[2][b][0], vw[3][b][0], 0x7362) ^ 0x80808080u;
-#pragma unroll
-                    for (int n = 0; n < 4; n++) {
-                        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        const uint32_t sel = n & 1 ? 0x4342 : 0x4140;
-                        mma(part, a, halves(n < 2 ? x0 : x1, sel), halves(n < 2 ? y0 : y1, sel));
-                        part[0] += part[2];
-                        part[1] += part[3];
-                        if constexpr (decltype(scaled)::value) part[0] *= down, part[1] *= down;
-                        o[b][n][0] = fmaf(o[b][n][0], keep, part[0]);
-                        o[b][n][1] = fmaf(o[b][n][1], keep, part[1]);
-                    }
-                };
-                // Scales between 2^-14 and 2 (nearly always all of them) multiply the weights' halves in F16 pairs: the
-                // product's rounding error is exact in F16 and goes to the low half. The weights being up to 2^14 and the low
-                // halves reaching 2^-24, nothing overflows and what is lost is below 2^-24 of the largest weight's product.
-                uint32_t low = vd[0][0], high = vd[0][0];
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int b = 0; b < S::kBlocks; b++) low = __vminu2(low, vd[i][b]), high = __vmaxu2(high, vd[i][b]);
-                const bool plain = (low & 0xffffu) >= 0x0400u && low >= 0x04000000u && (high & 0xffffu) < 0x4000u && high < 0x40000000u;
-                if (__all_sync(0xffffffffu, plain)) {
-                    auto go = [&](auto index) {
-                        constexpr int b = decltype(index)::value;
-                        if constexpr (b < S::kBlocks) {
-                            const __half2 d0 = h2(pair_of<b, S::kBlocks + b>(vd[0])), d1 = h2(pair_of<b, S::kBlocks + b>(vd[1]));
-                            const __half2 w0 = __hmul2_rn(h2(pf[0]), d0), w1 = __hmul2_rn(h2(pf[2]), d1);
-                            const uint32_t a[4] = {u32(w0), u32(__hfma2(h2(pf[1]), d0, __hfma2(h2(pf[0]), d0, __hneg2(w0)))), u32(w1),
-                                                   u32(__hfma2(h2(pf[3]), d1, __hfma2(h2(pf[2]), d1, __hneg2(w1))))};
-                            block(b, a, std::false_type{}, 1.0f);
-                        }
-                    };
-                    go(std::integral_constant<int, 0>{}), go(std::integral_constant<int, 1>{}), go(std::integral_constant<int, 2>{});
-                    go(std::integral_constant<int, 3>{}), go(std::integral_constant<int, 4>{}), go(std::integral_constant<int, 5>{});
-                    go(std::integral_constant<int, 6>{}), go(std::integral_constant<int, 7>{});
-                } else {
-                    // any scales: the product in float32, times a power of two that brings the tile's largest scale below 1
-#pragma unroll
-                    for (int b = 0; b < S::kBlocks; b++) {
-                        float d[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            d[i] = 2 * t + (i & 1) + 8 * (i >> 1) < here ? half_of(vd[i >> 1], (i & 1) * S::kBlocks + b) : 0.0f;
-                        float big = fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fabsf(d[3])));
-                        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-                        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-                        int e = (int) (__float_as_uint(big) >> 23);
-                        if (e == 0 || e == 255) e = 126;
-                        const float up = __uint_as_float((uint32_t) (253 - e) << 23), down = __uint_as_float((uint32_t) (e + 1) << 23);
-                        float w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) w[i] = edge && p[i] == 0.0f ? 0.0f : p[i] * (d[i] * up);
-                        uint32_t a[4];
-                        split(w[0], w[1], a[0], a[1]);
-                        split(w[2], w[3], a[2], a[3]);
-                        block(b, a, std::true_type{}, down);
-                    }
-                }
-            } else {
-                auto product = [&](bool mine) {
-#pragma unroll
-                    for (int n = 0; n < S::kGroups; n++)
-#pragma unroll
-                        for (int r = 0; r < S::kRun; r++) {
-                            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            const uint32_t sel = r & 1 ? 0x7632 : 0x5410;
-                            mma(part, pf, __byte_perm(vw[0][n][r / 2], vw[1][n][r / 2], sel), __byte_perm(vw[2][n][r / 2], vw[3][n][r / 2], sel));
-                            if (mine) {
-                                o[n][r][0] = fmaf(o[n][r][0], keep, part[0] + part[2]);
-                                o[n][r][1] = fmaf(o[n][r][1], keep, part[1] + part[3]);
-                            }
-                        }
-                };
-                if (edge && g.n_tok > 1) {
-                    // Where rows see different positions, a value that is NaN or infinite must not meet the weight 0 of a row
-                    // that does not see it: one product per token, from the last, with the values behind its position zeroed.
-                    const int first = tile * kRows / g.group;
-                    for (int token = min((tile * kRows + kRows - 1) / g.group, g.n_tok - 1); token >= first; token--) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (p0 + 2 * t + (i & 1) + 8 * (i >> 1) >= all_see + token) {
-#pragma unroll
-                                for (int n = 0; n < S::kGroups; n++) zero(vw[i][n]);
-                            }
-                        product(row.token == token);
-                    }
-                } else {
-                    product(true);
-                }
-            }
-        }
-
-        // ---- join the warps ----
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (t == 0) {
-            sm[warp][gq] = m;
-            sl[warp][gq] = l;
-        }
-#pragma unroll
-        for (int n = 0; n < S::kGroups; n++)
-#pragma unroll
-            for (int r = 0; r < S::kRun; r++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) so[warp][gq][n * 8 * S::kRun + (2 * t + j) * S::kRun + r] = o[n][r][j];
-        __syncthreads();
-        {
-            const int i = tid / 16;  // a row per 16 threads
-            float top = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kWarps; w++) top = fmaxf(top, sm[w][i]);
-            const float base = top == -INFINITY ? 0.0f : top;
-            float f[kWarps], sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWarps; w++) {
-                f[w] = ex2(sm[w][i] - base);
-                sum = fmaf(sl[w][i], f[w], sum);
-            }
-            const Row mine = row_of(g, h, tile, i);
-            const bool whole = c0 == 0 && c1 == chunks;
-            float * to = whole ? out + ((seq * g.n_tok + mine.token) * g.n_head + mine.head) * D
-                               : ws + (2 * blockIdx.x + (c0 == 0 ? 1 : 0)) * partial_floats(D) + i * D;
-            const float inv = !whole ? 1.0f : sum != 0.0f ? 1.0f / sum : 0.0f;
-            if (!whole || mine.there) {
-                for (int d = tid & 15; d < D; d += 16) {
-                    float v = 0.0f;
-#pragma unroll
-                    for (int w = 0; w < kWarps; w++) v = fmaf(so[w][i][d], f[w], v);
-                    to[d] = v * inv;
-                }
-            }
-            if (!whole && (tid & 15) == 0) {
-                float * ml = ws + (2 * blockIdx.x + (c0 == 0 ? 1 : 0)) * partial_floats(D) + kRows * D;
-                ml[i] = top;
-                ml[kRows + i] = sum;
-            }
-        }
-        __syncthreads();  // sq, so are written again by the next run
+        __syncthreads();  // the shared memory is written again by the next run
     }
+}
+
+// The work cut by items: a cluster of `cluster` CTAs per item, each an equal run of its chunks, joined over distributed
+// shared memory: the CTA of rank r writes rows r, r + cluster, ... One launch, and no length but the item's own is read.
+template <bool Q8, int D>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
+    kv_attention_item_kernel(KvView c, Geometry g, int cluster, const float * __restrict__ q, int64_t ldq, float scale, float * __restrict__ out) {
+    __shared__ Shared<D> sh;
+    __shared__ float jm[kRows], jl[kRows];
+    const int tid = threadIdx.x, rank = blockIdx.x % cluster;
+    const int64_t unit = blockIdx.x / cluster, seq = unit / g.items;
+    const int item = (int) (unit % g.items), h = item / g.tiles, tile = item % g.tiles;
+    const int64_t len = kv_len(c, seq, tid == 0), chunks = (len + kChunk - 1) / kChunk, per = (chunks + cluster - 1) / cluster;
+    const int64_t c0 = rank * per < chunks ? rank * per : chunks, c1 = c0 + per < chunks ? c0 + per : chunks;
+    attend<Q8, D>(c, g, q, ldq, scale, sh, seq, len, h, tile, c0, c1);
+    {
+        const int i = tid / 16;
+        const Joined<D> all(sh, i);
+        for (int d = tid & 15; d < D; d += 16) sh.so[0][i][d] = all.value(sh, i, d);  // read and written by this thread alone
+        if ((tid & 15) == 0) jm[i] = all.m, jl[i] = all.l;
+    }
+    const cooperative_groups::cluster_group group = cooperative_groups::this_cluster();
+    group.sync();
+    for (int e = tid; e < kRows / cluster * D; e += kThreads) {
+        const int i = e / D * cluster + rank, d = e % D;
+        const Row row = row_of(g, h, tile, i);
+        if (!row.there) continue;
+        float m = -INFINITY, l = 0.0f, v = 0.0f;
+        for (int r = 0; r < cluster; r++) m = fmaxf(m, *group.map_shared_rank(&jm[i], r));
+        const float base = m == -INFINITY ? 0.0f : m;
+        for (int r = 0; r < cluster; r++) {
+            const float f = ex2(*group.map_shared_rank(&jm[i], r) - base);
+            l = fmaf(*group.map_shared_rank(&jl[i], r), f, l);
+            v = fmaf(*group.map_shared_rank(&sh.so[0][i][d], r), f, v);
+        }
+        out[((seq * g.n_tok + row.token) * g.n_head + row.head) * D + d] = l != 0.0f ? v * (1.0f / l) : 0.0f;
+    }
+    group.sync();  // the others read this CTA's shared memory until here
 }
 
 // Joins the partials of items that several CTAs worked on, and writes the zeros of empty sequences. One CTA per row of an
@@ -619,27 +685,42 @@ Geometry geometry(const b200_context * ctx, const b200_kv_cache * c, int64_t max
     g.items = (int64_t) c->n_kv_head * g.tiles;
     g.n_seq = n_seq;
     g.ctas = (int64_t) ctx->num_sms * ctas_per_sm_of(c->type == B200_TYPE_Q8_0, c->head_dim);
-    const int64_t most = (max_pages * c->page_size + kChunk - 1) / kChunk * n_seq * g.items;  // chunks, if every length were the largest
-    if (g.ctas > most) g.ctas = most > 0 ? most : 1;
+    // By items when the lengths that the table allows are short: the cluster (1 to 8 CTAs) is the largest that all items fit
+    // on the GPU with at once.
+    const int64_t most = (max_pages * c->page_size + kChunk - 1) / kChunk;  // chunks of the longest sequence there can be
+    g.cluster = 8;
+    while (g.cluster > 1 && n_seq * g.items * g.cluster > g.ctas) g.cluster /= 2;
+    if (most > kItemChunks * g.cluster) g.cluster = 0;
+    if (g.ctas > most * n_seq * g.items) g.ctas = most > 0 ? most * n_seq * g.items : 1;
     return g;
 }
 
 template <bool Q8, int D>
 cudaError_t launch(const KvView & c, const Geometry & g, const float * q, int64_t ldq, float scale, float * out, float * ws, cudaStream_t st) {
-    kv_attention_kernel<Q8, D><<<(unsigned) g.ctas, kThreads, 0, st>>>(c, g, q, ldq, scale, out, ws);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned) (g.n_seq * g.items * kRows), 1, 1);
-    cfg.blockDim = dim3(32 * kJoinWarps, 1, 1);
-    cfg.stream = st;
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    if (g.cluster) {
+        cfg.gridDim = dim3((unsigned) (g.n_seq * g.items * g.cluster), 1, 1);
+        cfg.blockDim = dim3(kThreads, 1, 1);
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned) g.cluster;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        return cudaLaunchKernelEx(&cfg, kv_attention_item_kernel<Q8, D>, c, g, g.cluster, q, ldq, scale, out);
+    }
+    kv_attention_kernel<Q8, D><<<(unsigned) g.ctas, kThreads, 0, st>>>(c, g, q, ldq, scale, out, ws);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    cfg.gridDim = dim3((unsigned) (g.n_seq * g.items * kRows), 1, 1);
+    cfg.blockDim = dim3(32 * kJoinWarps, 1, 1);
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     return cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<D>, c, g, out, (const float *) ws);
 }
+
+size_t workspace_bytes_of(const Geometry & g, int D) { return g.cluster ? 0 : (size_t) (2 * g.ctas * partial_floats(D)) * sizeof(float); }
 
 bool fits(const b200_kv_cache * c, int64_t max_pages, int64_t n_seq, int64_t n_tok, int64_t n_head) {
     return c && c->n_kv_head > 0 && c->page_size > 0 && max_pages >= 0 && n_seq > 0 && n_tok > 0 && n_tok <= 16 && n_head > 0 && n_head <= 65535 &&
@@ -653,7 +734,7 @@ extern "C" {
 size_t b200_kv_attention_workspace(b200_context * ctx, const b200_kv_cache * cache, int64_t max_pages, int64_t n_seq, int64_t n_tok,
                                    int64_t n_head) {
     if (!ctx || !fits(cache, max_pages, n_seq, n_tok, n_head)) return 0;
-    return (size_t) (2 * geometry(ctx, cache, max_pages, n_seq, n_tok, n_head).ctas * partial_floats(cache->head_dim)) * sizeof(float);
+    return workspace_bytes_of(geometry(ctx, cache, max_pages, n_seq, n_tok, n_head), cache->head_dim);
 }
 
 b200_status b200_kv_attention(b200_context * ctx, void * stream, const b200_kv_cache * cache, const int32_t * table, int64_t max_pages,
@@ -670,7 +751,8 @@ b200_status b200_kv_attention(b200_context * ctx, void * stream, const b200_kv_c
     if (ldq < n_head * c.head_dim) return kv_fail(ctx, B200_ERR_INVALID, what, "the row stride is below n_head * head_dim");
     if (!q || !out || ((uintptr_t) q & 3) || ((uintptr_t) out & 3)) return kv_fail(ctx, B200_ERR_INVALID, what, "NULL or misaligned q or out");
     const Geometry g = geometry(ctx, cache, max_pages, n_seq, n_tok, n_head);
-    if (!workspace || workspace_bytes < 2 * (size_t) (g.ctas * partial_floats(c.head_dim)) * sizeof(float) || ((uintptr_t) workspace & 255))
+    const size_t need = workspace_bytes_of(g, c.head_dim);
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t) workspace & 255)))
         return kv_fail(ctx, B200_ERR_INVALID, what, "the workspace is missing, misaligned or too small");
     DeviceScope scope(ctx->device);
     if (scope.status != cudaSuccess) return kv_cuda(ctx, scope.status, what);

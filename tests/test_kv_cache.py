@@ -65,7 +65,7 @@ def test_the_python_layer_refuses_what_it_cannot_pass_on(pkg):
 
     ctx = bare(pkg)
     cache = pkg.KvCache.__new__(pkg.KvCache)
-    cache.ctx, cache.s, cache.data = ctx, pkg.KvCacheStruct(type=pkg.F16, n_kv_head=2, head_dim=64, page_size=16, n_pages=1), None
+    cache.ctx, cache.open, cache.n_kv_head, cache.head_dim, cache.data = ctx, True, 2, 64, None
     x = torch.zeros(1, 1, 2, 64)
     table, lens = torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
     with pytest.raises(ValueError, match="cuda:0"):  # host tensors
