@@ -61,6 +61,7 @@ struct b200_context {
     // Expanded copies of K-quant weights used with many activation rows, by weight data pointer; dropped when the
     // weight is written or freed.
     std::unordered_map<const void *, KqExpansion> kq;
+    unsigned kv_shapes = 0;  // kv_attention kernels (a bit per cache type and head_dim) set up for their shared memory
 };
 
 // Makes `device` current for a scope (a call on a context whose device is not the caller's current one).

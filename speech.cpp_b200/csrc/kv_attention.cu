@@ -52,12 +52,6 @@ struct Geometry {
     int cluster;                      // CTAs that share an item (0: the work is cut by positions)
 };
 
-// CTAs per SM, by what registers allow (__launch_bounds__ holds the compiler to it).
-template <bool Q8, int D>
-constexpr int ctas_per_sm() { return D == 256 ? 2 : 3; }
-
-int ctas_per_sm_of(bool q8, int D) { (void) q8; return D == 256 ? 2 : 3; }
-
 constexpr int64_t partial_floats(int D) { return (int64_t) kRows * (D + 2); }  // o [kRows][D], m [kRows], l [kRows]
 
 __device__ __forceinline__ float ex2(float x) {
@@ -72,27 +66,28 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// N 32-bit words from p (aligned to their size; N = 3, 8: to one and four words). The cache is read once: not kept in L1.
-template <int N>
-__device__ __forceinline__ void load(uint32_t (&w)[N], const uint8_t * p) {
-    if constexpr (N == 4 || N == 8) {
-#pragma unroll
-        for (int i = 0; i < N; i += 4)
-            asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
-                         : "l"(p + 4 * i));
-    } else if constexpr (N == 2) {
-        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(w[i]) : "l"(p + 4 * i));
-    }
+// 16 bytes from global to shared memory, asynchronously; zeros when !there (nothing is read then).
+__device__ __forceinline__ void copy16(uint32_t to, const uint8_t * from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
 
+__device__ __forceinline__ void copy16(uint32_t to, const uint8_t * from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+
+// N 32-bit words at a shared address.
 template <int N>
-__device__ __forceinline__ void zero(uint32_t (&w)[N]) {
+__device__ __forceinline__ void lds(uint32_t (&w)[N], uint32_t at) {
+    if constexpr (N % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < N; i++) w[i] = 0;
+        for (int i = 0; i < N; i += 4)
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "r"(at + 4 * i));
+    } else if constexpr (N == 2) {
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(at + 4 * i));
+    }
 }
 
 __device__ __forceinline__ __half2 h2(uint32_t w) { return *reinterpret_cast<const __half2 *>(&w); }
@@ -120,11 +115,11 @@ __device__ __forceinline__ uint32_t halves(uint32_t biased, uint32_t sel) {
 }
 
 __device__ __forceinline__ float half_of(const uint32_t * w, int i) {
-    return __half2float(__ushort_as_half((uint16_t) (w[i >> 1] >> (16 * (i & 1)))));
+    return i & 1 ? __high2float(h2(w[i >> 1])) : __low2float(h2(w[i >> 1]));
 }
 
-// How the n index of O = P V runs through the dimensions: groups of 8 kRun dimensions, lane quad g holding kRun contiguous
-// ones of each.
+// How a head's rows are taken apart. The n index of O = P V runs through the dimensions in groups of 8 kRun, lane quad g
+// holding kRun contiguous ones of each.
 template <bool Q8, int D>
 struct Shape {
     static constexpr int kBlocks = D / 32;
@@ -132,6 +127,31 @@ struct Shape {
     static constexpr int kGroups = D / (8 * kRun);
     static constexpr int kKeyWords = Q8 ? 2 : 4;           // a lane's words of a row's 32 dimensions
     static constexpr int kValueWords = Q8 ? 1 : kRun / 2;  // a lane's words of a row's group
+    // A piece is 16 positions: its key rows, value rows, and their scales. Each warp has a ring of kStages pieces in shared
+    // memory; the ring's depth and the CTAs per SM fill its 227 KB.
+    static constexpr int kRowBytes = Q8 ? D : 2 * D;
+    static constexpr int kScaleBytes = Q8 ? D / 16 : 0;    // of a row
+    static constexpr int kPiece = 32 * (kRowBytes + kScaleBytes);
+    static constexpr int kStages = Q8 ? (D == 256 ? 3 : 4) : (D == 64 ? 4 : D == 256 ? 2 : 3);
+    static constexpr int kCtas = Q8 ? (D == 256 ? 2 : 3) : (D == 256 ? 1 : D == 128 ? 2 : 3);
+    static_assert(D == 96 || kPiece % 128 == 0, "swizzled pieces keep the ring's alignment");
+    static constexpr int kBytes = kWarps * kStages * kPiece;
+    // The 16-byte chunks of a row are stored at chunk ^ swizzle(row), so that the lanes that read together read different
+    // banks: fragments of keys are read from rows 0-7 (Q8_0: four rows and 32 bytes of each at a time, F16: two rows and
+    // 64), of values from rows 0, 2, 4, 6 and so on. Rows of 96 or 192 bytes are apart by themselves (keys) or in pairs. Both
+    // take bits of the row to bits of the chunk, so swizzle(a | b) = swizzle(a) ^ swizzle(b).
+    static constexpr bool kSwizzled = D != 96;
+    static constexpr int key_swizzle(int row) {
+        return D == 96 ? 0 : !Q8 ? (row & 1) << 2 : D == 64 ? (row >> 1 & 1) << 1 : (row & 3) << 1;
+    }
+    static constexpr int value_swizzle(int row) {
+        return D == 96 ? 0 : !Q8 ? row & 6 : D == 64 ? (row >> 1 & 1) << 1 : (row >> 1 & 3) << 1;
+    }
+    // From the address of a lane's first fragment in a row to that of the one `bytes` further on in the row (pieces start at
+    // multiples of 128 bytes, and the swizzle moves chunks within 128).
+    static __device__ __forceinline__ uint32_t along(uint32_t at, uint32_t bytes) {
+        return kSwizzled ? (at ^ (bytes & 127)) + (bytes & ~127u) : at + bytes;
+    }
 };
 
 __device__ __forceinline__ int64_t chunks_of(const KvView & c, int64_t s, bool tell) { return (kv_len(c, s, tell) + kChunk - 1) / kChunk; }
@@ -203,26 +223,99 @@ __device__ __forceinline__ Row row_of(const Geometry & g, int h, int tile, int i
     return {n / g.group, h * g.group + n % g.group, n < g.n_tok * g.group};
 }
 
-// What a CTA holds while it works on one item.
-template <int D>
+// A CTA's shared memory: the warps' rings of pieces, and, at the ring's place once a run is done, each warp's o.
+template <bool Q8, int D>
 struct Shared {
-    __align__(16) uint32_t sq[D / 16][32][4];  // the query tile as fragments
-    float so[kWarps][kRows][D + 4];            // the warps' results
-    float sm[kWarps][kRows], sl[kWarps][kRows];
+    uint8_t * ring;  // dynamic: [kWarps][kStages][kPiece]
+    float (*sm)[kRows];
+    float (*sl)[kRows];
+    static constexpr int kRingBytes = Shape<Q8, D>::kStages * Shape<Q8, D>::kPiece;
+    static constexpr int kPitch = D + 4;
+    static_assert(kRows * kPitch * 4 <= kRingBytes, "a warp's o fits its ring");
+    __device__ __forceinline__ float & o(int w, int row, int d) const {
+        return reinterpret_cast<float *>(ring + w * kRingBytes)[row * kPitch + d];
+    }
 };
 
 // Chunks [c0, c1) of one item: the warps' m, l and o are left in shared memory (synchronised).
 template <bool Q8, int D>
-__device__ __forceinline__ void attend(const KvView & c, const Geometry & g, const float * __restrict__ q, int64_t ldq, float scale, Shared<D> & sh,
-                                       int64_t seq, int64_t len, int h, int tile, int64_t c0, int64_t c1) {
+__device__ __forceinline__ void attend(const KvView & c, const Geometry & g, const float * __restrict__ q, int64_t ldq, float scale,
+                                       const Shared<Q8, D> & sh, int64_t seq, int64_t len, int h, int tile, int64_t c0, int64_t c1) {
     using S = Shape<Q8, D>;
+    constexpr int kRowBytes = S::kRowBytes, kValues = 16 * kRowBytes, kKeyScales = 32 * kRowBytes, kValueScales = kKeyScales + 16 * S::kScaleBytes;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int gq = lane >> 2, t = lane & 3;  // the fragment's group and thread in it
     const Row row = row_of(g, h, tile, gq);
+    const int p_end = (int) (c1 * kChunk < len ? c1 * kChunk : len);
+    const int all_see = (int) len - g.n_tok + 1;  // positions below are seen by every row
+    const int seen = row.there ? all_see + row.token : 0;
 
-    // ---- the query tile: each warp makes the fragments of its share of the k steps ----
+    // ---- the ring: pieces p0 = c0 * 64 + warp * 16, then every 64, copied kStages - 1 ahead ----
+    const uint32_t ring = smem_addr(sh.ring) + warp * Shared<Q8, D>::kRingBytes;
+    const int64_t page_bytes = (int64_t) c.n_kv_head * c.page_size * kRowBytes;
+    const int64_t head_bytes = (int64_t) h * c.page_size * kRowBytes;
+    const int page_step = kChunk / c.page_size, slot_step = kChunk % c.page_size;
+    int p_copy = (int) c0 * kChunk + warp * 16;  // the next piece to copy, its place in the table, its page (asked for early)
+    int in_table = p_copy / c.page_size, slot = p_copy % c.page_size, stage_copy = 0;
+    int page = p_copy < p_end ? kv_page(c, seq, in_table, lane == 0) : -1;
+    // where this lane's first 16 bytes of a piece go: row lane / (chunks of a row), chunk lane % (chunks of a row)
+    const uint32_t copy_key = lane * 16 ^ S::key_swizzle(lane / (kRowBytes / 16)) * 16;
+    const uint32_t copy_value = lane * 16 ^ S::value_swizzle(lane / (kRowBytes / 16)) * 16;
+    unsigned found = 0;  // bit per stage: its piece has a page
+    auto copy_piece = [&] {
+        if (p_copy < p_end) {
+            const int here = page < 0 ? 0 : p_end - p_copy;  // rows of the piece; the others are zeros
+            const int64_t at = head_bytes + max(page, 0) * page_bytes + (int64_t) slot * kRowBytes;
+            const uint32_t to = ring + stage_copy * S::kPiece;
+            constexpr int kRowChunks = kRowBytes / 16, kCopies = kRowChunks / 2;  // a piece's rows are contiguous: 16 kRowChunks chunks
+            auto each = [&](auto whole) {
+#pragma unroll
+                for (int j = 0; j < kCopies; j++) {
+                    uint32_t key_to, value_to, r;
+                    if constexpr (S::kSwizzled) {  // 32 / kRowChunks rows further each time: their swizzle is a constant
+                        r = lane / kRowChunks + j * (32 / kRowChunks);
+                        key_to = (copy_key ^ (S::key_swizzle(j * (32 / kRowChunks)) * 16)) + j * 512;
+                        value_to = (copy_value ^ (S::value_swizzle(j * (32 / kRowChunks)) * 16)) + j * 512;
+                    } else {
+                        r = (lane + 32 * j) / kRowChunks;
+                        key_to = value_to = (lane + 32 * j) * 16;
+                    }
+                    if constexpr (decltype(whole)::value) {
+                        copy16(to + key_to, c.k + at + lane * 16 + j * 512);
+                        copy16(to + kValues + value_to, c.v + at + lane * 16 + j * 512);
+                    } else {
+                        copy16(to + key_to, c.k + at + lane * 16 + j * 512, (int) r < here);
+                        copy16(to + kValues + value_to, c.v + at + lane * 16 + j * 512, (int) r < here);
+                    }
+                }
+            };
+            if (here >= 16) each(std::true_type{});
+            else each(std::false_type{});
+            if constexpr (Q8) {  // whole, rows behind the end too: they lie in the page
+                if (lane < S::kScaleBytes) copy16(to + kKeyScales + lane * 16, reinterpret_cast<const uint8_t *>(c.kd) + at / 16 + lane * 16, page >= 0);
+                else if (lane < 2 * S::kScaleBytes)
+                    copy16(to + kKeyScales + lane * 16, reinterpret_cast<const uint8_t *>(c.vd) + at / 16 + (lane - S::kScaleBytes) * 16, page >= 0);
+            }
+            found = page < 0 ? found & ~(1u << stage_copy) : found | 1u << stage_copy;
+            p_copy += kChunk;
+            in_table += page_step;
+            slot += slot_step;
+            if (slot >= c.page_size) slot -= c.page_size, in_table++;
+            if (p_copy < p_end) page = kv_page(c, seq, in_table, lane == 0);
+            stage_copy = stage_copy + 1 == S::kStages ? 0 : stage_copy + 1;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int n = 0; n < S::kStages - 1; n++) copy_piece();
+
+    // ---- the query tile's fragments ----
     // k step 2 j + b of lane (gq, t) holds dimensions 32 j + 8 t + 4 b .. + 3 of row gq: hi in registers 0 and 2, lo in
     // 1 and 3. The row is scaled by 2^k to a largest magnitude in [2^14, 2^15).
+    // Q8_0: key bytes enter as q + 128 in the low byte of an F16, which is (q + 128) 2^-24 (a subnormal, and exact); `bias` is
+    // what the 128 adds to a block's sum.
+    uint32_t qf[D / 16][4];
+    float bias[Q8 ? S::kBlocks : 1];
     float factor;  // what a raw score is multiplied by: scale log2(e) 2^-k
     {
         const float * src = q + (seq * g.n_tok + row.token) * ldq + (int64_t) row.head * D + 8 * t;
@@ -240,93 +333,75 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
         factor = scale * 1.4426950408889634f * __uint_as_float((uint32_t) (127 - k) << 23);
 #pragma unroll
         for (int j = 0; j < D / 16; j++) {
-            if (j % kWarps != warp) continue;
-            uint32_t hi[2], lo[2];
-            split(x[4 * j] * up, x[4 * j + 1] * up, hi[0], lo[0]);
-            split(x[4 * j + 2] * up, x[4 * j + 3] * up, hi[1], lo[1]);
-            *reinterpret_cast<uint4 *>(sh.sq[j][lane]) = make_uint4(hi[0], lo[0], hi[1], lo[1]);
+            split(x[4 * j] * up, x[4 * j + 1] * up, qf[j][0], qf[j][1]);
+            split(x[4 * j + 2] * up, x[4 * j + 3] * up, qf[j][2], qf[j][3]);
         }
-    }
-    __syncthreads();
-
-    // ---- this warp's tiles of positions [c0 * 64, c1 * 64) ----
-    constexpr int kRowBytes = Q8 ? D : 2 * D;
-    const int p_end = (int) (c1 * kChunk < len ? c1 * kChunk : len);
-    const int all_see = (int) len - g.n_tok + 1;  // positions below are seen by every row
-    const int seen = row.there ? all_see + row.token : 0;
-    const int64_t page_bytes = (int64_t) c.n_kv_head * c.page_size * kRowBytes;
-    const int64_t head_bytes = (int64_t) h * c.page_size * kRowBytes;
-    const uint8_t * kl = c.k + head_bytes + gq * kRowBytes + t * (Q8 ? 8 : 16);                      // this lane's bytes of page 0
-    const uint8_t * vl = c.v + head_bytes + 2 * t * kRowBytes + gq * S::kRun * (Q8 ? 1 : 2);
-    const uint8_t * kdl = reinterpret_cast<const uint8_t *>(c.kd) + head_bytes / 16 + t * (D / 8);  // a row's scales: D / 16 bytes
-    const uint8_t * vdl = reinterpret_cast<const uint8_t *>(c.vd) + head_bytes / 16 + t * (D / 8);
-    const int page_step = kChunk / c.page_size, slot_step = kChunk % c.page_size;
-    float o[S::kGroups][S::kRun][2] = {}, m = -INFINITY, l = 0.0f;
-    int p0 = (int) c0 * kChunk + warp * 16;
-    int in_table = p0 / c.page_size, slot = p0 % c.page_size;
-    for (; p0 < p_end; p0 += kChunk) {
-        const int page = kv_page(c, seq, in_table, lane == 0);
-        const int64_t at = page * page_bytes + slot * kRowBytes;
-        in_table += page_step;
-        slot += slot_step;
-        if (slot >= c.page_size) slot -= c.page_size, in_table++;
-        if (page < 0) continue;
-        const int here = p_end - p0;  // positions of the tile: 16 or more, or its end
-        const bool edge = p0 + 16 > all_see || here < 16;
-        uint32_t kw[2][S::kBlocks][S::kKeyWords], vw[4][S::kGroups][S::kValueWords];
-        uint32_t kd[2][Q8 ? S::kBlocks : 1], vd[2][Q8 ? S::kBlocks : 1];
-        // keys of positions gq, gq + 8; values of positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9, whose scores this lane holds
-#pragma unroll
-        for (int i = 0; i < 2; i++)
+        if constexpr (Q8) {
+            factor *= 0x1p24f;
 #pragma unroll
             for (int b = 0; b < S::kBlocks; b++) {
-                if (edge && gq + 8 * i >= here) zero(kw[i][b]);
-                else load(kw[i][b], kl + at + i * 8 * kRowBytes + b * (Q8 ? 32 : 64));
-            }
-        if constexpr (Q8) {  // the scales of two neighbouring rows are kBlocks words; the tile's rows all lie in its page
+                float sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                load(kd[i], kdl + at / 16 + i * (D / 2));
-                load(vd[i], vdl + at / 16 + i * (D / 2));
+                for (int i = 0; i < 8; i++) sum = fmaf(x[8 * b + i], up, sum);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                bias[b] = sum * -0x1p-17f;
             }
         }
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int n = 0; n < S::kGroups; n++) {
-                if (edge && 2 * t + (i & 1) + 8 * (i >> 1) >= here) zero(vw[i][n]);
-                else load(vw[i][n], vl + at + ((i & 1) + 8 * (i >> 1)) * kRowBytes + n * 8 * S::kRun * (Q8 ? 1 : 2));
-            }
+    }
+
+    // this lane's places in a piece: dimensions 8 t of key row gq, kRun gq of value row 2 t (rows 8 further, and row 2 t + 1
+    // beside 2 t, are swizzled alike)
+    const uint32_t key_at = gq * kRowBytes + ((t * (Q8 ? 8 : 16)) ^ (S::key_swizzle(gq) * 16));
+    const uint32_t value_at = kValues + 2 * t * kRowBytes + ((gq * S::kRun * (Q8 ? 1 : 2)) ^ (S::value_swizzle(2 * t) * 16));
+
+    float2 o[S::kGroups][S::kRun] = {};
+    float m = -INFINITY, l = 0.0f;
+    int stage = 0;
+    for (int p0 = (int) c0 * kChunk + warp * 16; p0 < p_end; p0 += kChunk) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+        __syncwarp();  // the piece is here for every lane, and every lane is done with the one before, whose place is refilled
+        copy_piece();
+        const uint32_t at = ring + stage * S::kPiece;
+        const int here = found >> stage & 1 ? min(p_end - p0, 16) : 0;  // positions of the piece
+        stage = stage + 1 == S::kStages ? 0 : stage + 1;
+        const bool edge = here < 16 || p0 + 16 > all_see;
 
         // ---- scores: s[2 i + j] is position 2 t + j + 8 i of row gq ----
         float s[4];
+        {
+            uint32_t kd[2][Q8 ? S::kBlocks : 1];
+            if constexpr (Q8) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            s[2 * i] = s[2 * i + 1] = 0.0f;
-#pragma unroll
-            for (int b = 0; b < S::kBlocks; b++) {
-                const uint4 a0 = *reinterpret_cast<const uint4 *>(sh.sq[2 * b][lane]), a1 = *reinterpret_cast<const uint4 *>(sh.sq[2 * b + 1][lane]);
-                const uint32_t f0[4] = {a0.x, a0.y, a0.z, a0.w}, f1[4] = {a1.x, a1.y, a1.z, a1.w};
-                if constexpr (Q8) {
-                    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    const uint32_t w0 = kw[i][b][0] ^ 0x80808080u, w1 = kw[i][b][1] ^ 0x80808080u;
-                    mma(part, f0, halves(w0, 0x4140), halves(w0, 0x4342));
-                    mma(part, f1, halves(w1, 0x4140), halves(w1, 0x4342));
-                    s[2 * i] = fmaf(half_of(kd[i], b), part[0] + part[2], s[2 * i]);
-                    s[2 * i + 1] = fmaf(half_of(kd[i], S::kBlocks + b), part[1] + part[3], s[2 * i + 1]);
-                } else {
-                    mma(sum, f0, kw[i][b][0], kw[i][b][1]);
-                    mma(sum, f1, kw[i][b][2], kw[i][b][3]);
-                }
+                for (int i = 0; i < 2; i++) lds(kd[i], at + kKeyScales + (2 * t + 8 * i) * S::kScaleBytes);
             }
-            if constexpr (!Q8) {
-                s[2 * i] = sum[0] + sum[2];
-                s[2 * i + 1] = sum[1] + sum[3];
+            float sum[2][4] = {};
+            float2 part[2] = {};
+#pragma unroll
+            for (int b = 0; b < S::kBlocks; b++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    uint32_t w[S::kKeyWords];
+                    lds(w, S::along(at + key_at, b * (Q8 ? 32 : 64)) + i * 8 * kRowBytes);
+                    if constexpr (Q8) {
+                        float r[4] = {bias[b], bias[b], 0.0f, 0.0f};
+                        const uint32_t w0 = w[0] ^ 0x80808080u, w1 = w[1] ^ 0x80808080u;
+                        mma(r, qf[2 * b], __byte_perm(w0, 0, 0x4140), __byte_perm(w0, 0, 0x4342));
+                        mma(r, qf[2 * b + 1], __byte_perm(w1, 0, 0x4140), __byte_perm(w1, 0, 0x4342));
+                        part[i] = __ffma2_rn(make_float2(half_of(kd[i], b), half_of(kd[i], S::kBlocks + b)),
+                                             __fadd2_rn(make_float2(r[0], r[1]), make_float2(r[2], r[3])), part[i]);
+                    } else {
+                        mma(sum[i], qf[2 * b], w[0], w[1]);
+                        mma(sum[i], qf[2 * b + 1], w[2], w[3]);
+                    }
+                }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                if constexpr (!Q8) part[i] = __fadd2_rn(make_float2(sum[i][0], sum[i][1]), make_float2(sum[i][2], sum[i][3]));
+                s[2 * i] = part[i].x * factor;
+                s[2 * i + 1] = part[i].y * factor;
             }
         }
-#pragma unroll
-        for (int i = 0; i < 4; i++) s[i] *= factor;
         if (edge) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -343,33 +418,42 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
         const float base = m_new == -INFINITY ? 0.0f : m_new;
         const float keep = ex2(m - base);
         m = m_new;
-        float p[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) p[i] = ex2(s[i] - base);
-        l = fmaf(l, keep, (p[0] + p[1]) + (p[2] + p[3]));
-
-        // ---- o = o keep + P V ----
+        for (int i = 0; i < 4; i++) s[i] = ex2(s[i] - base);
+        l = fmaf(l, keep, (s[0] + s[1]) + (s[2] + s[3]));
         uint32_t pf[4];  // the weights' fragment: hi, lo of positions 2 t, 2 t + 1, then of 2 t + 8, 2 t + 9
-        split(p[0], p[1], pf[0], pf[1]);
-        split(p[2], p[3], pf[2], pf[3]);
+        split(s[0], s[1], pf[0], pf[1]);
+        split(s[2], s[3], pf[2], pf[3]);
+
+        // ---- o = o keep + P V: values of rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9, the positions whose weights this lane holds ----
+        const float2 keep2 = make_float2(keep, keep);
+        auto values = [&](uint32_t(&w)[4][S::kValueWords], int n) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                lds(w[i], (Q8 ? S::along(at + value_at, 32 * n) : at + value_at + 16 * S::kRun * n) + ((i & 1) + 8 * (i >> 1)) * kRowBytes);
+        };
         if constexpr (Q8) {
+            uint32_t vd[2][S::kBlocks];
+#pragma unroll
+            for (int i = 0; i < 2; i++) lds(vd[i], at + kValueScales + (2 * t + 8 * i) * S::kScaleBytes);
+            using Fragment = uint32_t[4];
             // one block of 32 dimensions: weights times scales (fragment a), times 2^k and back where `down` is not 1
-            auto block = [&](int b, const uint32_t(&a)[4], auto scaled, float down) {
-                // two rows' four bytes each, interleaved: (row, row + 1) pairs of dimensions 0, 1 and 2, 3
-                const uint32_t x0 = __byte_perm(vw[0][b][0], vw[1][b][0], 0x5140) ^ 0x80808080u;
-                const uint32_t x1 = __byte_perm(vw[0][b][0], vw[1][b][0], 0x7362) ^ 0x80808080u;
-                const uint32_t y0 = __byte_perm(vw[2][b][0], vw[3][b][0], 0x5140) ^ 0x80808080u;
-                const uint32_t y1 = __byte_perm(vw[2][b][0], vw[3][b][0], 0x7362) ^ 0x80808080u;
+            auto block = [&](int b, const Fragment & a, auto scaled, float down) {
+                uint32_t w[4][S::kValueWords], x[2][2];  // two rows' four bytes each, interleaved: (row, row + 1) pairs
+                values(w, b);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    x[i][0] = __byte_perm(w[2 * i][0], w[2 * i + 1][0], 0x5140) ^ 0x80808080u;
+                    x[i][1] = __byte_perm(w[2 * i][0], w[2 * i + 1][0], 0x7362) ^ 0x80808080u;
+                }
 #pragma unroll
                 for (int n = 0; n < 4; n++) {
-                    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                     const uint32_t sel = n & 1 ? 0x4342 : 0x4140;
-                    mma(part, a, halves(n < 2 ? x0 : x1, sel), halves(n < 2 ? y0 : y1, sel));
-                    part[0] += part[2];
-                    part[1] += part[3];
-                    if constexpr (decltype(scaled)::value) part[0] *= down, part[1] *= down;
-                    o[b][n][0] = fmaf(o[b][n][0], keep, part[0]);
-                    o[b][n][1] = fmaf(o[b][n][1], keep, part[1]);
+                    mma(r, a, halves(x[0][n / 2], sel), halves(x[1][n / 2], sel));
+                    float2 part = __fadd2_rn(make_float2(r[0], r[1]), make_float2(r[2], r[3]));
+                    if constexpr (decltype(scaled)::value) part.x *= down, part.y *= down;
+                    o[b][n] = __ffma2_rn(o[b][n], keep2, part);
                 }
             };
             // Scales between 2^-14 and 2 (nearly always all of them) multiply the weights' halves in F16 pairs: the
@@ -385,10 +469,13 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                 auto go = [&](auto index) {
                     constexpr int b = decltype(index)::value;
                     if constexpr (b < S::kBlocks) {
-                        const __half2 d0 = h2(pair_of<b, S::kBlocks + b>(vd[0])), d1 = h2(pair_of<b, S::kBlocks + b>(vd[1]));
-                        const __half2 w0 = __hmul2_rn(h2(pf[0]), d0), w1 = __hmul2_rn(h2(pf[2]), d1);
-                        const uint32_t a[4] = {u32(w0), u32(__hfma2(h2(pf[1]), d0, __hfma2(h2(pf[0]), d0, __hneg2(w0)))), u32(w1),
-                                               u32(__hfma2(h2(pf[3]), d1, __hfma2(h2(pf[2]), d1, __hneg2(w1))))};
+                        Fragment a;
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const __half2 d = h2(pair_of<b, S::kBlocks + b>(vd[i])), hi = h2(pf[2 * i]), w = __hmul2_rn(hi, d);
+                            a[2 * i] = u32(w);
+                            a[2 * i + 1] = u32(__hfma2(h2(pf[2 * i + 1]), d, __hfma2(hi, d, __hneg2(w))));
+                        }
                         block(b, a, std::false_type{}, 1.0f);
                     }
                 };
@@ -396,14 +483,15 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                 go(std::integral_constant<int, 3>{}), go(std::integral_constant<int, 4>{}), go(std::integral_constant<int, 5>{});
                 go(std::integral_constant<int, 6>{}), go(std::integral_constant<int, 7>{});
             } else {
-                // any scales: the product in float32, times a power of two that brings the tile's largest scale below 1
+                // any scales: the product in float32, times a power of two that brings the piece's largest scale below 1
 #pragma unroll
                 for (int b = 0; b < S::kBlocks; b++) {
-                    float d[4];
+                    float d[4], big = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
+                    for (int i = 0; i < 4; i++) {
                         d[i] = 2 * t + (i & 1) + 8 * (i >> 1) < here ? half_of(vd[i >> 1], (i & 1) * S::kBlocks + b) : 0.0f;
-                    float big = fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fabsf(d[3])));
+                        big = fmaxf(big, fabsf(d[i]));
+                    }
                     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
                     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
                     int e = (int) (__float_as_uint(big) >> 23);
@@ -411,48 +499,50 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                     const float up = __uint_as_float((uint32_t) (253 - e) << 23), down = __uint_as_float((uint32_t) (e + 1) << 23);
                     float w[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) w[i] = edge && p[i] == 0.0f ? 0.0f : p[i] * (d[i] * up);
-                    uint32_t a[4];
+                    for (int i = 0; i < 4; i++) w[i] = edge && s[i] == 0.0f ? 0.0f : s[i] * (d[i] * up);
+                    Fragment a;
                     split(w[0], w[1], a[0], a[1]);
                     split(w[2], w[3], a[2], a[3]);
                     block(b, a, std::true_type{}, down);
                 }
             }
         } else {
-            auto product = [&](bool mine) {
+            // `below`: rows from this place in the piece on enter as zeros
+            auto product = [&](int below, bool mine) {
 #pragma unroll
-                for (int n = 0; n < S::kGroups; n++)
+                for (int n = 0; n < S::kGroups; n++) {
+                    uint32_t w[4][S::kValueWords];
+                    values(w, n);
+                    if (below < 16) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+#pragma unroll
+                            for (int r = 0; r < S::kValueWords; r++)
+                                if (2 * t + (i & 1) + 8 * (i >> 1) >= below) w[i][r] = 0;
+                    }
 #pragma unroll
                     for (int r = 0; r < S::kRun; r++) {
                         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                         const uint32_t sel = r & 1 ? 0x7632 : 0x5410;
-                        mma(part, pf, __byte_perm(vw[0][n][r / 2], vw[1][n][r / 2], sel), __byte_perm(vw[2][n][r / 2], vw[3][n][r / 2], sel));
-                        if (mine) {
-                            o[n][r][0] = fmaf(o[n][r][0], keep, part[0] + part[2]);
-                            o[n][r][1] = fmaf(o[n][r][1], keep, part[1] + part[3]);
-                        }
+                        mma(part, pf, __byte_perm(w[0][r / 2], w[1][r / 2], sel), __byte_perm(w[2][r / 2], w[3][r / 2], sel));
+                        if (mine) o[n][r] = __ffma2_rn(o[n][r], keep2, __fadd2_rn(make_float2(part[0], part[1]), make_float2(part[2], part[3])));
                     }
+                }
             };
             if (edge && g.n_tok > 1) {
                 // Where rows see different positions, a value that is NaN or infinite must not meet the weight 0 of a row
-                // that does not see it: one product per token, from the last, with the values behind its position zeroed.
-                const int first = tile * kRows / g.group;
-                for (int token = min((tile * kRows + kRows - 1) / g.group, g.n_tok - 1); token >= first; token--) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (p0 + 2 * t + (i & 1) + 8 * (i >> 1) >= all_see + token) {
-#pragma unroll
-                            for (int n = 0; n < S::kGroups; n++) zero(vw[i][n]);
-                        }
-                    product(row.token == token);
-                }
+                // that does not see it: one product per token, with the values behind its position zeroed.
+                const int last = min((tile * kRows + kRows - 1) / g.group, g.n_tok - 1);
+                for (int token = tile * kRows / g.group; token <= last; token++) product(all_see + token - p0, row.token == token);
             } else {
-                product(true);
+                product(16, true);
             }
         }
     }
 
     // ---- join the warps ----
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();  // the ring is read no more: o takes its place
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     if (t == 0) {
@@ -462,17 +552,18 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
 #pragma unroll
     for (int n = 0; n < S::kGroups; n++)
 #pragma unroll
-        for (int r = 0; r < S::kRun; r++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) sh.so[warp][gq][n * 8 * S::kRun + (2 * t + j) * S::kRun + r] = o[n][r][j];
+        for (int r = 0; r < S::kRun; r++) {
+            sh.o(warp, gq, n * 8 * S::kRun + 2 * t * S::kRun + r) = o[n][r].x;
+            sh.o(warp, gq, n * 8 * S::kRun + (2 * t + 1) * S::kRun + r) = o[n][r].y;
+        }
     __syncthreads();
 }
 
 // The CTA's sum of the warps' results for one row: the factors of the warps, and m and l.
-template <int D>
+template <bool Q8, int D>
 struct Joined {
     float f[kWarps], m, l;
-    __device__ __forceinline__ Joined(const Shared<D> & sh, int i) {
+    __device__ __forceinline__ Joined(const Shared<Q8, D> & sh, int i) {
         m = -INFINITY;
         l = 0.0f;
 #pragma unroll
@@ -484,19 +575,21 @@ struct Joined {
             l = fmaf(sh.sl[w][i], f[w], l);
         }
     }
-    __device__ __forceinline__ float value(const Shared<D> & sh, int i, int d) const {
+    __device__ __forceinline__ float value(const Shared<Q8, D> & sh, int i, int d) const {
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) v = fmaf(sh.so[w][i][d], f[w], v);
+        for (int w = 0; w < kWarps; w++) v = fmaf(sh.o(w, i, d), f[w], v);
         return v;
     }
 };
 
 // The work cut by positions: CTA b takes chunks [b share, (b + 1) share) of all items' chunks.
 template <bool Q8, int D>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
+__global__ void __launch_bounds__(kThreads, Shape<Q8, D>::kCtas)
     kv_attention_kernel(KvView c, Geometry g, const float * __restrict__ q, int64_t ldq, float scale, float * __restrict__ out, float * __restrict__ ws) {
-    __shared__ Shared<D> sh;
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
+    const Shared<Q8, D> sh{ring, sm, sl};
     __shared__ int64_t red[kWarps + 2];
     const int tid = threadIdx.x;
     pdl_launch_dependents();
@@ -524,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
         attend<Q8, D>(c, g, q, ldq, scale, sh, seq, len, h, tile, c0, c1);
 
         const int i = tid / 16;  // a row per 16 threads
-        const Joined<D> all(sh, i);
+        const Joined<Q8, D> all(sh, i);
         const Row row = row_of(g, h, tile, i);
         if (c0 == 0 && c1 == chunks) {  // the whole item
             const float inv = all.l != 0.0f ? 1.0f / all.l : 0.0f;
@@ -545,9 +638,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
 // The work cut by items: a cluster of `cluster` CTAs per item, each an equal run of its chunks, joined over distributed
 // shared memory: the CTA of rank r writes rows r, r + cluster, ... One launch, and no length but the item's own is read.
 template <bool Q8, int D>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
+__global__ void __launch_bounds__(kThreads, Shape<Q8, D>::kCtas)
     kv_attention_item_kernel(KvView c, Geometry g, int cluster, const float * __restrict__ q, int64_t ldq, float scale, float * __restrict__ out) {
-    __shared__ Shared<D> sh;
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
+    const Shared<Q8, D> sh{ring, sm, sl};
     __shared__ float jm[kRows], jl[kRows];
     const int tid = threadIdx.x, rank = blockIdx.x % cluster;
     const int64_t unit = blockIdx.x / cluster, seq = unit / g.items;
@@ -557,8 +652,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
     attend<Q8, D>(c, g, q, ldq, scale, sh, seq, len, h, tile, c0, c1);
     {
         const int i = tid / 16;
-        const Joined<D> all(sh, i);
-        for (int d = tid & 15; d < D; d += 16) sh.so[0][i][d] = all.value(sh, i, d);  // read and written by this thread alone
+        const Joined<Q8, D> all(sh, i);
+        for (int d = tid & 15; d < D; d += 16) sh.o(0, i, d) = all.value(sh, i, d);  // read and written by this thread alone
         if ((tid & 15) == 0) jm[i] = all.m, jl[i] = all.l;
     }
     const cooperative_groups::cluster_group group = cooperative_groups::this_cluster();
@@ -573,7 +668,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<Q8, D>())
         for (int r = 0; r < cluster; r++) {
             const float f = ex2(*group.map_shared_rank(&jm[i], r) - base);
             l = fmaf(*group.map_shared_rank(&jl[i], r), f, l);
-            v = fmaf(*group.map_shared_rank(&sh.so[0][i][d], r), f, v);
+            v = fmaf(*group.map_shared_rank(&sh.o(0, i, d), r), f, v);
         }
         out[((seq * g.n_tok + row.token) * g.n_head + row.head) * D + d] = l != 0.0f ? v * (1.0f / l) : 0.0f;
     }
@@ -676,6 +771,17 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv_attention_join_kernel(KvVi
     }
 }
 
+// Calls f with the Shape of a cache's type and head_dim.
+template <class F>
+void with_shape(bool q8, int D, F f) {
+    switch (D) {
+    case 64: q8 ? f(Shape<true, 64>{}) : f(Shape<false, 64>{}); break;
+    case 96: q8 ? f(Shape<true, 96>{}) : f(Shape<false, 96>{}); break;
+    case 128: q8 ? f(Shape<true, 128>{}) : f(Shape<false, 128>{}); break;
+    default: q8 ? f(Shape<true, 256>{}) : f(Shape<false, 256>{}); break;
+    }
+}
+
 Geometry geometry(const b200_context * ctx, const b200_kv_cache * c, int64_t max_pages, int64_t n_seq, int64_t n_tok, int64_t n_head) {
     Geometry g;
     g.n_tok = (int) n_tok;
@@ -684,7 +790,7 @@ Geometry geometry(const b200_context * ctx, const b200_kv_cache * c, int64_t max
     g.tiles = (g.n_tok * g.group + kRows - 1) / kRows;
     g.items = (int64_t) c->n_kv_head * g.tiles;
     g.n_seq = n_seq;
-    g.ctas = (int64_t) ctx->num_sms * ctas_per_sm_of(c->type == B200_TYPE_Q8_0, c->head_dim);
+    with_shape(c->type == B200_TYPE_Q8_0, c->head_dim, [&](auto shape) { g.ctas = (int64_t) ctx->num_sms * decltype(shape)::kCtas; });
     // By items when the lengths that the table allows are short: the cluster (1 to 8 CTAs) is the largest that all items fit
     // on the GPU with at once.
     const int64_t most = (max_pages * c->page_size + kChunk - 1) / kChunk;  // chunks of the longest sequence there can be
@@ -695,8 +801,16 @@ Geometry geometry(const b200_context * ctx, const b200_kv_cache * c, int64_t max
     return g;
 }
 
+// ready: the kernels of this shape may use their shared memory on this device (set once per context).
 template <bool Q8, int D>
-cudaError_t launch(const KvView & c, const Geometry & g, const float * q, int64_t ldq, float scale, float * out, float * ws, cudaStream_t st) {
+cudaError_t launch(const KvView & c, const Geometry & g, const float * q, int64_t ldq, float scale, float * out, float * ws, cudaStream_t st,
+                   bool ready) {
+    constexpr int kBytes = Shape<Q8, D>::kBytes;
+    if (!ready) {
+        cudaError_t e = cudaFuncSetAttribute(kv_attention_kernel<Q8, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kv_attention_item_kernel<Q8, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+        if (e != cudaSuccess) return e;
+    }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     cfg.stream = st;
@@ -705,12 +819,13 @@ cudaError_t launch(const KvView & c, const Geometry & g, const float * q, int64_
     if (g.cluster) {
         cfg.gridDim = dim3((unsigned) (g.n_seq * g.items * g.cluster), 1, 1);
         cfg.blockDim = dim3(kThreads, 1, 1);
+        cfg.dynamicSmemBytes = kBytes;
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = (unsigned) g.cluster;
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         return cudaLaunchKernelEx(&cfg, kv_attention_item_kernel<Q8, D>, c, g, g.cluster, q, ldq, scale, out);
     }
-    kv_attention_kernel<Q8, D><<<(unsigned) g.ctas, kThreads, 0, st>>>(c, g, q, ldq, scale, out, ws);
+    kv_attention_kernel<Q8, D><<<(unsigned) g.ctas, kThreads, kBytes, st>>>(c, g, q, ldq, scale, out, ws);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     cfg.gridDim = dim3((unsigned) (g.n_seq * g.items * kRows), 1, 1);
@@ -757,19 +872,14 @@ b200_status b200_kv_attention(b200_context * ctx, void * stream, const b200_kv_c
     DeviceScope scope(ctx->device);
     if (scope.status != cudaSuccess) return kv_cuda(ctx, scope.status, what);
     cudaStream_t st = stream ? (cudaStream_t) stream : ctx->stream;
-    auto go = [&](auto dim) {
-        constexpr int D = decltype(dim)::value;
-        return cache->type == B200_TYPE_Q8_0 ? launch<true, D>(c, g, q, ldq, scale, out, (float *) workspace, st)
-                                             : launch<false, D>(c, g, q, ldq, scale, out, (float *) workspace, st);
-    };
+    const bool q8 = cache->type == B200_TYPE_Q8_0;
+    const unsigned bit = 1u << ((c.head_dim / 32) + (q8 ? 16 : 0));
     cudaError_t e = cudaErrorInvalidValue;
-    switch (c.head_dim) {
-    case 64: e = go(std::integral_constant<int, 64>{}); break;
-    case 96: e = go(std::integral_constant<int, 96>{}); break;
-    case 128: e = go(std::integral_constant<int, 128>{}); break;
-    case 256: e = go(std::integral_constant<int, 256>{}); break;
-    default: break;
-    }
+    with_shape(q8, c.head_dim, [&](auto shape) {
+        using S = decltype(shape);
+        e = launch<S::kKeyWords == 2, 32 * S::kBlocks>(c, g, q, ldq, scale, out, (float *) workspace, st, ctx->kv_shapes & bit);
+    });
+    if (e == cudaSuccess) ctx->kv_shapes |= bit;
     return kv_cuda(ctx, e, what);
 }
 
