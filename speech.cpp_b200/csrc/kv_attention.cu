@@ -60,10 +60,16 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// d = A B + c; the second form with c = (c0, c0, 0, 0): all of it in rows 0-7.
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0 = 0.0f) {
+    const float c[4] = {c0, c0, 0.0f, 0.0f};
+    mma(d, a, b0, b1, c);
 }
 
 // 16 bytes from global to shared memory, asynchronously; zeros when !there (nothing is read then).
@@ -384,15 +390,15 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                     uint32_t w[S::kKeyWords];
                     lds(w, S::along(at + key_at, b * (Q8 ? 32 : 64)) + i * 8 * kRowBytes);
                     if constexpr (Q8) {
-                        float r[4] = {bias[b], bias[b], 0.0f, 0.0f};
+                        float r[4];
                         const uint32_t w0 = w[0] ^ 0x80808080u, w1 = w[1] ^ 0x80808080u;
-                        mma(r, qf[2 * b], __byte_perm(w0, 0, 0x4140), __byte_perm(w0, 0, 0x4342));
-                        mma(r, qf[2 * b + 1], __byte_perm(w1, 0, 0x4140), __byte_perm(w1, 0, 0x4342));
+                        mma(r, qf[2 * b], __byte_perm(w0, 0, 0x4140), __byte_perm(w0, 0, 0x4342), bias[b]);
+                        mma(r, qf[2 * b + 1], __byte_perm(w1, 0, 0x4140), __byte_perm(w1, 0, 0x4342), r);
                         part[i] = __ffma2_rn(make_float2(half_of(kd[i], b), half_of(kd[i], S::kBlocks + b)),
                                              __fadd2_rn(make_float2(r[0], r[1]), make_float2(r[2], r[3])), part[i]);
                     } else {
-                        mma(sum[i], qf[2 * b], w[0], w[1]);
-                        mma(sum[i], qf[2 * b + 1], w[2], w[3]);
+                        mma(sum[i], qf[2 * b], w[0], w[1], sum[i]);
+                        mma(sum[i], qf[2 * b + 1], w[2], w[3], sum[i]);
                     }
                 }
 #pragma unroll
@@ -448,7 +454,7 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                 }
 #pragma unroll
                 for (int n = 0; n < 4; n++) {
-                    float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float r[4];
                     const uint32_t sel = n & 1 ? 0x4342 : 0x4140;
                     mma(r, a, halves(x[0][n / 2], sel), halves(x[1][n / 2], sel));
                     float2 part = __fadd2_rn(make_float2(r[0], r[1]), make_float2(r[2], r[3]));
@@ -522,7 +528,7 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                     }
 #pragma unroll
                     for (int r = 0; r < S::kRun; r++) {
-                        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        float part[4];
                         const uint32_t sel = r & 1 ? 0x7632 : 0x5410;
                         mma(part, pf, __byte_perm(w[0][r / 2], w[1][r / 2], sel), __byte_perm(w[2][r / 2], w[3][r / 2], sel));
                         if (mine) o[n][r] = __ffma2_rn(o[n][r], keep2, __fadd2_rn(make_float2(part[0], part[1]), make_float2(part[2], part[3])));
