@@ -60,15 +60,15 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// d = A B + c; the second form with c = (c0, c0, 0, 0): all of it in rows 0-7.
+// d = A B + c, and d = A B.
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0 = 0.0f) {
-    const float c[4] = {c0, c0, 0.0f, 0.0f};
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    const float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     mma(d, a, b0, b1, c);
 }
 
@@ -133,15 +133,16 @@ struct Shape {
     static constexpr int kGroups = D / (8 * kRun);
     static constexpr int kKeyWords = Q8 ? 2 : 4;           // a lane's words of a row's 32 dimensions
     static constexpr int kValueWords = Q8 ? 1 : kRun / 2;  // a lane's words of a row's group
-    // A piece is 16 positions: its key rows, value rows, and their scales. Each warp has a ring of kStages pieces in shared
-    // memory; the ring's depth and the CTAs per SM fill its 227 KB.
+    // A piece is 16 positions: its key rows, value rows, and their scales. A warp takes kSub pieces at a time, from a ring of
+    // kStages such in shared memory; the ring's depth and the CTAs per SM fill its 227 KB.
+    static constexpr int kSub = Q8 && D <= 128 ? 2 : 1;
     static constexpr int kRowBytes = Q8 ? D : 2 * D;
     static constexpr int kScaleBytes = Q8 ? D / 16 : 0;    // of a row
     static constexpr int kPiece = 32 * (kRowBytes + kScaleBytes);
-    static constexpr int kStages = Q8 ? (D == 256 ? 3 : 4) : (D == 64 ? 4 : D == 256 ? 2 : 3);
-    static constexpr int kCtas = Q8 ? (D == 256 ? 2 : 3) : (D == 256 ? 1 : D == 128 ? 2 : 3);
+    static constexpr int kStages = Q8 ? 3 : (D == 64 ? 4 : D == 256 ? 2 : 3);
+    static constexpr int kCtas = Q8 ? (D == 64 ? 3 : 2) : (D == 256 ? 1 : D == 128 ? 2 : 3);
     static_assert(D == 96 || kPiece % 128 == 0, "swizzled pieces keep the ring's alignment");
-    static constexpr int kBytes = kWarps * kStages * kPiece;
+    static constexpr int kStage = kSub * kPiece, kBytes = kWarps * kStages * kStage;
     // The 16-byte chunks of a row are stored at chunk ^ swizzle(row), so that the lanes that read together read different
     // banks: fragments of keys are read from rows 0-7 (Q8_0: four rows and 32 bytes of each at a time, F16: two rows and
     // 64), of values from rows 0, 2, 4, 6 and so on. Rows of 96 or 192 bytes are apart by themselves (keys) or in pairs. Both
@@ -232,10 +233,10 @@ __device__ __forceinline__ Row row_of(const Geometry & g, int h, int tile, int i
 // A CTA's shared memory: the warps' rings of pieces, and, at the ring's place once a run is done, each warp's o.
 template <bool Q8, int D>
 struct Shared {
-    uint8_t * ring;  // dynamic: [kWarps][kStages][kPiece]
+    uint8_t * ring;  // dynamic: [kWarps][kStages][kSub][kPiece]
     float (*sm)[kRows];
     float (*sl)[kRows];
-    static constexpr int kRingBytes = Shape<Q8, D>::kStages * Shape<Q8, D>::kPiece;
+    static constexpr int kRingBytes = Shape<Q8, D>::kStages * Shape<Q8, D>::kStage;
     static constexpr int kPitch = D + 4;
     static_assert(kRows * kPitch * 4 <= kRingBytes, "a warp's o fits its ring");
     __device__ __forceinline__ float & o(int w, int row, int d) const {
@@ -256,64 +257,80 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
     const int all_see = (int) len - g.n_tok + 1;  // positions below are seen by every row
     const int seen = row.there ? all_see + row.token : 0;
 
-    // ---- the ring: pieces p0 = c0 * 64 + warp * 16, then every 64, copied kStages - 1 ahead ----
+    // ---- the ring: steps of kSub pieces, the warps in turn through [c0 * 64, c1 * 64), copied kStages - 1 ahead ----
+    constexpr int kSub = S::kSub, kStep = kWarps * 16 * kSub;
     const uint32_t ring = smem_addr(sh.ring) + warp * Shared<Q8, D>::kRingBytes;
     const int64_t page_bytes = (int64_t) c.n_kv_head * c.page_size * kRowBytes;
-    const int64_t head_bytes = (int64_t) h * c.page_size * kRowBytes;
-    const int page_step = kChunk / c.page_size, slot_step = kChunk % c.page_size;
-    int p_copy = (int) c0 * kChunk + warp * 16;  // the next piece to copy, its place in the table, its page (asked for early)
+    const uint8_t * kh = c.k + (int64_t) h * c.page_size * kRowBytes + lane * 16;
+    const int64_t to_values = c.v - c.k;
+    const uint8_t * scales = nullptr;  // this lane's 16 bytes of a piece's scales: the keys', then the values'
+    if constexpr (Q8)
+        scales = reinterpret_cast<const uint8_t *>(lane < S::kScaleBytes ? c.kd : c.vd) + (int64_t) h * c.page_size * S::kScaleBytes +
+                 (lane < S::kScaleBytes ? lane : lane - S::kScaleBytes) * 16;
+    const int page_step = kStep / c.page_size, slot_step = kStep % c.page_size;
+    int p_copy = (int) c0 * kChunk + warp * 16 * kSub;  // the next step to copy, its place in the table, its pages (asked for early)
     int in_table = p_copy / c.page_size, slot = p_copy % c.page_size, stage_copy = 0;
-    int page = p_copy < p_end ? kv_page(c, seq, in_table, lane == 0) : -1;
+    int page[kSub];
+    auto find_pages = [&] {
+#pragma unroll
+        for (int u = 0; u < kSub; u++)
+            page[u] = p_copy + 16 * u < p_end ? kv_page(c, seq, in_table + (slot + 16 * u >= c.page_size), lane == 0) : -1;
+    };
+    find_pages();
     // where this lane's first 16 bytes of a piece go: row lane / (chunks of a row), chunk lane % (chunks of a row)
     const uint32_t copy_key = lane * 16 ^ S::key_swizzle(lane / (kRowBytes / 16)) * 16;
     const uint32_t copy_value = lane * 16 ^ S::value_swizzle(lane / (kRowBytes / 16)) * 16;
-    unsigned found = 0;  // bit per stage: its piece has a page
-    auto copy_piece = [&] {
+    unsigned found = 0;  // bit kSub stage + u: the piece has a page
+    auto copy_step = [&] {
         if (p_copy < p_end) {
-            const int here = page < 0 ? 0 : p_end - p_copy;  // rows of the piece; the others are zeros
-            const int64_t at = head_bytes + max(page, 0) * page_bytes + (int64_t) slot * kRowBytes;
-            const uint32_t to = ring + stage_copy * S::kPiece;
-            constexpr int kRowChunks = kRowBytes / 16, kCopies = kRowChunks / 2;  // a piece's rows are contiguous: 16 kRowChunks chunks
-            auto each = [&](auto whole) {
 #pragma unroll
-                for (int j = 0; j < kCopies; j++) {
-                    uint32_t key_to, value_to, r;
-                    if constexpr (S::kSwizzled) {  // 32 / kRowChunks rows further each time: their swizzle is a constant
-                        r = lane / kRowChunks + j * (32 / kRowChunks);
-                        key_to = (copy_key ^ (S::key_swizzle(j * (32 / kRowChunks)) * 16)) + j * 512;
-                        value_to = (copy_value ^ (S::value_swizzle(j * (32 / kRowChunks)) * 16)) + j * 512;
-                    } else {
-                        r = (lane + 32 * j) / kRowChunks;
-                        key_to = value_to = (lane + 32 * j) * 16;
+            for (int u = 0; u < kSub; u++) {
+                const int here = page[u] < 0 ? 0 : p_end - p_copy - 16 * u;  // rows of the piece; the others are zeros
+                const int in_page = slot + 16 * u - (slot + 16 * u >= c.page_size ? c.page_size : 0);
+                const int64_t at = max(page[u], 0) * page_bytes + in_page * kRowBytes;
+                const uint8_t * from = kh + at;
+                const uint32_t to = ring + stage_copy * S::kStage + u * S::kPiece;
+                constexpr int kRowChunks = kRowBytes / 16, kCopies = kRowChunks / 2;  // a piece's rows are contiguous: 16 kRowChunks chunks
+                auto each = [&](auto whole) {
+#pragma unroll
+                    for (int j = 0; j < kCopies; j++) {
+                        uint32_t key_to, value_to, r;
+                        if constexpr (S::kSwizzled) {  // 32 / kRowChunks rows further each time: their swizzle is a constant
+                            r = lane / kRowChunks + j * (32 / kRowChunks);
+                            key_to = (copy_key ^ (S::key_swizzle(j * (32 / kRowChunks)) * 16)) + j * 512;
+                            value_to = (copy_value ^ (S::value_swizzle(j * (32 / kRowChunks)) * 16)) + j * 512;
+                        } else {
+                            r = (lane + 32 * j) / kRowChunks;
+                            key_to = value_to = (lane + 32 * j) * 16;
+                        }
+                        if constexpr (decltype(whole)::value) {
+                            copy16(to + key_to, from + j * 512);
+                            copy16(to + kValues + value_to, from + to_values + j * 512);
+                        } else {
+                            copy16(to + key_to, from + j * 512, (int) r < here);
+                            copy16(to + kValues + value_to, from + to_values + j * 512, (int) r < here);
+                        }
                     }
-                    if constexpr (decltype(whole)::value) {
-                        copy16(to + key_to, c.k + at + lane * 16 + j * 512);
-                        copy16(to + kValues + value_to, c.v + at + lane * 16 + j * 512);
-                    } else {
-                        copy16(to + key_to, c.k + at + lane * 16 + j * 512, (int) r < here);
-                        copy16(to + kValues + value_to, c.v + at + lane * 16 + j * 512, (int) r < here);
-                    }
+                };
+                if (here >= 16) each(std::true_type{});
+                else each(std::false_type{});
+                if constexpr (Q8) {  // whole, rows behind the end too: they lie in the page
+                    if (lane < 2 * S::kScaleBytes) copy16(to + kKeyScales + lane * 16, scales + at / 16, page[u] >= 0);
                 }
-            };
-            if (here >= 16) each(std::true_type{});
-            else each(std::false_type{});
-            if constexpr (Q8) {  // whole, rows behind the end too: they lie in the page
-                if (lane < S::kScaleBytes) copy16(to + kKeyScales + lane * 16, reinterpret_cast<const uint8_t *>(c.kd) + at / 16 + lane * 16, page >= 0);
-                else if (lane < 2 * S::kScaleBytes)
-                    copy16(to + kKeyScales + lane * 16, reinterpret_cast<const uint8_t *>(c.vd) + at / 16 + (lane - S::kScaleBytes) * 16, page >= 0);
+                const unsigned bit = 1u << (kSub * stage_copy + u);
+                found = page[u] < 0 ? found & ~bit : found | bit;
             }
-            found = page < 0 ? found & ~(1u << stage_copy) : found | 1u << stage_copy;
-            p_copy += kChunk;
+            p_copy += kStep;
             in_table += page_step;
             slot += slot_step;
             if (slot >= c.page_size) slot -= c.page_size, in_table++;
-            if (p_copy < p_end) page = kv_page(c, seq, in_table, lane == 0);
+            find_pages();
             stage_copy = stage_copy + 1 == S::kStages ? 0 : stage_copy + 1;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
-    for (int n = 0; n < S::kStages - 1; n++) copy_piece();
+    for (int n = 0; n < S::kStages - 1; n++) copy_step();
 
     // ---- the query tile's fragments ----
     // k step 2 j + b of lane (gq, t) holds dimensions 32 j + 8 t + 4 b .. + 3 of row gq: hi in registers 0 and 2, lo in
@@ -364,22 +381,29 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
     float2 o[S::kGroups][S::kRun] = {};
     float m = -INFINITY, l = 0.0f;
     int stage = 0;
-    for (int p0 = (int) c0 * kChunk + warp * 16; p0 < p_end; p0 += kChunk) {
+    for (int p0 = (int) c0 * kChunk + warp * 16 * kSub; p0 < p_end; p0 += kStep) {
         asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
-        __syncwarp();  // the piece is here for every lane, and every lane is done with the one before, whose place is refilled
-        copy_piece();
-        const uint32_t at = ring + stage * S::kPiece;
-        const int here = found >> stage & 1 ? min(p_end - p0, 16) : 0;  // positions of the piece
+        __syncwarp();  // the step is here for every lane, and every lane is done with the one before, whose place is refilled
+        const uint32_t at = ring + stage * S::kStage;
+        int here[kSub];  // positions of the pieces
+        bool edge = p0 + 16 * kSub > all_see;
+#pragma unroll
+        for (int u = 0; u < kSub; u++) {
+            here[u] = found >> (kSub * stage + u) & 1 ? p_end - p0 - 16 * u : 0;
+            edge = edge || here[u] < 16;
+        }
         stage = stage + 1 == S::kStages ? 0 : stage + 1;
-        const bool edge = here < 16 || p0 + 16 > all_see;
+        copy_step();
 
-        // ---- scores: s[2 i + j] is position 2 t + j + 8 i of row gq ----
-        float s[4];
-        {
+        // ---- scores: s[u][2 i + j] is position 16 u + 2 t + j + 8 i of row gq ----
+        float s[kSub][4];
+#pragma unroll
+        for (int u = 0; u < kSub; u++) {
+            const uint32_t keys = at + u * S::kPiece + key_at;
             uint32_t kd[2][Q8 ? S::kBlocks : 1];
             if constexpr (Q8) {
 #pragma unroll
-                for (int i = 0; i < 2; i++) lds(kd[i], at + kKeyScales + (2 * t + 8 * i) * S::kScaleBytes);
+                for (int i = 0; i < 2; i++) lds(kd[i], at + u * S::kPiece + kKeyScales + (2 * t + 8 * i) * S::kScaleBytes);
             }
             float sum[2][4] = {};
             float2 part[2] = {};
@@ -388,14 +412,14 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     uint32_t w[S::kKeyWords];
-                    lds(w, S::along(at + key_at, b * (Q8 ? 32 : 64)) + i * 8 * kRowBytes);
+                    lds(w, S::along(keys, b * (Q8 ? 32 : 64)) + i * 8 * kRowBytes);
                     if constexpr (Q8) {
                         float r[4];
                         const uint32_t w0 = w[0] ^ 0x80808080u, w1 = w[1] ^ 0x80808080u;
-                        mma(r, qf[2 * b], __byte_perm(w0, 0, 0x4140), __byte_perm(w0, 0, 0x4342), bias[b]);
+                        mma(r, qf[2 * b], __byte_perm(w0, 0, 0x4140), __byte_perm(w0, 0, 0x4342));
                         mma(r, qf[2 * b + 1], __byte_perm(w1, 0, 0x4140), __byte_perm(w1, 0, 0x4342), r);
-                        part[i] = __ffma2_rn(make_float2(half_of(kd[i], b), half_of(kd[i], S::kBlocks + b)),
-                                             __fadd2_rn(make_float2(r[0], r[1]), make_float2(r[2], r[3])), part[i]);
+                        const float2 whole = __fadd2_rn(make_float2(r[0], r[1]), __fadd2_rn(make_float2(r[2], r[3]), make_float2(bias[b], bias[b])));
+                        part[i] = __ffma2_rn(make_float2(half_of(kd[i], b), half_of(kd[i], S::kBlocks + b)), whole, part[i]);
                     } else {
                         mma(sum[i], qf[2 * b], w[0], w[1], sum[i]);
                         mma(sum[i], qf[2 * b + 1], w[2], w[3], sum[i]);
@@ -404,59 +428,90 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 if constexpr (!Q8) part[i] = __fadd2_rn(make_float2(sum[i][0], sum[i][1]), make_float2(sum[i][2], sum[i][3]));
-                s[2 * i] = part[i].x * factor;
-                s[2 * i + 1] = part[i].y * factor;
+                s[u][2 * i] = part[i].x * factor;
+                s[u][2 * i + 1] = part[i].y * factor;
             }
         }
         if (edge) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int j = 2 * t + (i & 1) + 8 * (i >> 1);
-                if (j >= here || p0 + j >= seen) s[i] = -INFINITY;
-            }
+            for (int u = 0; u < kSub; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int j = 2 * t + (i & 1) + 8 * (i >> 1);
+                    if (j >= here[u] || p0 + 16 * u + j >= seen) s[u][i] = -INFINITY;
+                }
         }
 
         // ---- weights: m is the running maximum less kShift (-infinity before any score) ----
-        float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kSub; u++) top = fmaxf(top, fmaxf(fmaxf(s[u][0], s[u][1]), fmaxf(s[u][2], s[u][3])));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const float m_new = fmaxf(m, top - kShift);
         const float base = m_new == -INFINITY ? 0.0f : m_new;
         const float keep = ex2(m - base);
         m = m_new;
+        l *= keep;
+        uint32_t pf[kSub][4];  // the weights' fragments: hi, lo of positions 2 t, 2 t + 1, then of 2 t + 8, 2 t + 9
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[i] = ex2(s[i] - base);
-        l = fmaf(l, keep, (s[0] + s[1]) + (s[2] + s[3]));
-        uint32_t pf[4];  // the weights' fragment: hi, lo of positions 2 t, 2 t + 1, then of 2 t + 8, 2 t + 9
-        split(s[0], s[1], pf[0], pf[1]);
-        split(s[2], s[3], pf[2], pf[3]);
+        for (int u = 0; u < kSub; u++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[u][i] = ex2(s[u][i] - base);
+            l += (s[u][0] + s[u][1]) + (s[u][2] + s[u][3]);
+            split(s[u][0], s[u][1], pf[u][0], pf[u][1]);
+            split(s[u][2], s[u][3], pf[u][2], pf[u][3]);
+        }
 
         // ---- o = o keep + P V: values of rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9, the positions whose weights this lane holds ----
         const float2 keep2 = make_float2(keep, keep);
-        auto values = [&](uint32_t(&w)[4][S::kValueWords], int n) {
+        using Words = uint32_t[4][S::kValueWords];
+        auto values = [&](Words & w, int u, int n) {
+            const uint32_t first = at + u * S::kPiece + value_at;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                lds(w[i], (Q8 ? S::along(at + value_at, 32 * n) : at + value_at + 16 * S::kRun * n) + ((i & 1) + 8 * (i >> 1)) * kRowBytes);
+            for (int i = 0; i < 4; i++) lds(w[i], (Q8 ? S::along(first, 32 * n) : first + 16 * S::kRun * n) + ((i & 1) + 8 * (i >> 1)) * kRowBytes);
         };
         if constexpr (Q8) {
-            uint32_t vd[2][S::kBlocks];
+            uint32_t vd[kSub][2][S::kBlocks];
 #pragma unroll
-            for (int i = 0; i < 2; i++) lds(vd[i], at + kValueScales + (2 * t + 8 * i) * S::kScaleBytes);
-            using Fragment = uint32_t[4];
-            // one block of 32 dimensions: weights times scales (fragment a), times 2^k and back where `down` is not 1
-            auto block = [&](int b, const Fragment & a, auto scaled, float down) {
-                uint32_t w[4][S::kValueWords], x[2][2];  // two rows' four bytes each, interleaved: (row, row + 1) pairs
-                values(w, b);
+            for (int u = 0; u < kSub; u++)
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    x[i][0] = __byte_perm(w[2 * i][0], w[2 * i + 1][0], 0x5140) ^ 0x80808080u;
-                    x[i][1] = __byte_perm(w[2 * i][0], w[2 * i + 1][0], 0x7362) ^ 0x80808080u;
+                for (int i = 0; i < 2; i++) lds(vd[u][i], at + u * S::kPiece + kValueScales + (2 * t + 8 * i) * S::kScaleBytes);
+            if (edge) {  // scales behind the end (their weights are 0) as 1, whatever lies there
+#pragma unroll
+                for (int u = 0; u < kSub; u++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const uint32_t a = 2 * t + 8 * i < here[u] ? 0 : 0x3c00, b = 2 * t + 1 + 8 * i < here[u] ? 0 : 0x3c00;
+#pragma unroll
+                        for (int n = 0; n < S::kBlocks; n++) {  // halves 2 n and 2 n + 1: the first kBlocks are row 2 t's
+                            const uint32_t low = 2 * n < S::kBlocks ? a : b, high = 2 * n + 1 < S::kBlocks ? a : b;
+                            if (low) vd[u][i][n] = (vd[u][i][n] & 0xffff0000u) | low;
+                            if (high) vd[u][i][n] = (vd[u][i][n] & 0xffffu) | high << 16;
+                        }
+                    }
+            }
+            using Fragments = uint32_t[S::kSub][4];
+            // one block of 32 dimensions: weights times scales (fragments a), times 2^k and back where `down` is not 1
+            auto block = [&](int b, const Fragments & a, auto scaled, float down) {
+                uint32_t x[S::kSub][2][2];  // two rows' four bytes each, interleaved: (row, row + 1) pairs
+#pragma unroll
+                for (int u = 0; u < kSub; u++) {
+                    Words w;
+                    values(w, u, b);
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        x[u][i][0] = __byte_perm(w[2 * i][0], w[2 * i + 1][0], 0x5140) ^ 0x80808080u;
+                        x[u][i][1] = __byte_perm(w[2 * i][0], w[2 * i + 1][0], 0x7362) ^ 0x80808080u;
+                    }
                 }
 #pragma unroll
                 for (int n = 0; n < 4; n++) {
                     float r[4];
                     const uint32_t sel = n & 1 ? 0x4342 : 0x4140;
-                    mma(r, a, halves(x[0][n / 2], sel), halves(x[1][n / 2], sel));
+                    mma(r, a[0], halves(x[0][0][n / 2], sel), halves(x[0][1][n / 2], sel));
+#pragma unroll
+                    for (int u = 1; u < kSub; u++) mma(r, a[u], halves(x[u][0][n / 2], sel), halves(x[u][1][n / 2], sel), r);
                     float2 part = __fadd2_rn(make_float2(r[0], r[1]), make_float2(r[2], r[3]));
                     if constexpr (decltype(scaled)::value) part.x *= down, part.y *= down;
                     o[b][n] = __ffma2_rn(o[b][n], keep2, part);
@@ -465,23 +520,27 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
             // Scales between 2^-14 and 2 (nearly always all of them) multiply the weights' halves in F16 pairs: the
             // product's rounding error is exact in F16 and goes to the low half. The weights being up to 2^14 and the low
             // halves reaching 2^-24, nothing overflows and what is lost is below 2^-24 of the largest weight's product.
-            uint32_t low = vd[0][0], high = vd[0][0];
+            uint32_t low = vd[0][0][0], high = vd[0][0][0];
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int u = 0; u < kSub; u++)
 #pragma unroll
-                for (int b = 0; b < S::kBlocks; b++) low = __vminu2(low, vd[i][b]), high = __vmaxu2(high, vd[i][b]);
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int b = 0; b < S::kBlocks; b++) low = __vminu2(low, vd[u][i][b]), high = __vmaxu2(high, vd[u][i][b]);
             const bool plain = (low & 0xffffu) >= 0x0400u && low >= 0x04000000u && (high & 0xffffu) < 0x4000u && high < 0x40000000u;
             if (__all_sync(0xffffffffu, plain)) {
                 auto go = [&](auto index) {
                     constexpr int b = decltype(index)::value;
                     if constexpr (b < S::kBlocks) {
-                        Fragment a;
+                        Fragments a;
 #pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            const __half2 d = h2(pair_of<b, S::kBlocks + b>(vd[i])), hi = h2(pf[2 * i]), w = __hmul2_rn(hi, d);
-                            a[2 * i] = u32(w);
-                            a[2 * i + 1] = u32(__hfma2(h2(pf[2 * i + 1]), d, __hfma2(hi, d, __hneg2(w))));
-                        }
+                        for (int u = 0; u < kSub; u++)
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                const __half2 d = h2(pair_of<b, S::kBlocks + b>(vd[u][i])), hi = h2(pf[u][2 * i]), w = __hmul2_rn(hi, d);
+                                a[u][2 * i] = u32(w);
+                                a[u][2 * i + 1] = u32(__hfma2(h2(pf[u][2 * i + 1]), d, __hfma2(hi, d, __hneg2(w))));
+                            }
                         block(b, a, std::false_type{}, 1.0f);
                     }
                 };
@@ -489,36 +548,42 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                 go(std::integral_constant<int, 3>{}), go(std::integral_constant<int, 4>{}), go(std::integral_constant<int, 5>{});
                 go(std::integral_constant<int, 6>{}), go(std::integral_constant<int, 7>{});
             } else {
-                // any scales: the product in float32, times a power of two that brings the piece's largest scale below 1
+                // any scales: the product in float32, times a power of two that brings the step's largest scale below 1
 #pragma unroll
                 for (int b = 0; b < S::kBlocks; b++) {
-                    float d[4], big = 0.0f;
+                    float d[kSub][4], big = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        d[i] = 2 * t + (i & 1) + 8 * (i >> 1) < here ? half_of(vd[i >> 1], (i & 1) * S::kBlocks + b) : 0.0f;
-                        big = fmaxf(big, fabsf(d[i]));
-                    }
+                    for (int u = 0; u < kSub; u++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            d[u][i] = half_of(vd[u][i >> 1], (i & 1) * S::kBlocks + b);
+                            big = fmaxf(big, fabsf(d[u][i]));
+                        }
                     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
                     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
                     int e = (int) (__float_as_uint(big) >> 23);
                     if (e == 0 || e == 255) e = 126;
                     const float up = __uint_as_float((uint32_t) (253 - e) << 23), down = __uint_as_float((uint32_t) (e + 1) << 23);
-                    float w[4];
+                    Fragments a;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) w[i] = edge && s[i] == 0.0f ? 0.0f : s[i] * (d[i] * up);
-                    Fragment a;
-                    split(w[0], w[1], a[0], a[1]);
-                    split(w[2], w[3], a[2], a[3]);
+                    for (int u = 0; u < kSub; u++) {
+                        float w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) w[i] = edge && s[u][i] == 0.0f ? 0.0f : s[u][i] * (d[u][i] * up);
+                        split(w[0], w[1], a[u][0], a[u][1]);
+                        split(w[2], w[3], a[u][2], a[u][3]);
+                    }
                     block(b, a, std::true_type{}, down);
                 }
             }
         } else {
+            static_assert(Q8 || kSub == 1, "an F16 step is one piece");
             // `below`: rows from this place in the piece on enter as zeros
             auto product = [&](int below, bool mine) {
 #pragma unroll
                 for (int n = 0; n < S::kGroups; n++) {
-                    uint32_t w[4][S::kValueWords];
-                    values(w, n);
+                    Words w;
+                    values(w, 0, n);
                     if (below < 16) {
 #pragma unroll
                         for (int i = 0; i < 4; i++)
@@ -530,7 +595,7 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                     for (int r = 0; r < S::kRun; r++) {
                         float part[4];
                         const uint32_t sel = r & 1 ? 0x7632 : 0x5410;
-                        mma(part, pf, __byte_perm(w[0][r / 2], w[1][r / 2], sel), __byte_perm(w[2][r / 2], w[3][r / 2], sel));
+                        mma(part, pf[0], __byte_perm(w[0][r / 2], w[1][r / 2], sel), __byte_perm(w[2][r / 2], w[3][r / 2], sel));
                         if (mine) o[n][r] = __ffma2_rn(o[n][r], keep2, __fadd2_rn(make_float2(part[0], part[1]), make_float2(part[2], part[3])));
                     }
                 }
