@@ -139,8 +139,8 @@ struct Shape {
     static constexpr int kRowBytes = Q8 ? D : 2 * D;
     static constexpr int kScaleBytes = Q8 ? D / 16 : 0;    // of a row
     static constexpr int kPiece = 32 * (kRowBytes + kScaleBytes);
-    static constexpr int kStages = Q8 ? 3 : (D == 64 ? 4 : D == 256 ? 2 : 3);
-    static constexpr int kCtas = Q8 ? (D == 64 ? 3 : 2) : (D == 256 ? 1 : D == 128 ? 2 : 3);
+    static constexpr int kStages = Q8 ? (D == 128 ? 2 : 3) : (D == 64 ? 4 : D == 256 ? 2 : 3);
+    static constexpr int kCtas = Q8 ? (D == 64 || D == 128 ? 3 : 2) : (D == 256 ? 1 : D == 128 ? 2 : 3);
     static_assert(D == 96 || kPiece % 128 == 0, "swizzled pieces keep the ring's alignment");
     static constexpr int kStage = kSub * kPiece, kBytes = kWarps * kStages * kStage;
     // The 16-byte chunks of a row are stored at chunk ^ swizzle(row), so that the lanes that read together read different

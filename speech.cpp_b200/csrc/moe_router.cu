@@ -1,14 +1,15 @@
 // moe_router.cu — the expert router (b200_moe_router): scores, group choice, top-k and weights of each row of logits.
 //
-// One warp per row; lane l holds experts l, l + 32, ... as 32-bit keys whose unsigned order is the values' order, and each
-// round of the top-k is a maximum over the lane's keys and one reduction instruction over the warp (another finds the lowest
-// expert with that key). Which experts are chosen has to be right where they are nearly equal:
-//  - without bias and groups the logits themselves are the keys, which decides exactly;
+// A warp takes one to 32 / top_k rows; lane l holds a row's experts l, l + 32, ... as 32-bit keys whose unsigned order is the
+// values' order, sorted within the lane. A round of the top-k is one reduction instruction over the lanes' first keys and a
+// shift in the lane that won. The keys' low bits hold the expert's place in the lane, so values that differ only there, or by
+// less than their rounding error, are not told apart; which experts are chosen has to be right all the same:
+//  - without bias and groups the keys are the logits, and rows with equal truncated neighbours are done again with whole keys;
 //  - otherwise scores are computed in float32 first, with a bound on their error, and the row is accepted if every
 //    comparison that decides (neighbours among the chosen and the next one, the last group kept and the first one left) is
-//    wider than that. The few rows that are not, and rows with anything non-finite, are done again in double.
-// The weights of the chosen, one per lane, are double either way. Reading the logits takes 4 B per expert; the rounds' some
-// 30 to 60 instructions each decide the time (about 10 us per 16384 rows of 256 experts against 2.7 us of HBM).
+//    wider than that. The rows that are not (some in a thousand), and rows with anything non-finite, are done in double.
+// The weights of the chosen are double either way, one lane for each, of all the warp's rows at once. Reading the logits
+// takes 4 B per expert (2.7 us of HBM for 16384 rows of 256); the instructions decide the time.
 #include <cmath>
 
 #include "kv.cuh"
@@ -26,6 +27,8 @@ struct RouterParams {
     // groups in the float32 pass: `lanes` lanes (a power of two, n_group * lanes <= 32) for each, the scores of a group
     // `pitch` floats apart in shared memory so that a step's lanes read different banks
     int lanes, pitch;
+    // a warp takes `rows` rows; each has `seats` lanes (a power of two, at least top_k) for its weights
+    int rows, seats;
     unsigned inv;  // expert e's group is e * inv >> 21 (e < 1024)
 };
 
@@ -136,11 +139,16 @@ __device__ __noinline__ int choose_exactly(const RouterParams & a, const float *
 
 // ---- rows by keys -----------------------------------------------------------------------------------------------------
 
-// The `rounds` largest of the warp's keys (0: out), ties to the lowest expert: lane k gets the k-th's expert and key.
+// The top_k largest of the warp's keys (0: out), ties to the lowest expert, exactly: lane k gets the k-th's expert. For rows
+// whose logits come too close for packed keys.
 template <int EPL>
-__device__ __forceinline__ void largest(unsigned (&key)[EPL], int rounds, int & id, unsigned & found) {
+__device__ __noinline__ int choose_by_logit(const RouterParams & a, const float * __restrict__ logits) {
     const int lane = threadIdx.x & 31;
-    for (int k = 0; k < rounds; k++) {
+    unsigned key[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; i++) key[i] = i * 32 + lane < a.E ? key_of(clean(logits[i * 32 + lane])) : 0;
+    int id = 0;
+    for (int k = 0; k < a.top_k; k++) {
         unsigned best = key[0];
 #pragma unroll
         for (int i = 1; i < EPL; i++) best = max(best, key[i]);
@@ -153,8 +161,27 @@ __device__ __forceinline__ void largest(unsigned (&key)[EPL], int rounds, int & 
 #pragma unroll
         for (int i = 0; i < EPL; i++)
             if (at == i * 32u + lane) key[i] = 0;
-        if (lane == k) id = (int) at, found = top;
+        if (lane == k) id = (int) at;
     }
+    return id;
+}
+
+// Sorts a lane's keys, largest first (odd-even merge sort).
+template <int N>
+__device__ __forceinline__ void sort_keys(unsigned (&key)[N]) {
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; i++)
+                    if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const unsigned x = key[i + j], y = key[i + j + k];
+                        key[i + j] = max(x, y);
+                        key[i + j + k] = min(x, y);
+                    }
 }
 
 // The larger pair of (a1 >= a2) and (b1 >= b2).
@@ -163,125 +190,152 @@ __device__ __forceinline__ void merge2(float & a1, float & a2, float b1, float b
     a1 = fmaxf(a1, b1);
 }
 
-// EPL: experts per lane. BY_LOGIT: no bias and no groups.
+// EPL: experts per lane (a power of two). BY_LOGIT: no bias and no groups.
 template <int EPL, bool BY_LOGIT>
 __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a, const float * __restrict__ logits, const float * __restrict__ bias,
                                                                  int64_t T, int32_t * __restrict__ ids, float * __restrict__ w) {
     extern __shared__ float shared[];  // groups: each warp's scores, [n_group][pitch]
+    constexpr unsigned kIndex = EPL - 1;  // a key's low bits give way to the expert's place in its lane, the first ones largest
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t t = blockIdx.x * (int64_t) kWarps + warp;
-    if (t >= T) return;
-    const float * row = logits + t * a.E;
-    float x[EPL], top = -INFINITY;
+    const int64_t t0 = (blockIdx.x * (int64_t) kWarps + warp) * a.rows;
+    int id = 0;                     // lane r * seats + k: the k-th expert of row t0 + r, and what its weight needs
+    float my_top = -INFINITY;
+    double my_total = 0.0;
+    for (int r = 0; r < a.rows && t0 + r < T; r++) {
+        const float * row = logits + (t0 + r) * a.E;
+        float x[EPL], top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < EPL; i++) {
-        x[i] = i * 32 + lane < a.E ? clean(row[i * 32 + lane]) : -INFINITY;
-        top = fmaxf(top, x[i]);
-    }
-    top = value_of(__reduce_max_sync(kAll, key_of(top)));
+        for (int i = 0; i < EPL; i++) {
+            x[i] = i * 32 + lane < a.E ? clean(row[i * 32 + lane]) : -INFINITY;
+            top = fmaxf(top, x[i]);
+        }
+        top = value_of(__reduce_max_sync(kAll, key_of(top)));
 
-    int id = 0;
-    if constexpr (BY_LOGIT) {
-        unsigned key[EPL], found = 0;
-#pragma unroll
-        for (int i = 0; i < EPL; i++) key[i] = i * 32 + lane < a.E ? key_of(x[i]) : 0;
-        largest<EPL>(key, a.top_k, id, found);
-    } else {
-        // float32 scores; `off` bounds the error of each. __expf(-d) is within 2 + 1.173 d units of its last place, so within
-        // 2^-22 absolutely; a sigmoid is that, a rounded sum and a quotient of two units: below 2^-20. A softmax's sum adds up
-        // to 32 terms per lane and five times over the warp (37 roundings, below 2^-18.7) of terms that are off by some 2^-20.7
-        // of the sum at most: below 2^-17 of the largest term. The sum with the bias rounds once more.
-        float sum = 0.0f, c[EPL], far = 0.0f;
-        bool finite = true;
-#pragma unroll
-        for (int i = 0; i < EPL; i++) {
-            const bool there = i * 32 + lane < a.E;
-            finite = finite && (!there || fabsf(x[i]) < INFINITY);
-            c[i] = a.score == B200_ROUTER_SIGMOID ? __fdividef(1.0f, 1.0f + __expf(-x[i])) : __expf(x[i] - top);
-            sum += there ? c[i] : 0.0f;
-        }
-        const float inv = a.score == B200_ROUTER_SOFTMAX ? __fdividef(1.0f, warp_sum(sum)) : 1.0f;
         unsigned key[EPL];
+        float off = 0.0f;  // bound on the error of a score
+        bool sure = true;
+        if constexpr (BY_LOGIT) {
 #pragma unroll
-        for (int i = 0; i < EPL; i++) {
-            const int e = i * 32 + lane;
-            c[i] *= inv;
-            if (bias && e < a.E) c[i] += bias[e];
-            finite = finite && (e >= a.E || fabsf(c[i]) < INFINITY);
-            if (e < a.E) far = fmaxf(far, fabsf(c[i]));
-            key[i] = e < a.E ? key_of(c[i]) : 0;
-        }
-        far = value_of(__reduce_max_sync(kAll, key_of(far)));
-        const float off = (a.score == B200_ROUTER_SIGMOID ? 0x1p-20f : 0x1p-17f * inv) + 0x1p-23f * far;
-        bool sure = __all_sync(kAll, finite);
-        if (sure && a.n_group > 1) {
-            const int size = a.E / a.n_group;
-            float * mine = shared + warp * a.n_group * a.pitch;
+            for (int i = 0; i < EPL; i++) key[i] = i * 32 + lane < a.E ? key_of(x[i]) : 0;
+        } else {
+            // float32 scores; `off` bounds the error of each. __expf(-d) is within 2 + 1.173 d units of its last place, so within
+            // 2^-22 absolutely; a sigmoid is that, a rounded sum and a quotient of two units: below 2^-20. A softmax's sum adds up
+            // to 32 terms per lane and five times over the warp (37 roundings, below 2^-18.7) of terms that are off by some
+            // 2^-20.7 of the sum at most: below 2^-17 of the largest term. The sum with the bias rounds once more.
+            float sum = 0.0f, c[EPL], far = 0.0f, flaw = 0.0f;  // flaw: NaN where a logit or a score is NaN or infinite
+#pragma unroll
+            for (int i = 0; i < EPL; i++) {
+                c[i] = a.score == B200_ROUTER_SIGMOID ? __fdividef(1.0f, 1.0f + __expf(-x[i])) : __expf(x[i] - top);
+                sum += i * 32 + lane < a.E ? c[i] : 0.0f;
+            }
+            const float inv = a.score == B200_ROUTER_SOFTMAX ? __fdividef(1.0f, warp_sum(sum)) : 1.0f;
 #pragma unroll
             for (int i = 0; i < EPL; i++) {
                 const int e = i * 32 + lane;
-                const int of = group_of(a, e);
-                if (e < a.E) mine[of * a.pitch + e - of * size] = c[i];
+                const bool there = e < a.E;
+                c[i] *= inv;
+                if (bias && there) c[i] += bias[e];
+                if (there) {
+                    far = fmaxf(far, fabsf(c[i]));
+                    flaw = fmaf(0.0f, x[i], fmaf(0.0f, c[i], flaw));
+                }
+                key[i] = there ? key_of(c[i]) : 0;
             }
-            __syncwarp();
-            const int g = lane / a.lanes;
-            float b1 = -INFINITY, b2 = -INFINITY;
-            if (g < a.n_group)
-                for (int n = lane % a.lanes; n < size; n += a.lanes) merge2(b1, b2, mine[g * a.pitch + n], -INFINITY);
-            for (int o = a.lanes >> 1; o > 0; o >>= 1) {
-                const float o1 = __shfl_xor_sync(kAll, b1, o), o2 = __shfl_xor_sync(kAll, b2, o);
-                merge2(b1, b2, o1, o2);
-            }
-            __syncwarp();
-            const float score = a.group_top == 2 && size > 1 ? b1 + b2 : b1;
-            // lane n: group n's score, and how many are before it
-            const float s = __shfl_sync(kAll, score, lane < a.n_group ? lane * a.lanes : 0);
-            int ahead = 0;
-            for (int n = 0; n < a.n_group; n++) {
-                const float other = __shfl_sync(kAll, s, n);
-                ahead += other > s || (other == s && n < lane);
-            }
-            const bool in = lane < a.n_group && ahead < a.topk_group;
-            const unsigned kept = __ballot_sync(kAll, in);
-            if (a.topk_group < a.n_group) {
-                const float low = value_of(__reduce_min_sync(kAll, in ? key_of(s) : kAll));
-                const float high = value_of(__reduce_max_sync(kAll, lane < a.n_group && !in ? key_of(s) : 0));
-                sure = low - high > 4.0f * off + 0x1p-22f * fmaxf(fabsf(low), fabsf(high));
-            }
+            sure = __all_sync(kAll, flaw == 0.0f);
+            far = value_of(__reduce_max_sync(kAll, key_of(far)));
+            off = (a.score == B200_ROUTER_SIGMOID ? 0x1p-20f : 0x1p-17f * inv) + 0x1p-23f * far;
+            if (sure && a.n_group > 1) {
+                const int size = a.E / a.n_group;
+                float * mine = shared + warp * a.n_group * a.pitch;
 #pragma unroll
-            for (int i = 0; i < EPL; i++) {
-                const int e = i * 32 + lane;
-                if (e < a.E && !(kept >> group_of(a, e) & 1)) key[i] = 0;
+                for (int i = 0; i < EPL; i++) {
+                    const int e = i * 32 + lane, of = group_of(a, e);
+                    if (e < a.E) mine[of * a.pitch + e - of * size] = c[i];
+                }
+                __syncwarp();
+                const int g = lane / a.lanes;
+                float b1 = -INFINITY, b2 = -INFINITY;
+                if (g < a.n_group)
+                    for (int n = lane % a.lanes; n < size; n += a.lanes) merge2(b1, b2, mine[g * a.pitch + n], -INFINITY);
+                for (int o = a.lanes >> 1; o > 0; o >>= 1) {
+                    const float o1 = __shfl_xor_sync(kAll, b1, o), o2 = __shfl_xor_sync(kAll, b2, o);
+                    merge2(b1, b2, o1, o2);
+                }
+                __syncwarp();
+                const float score = a.group_top == 2 && size > 1 ? b1 + b2 : b1;
+                // lane n: group n's score, and how many are before it
+                const float s = __shfl_sync(kAll, score, lane < a.n_group ? lane * a.lanes : 0);
+                int ahead = 0;
+                for (int n = 0; n < a.n_group; n++) {
+                    const float other = __shfl_sync(kAll, s, n);
+                    ahead += other > s || (other == s && n < lane);
+                }
+                const bool in = lane < a.n_group && ahead < a.topk_group;
+                const unsigned kept = __ballot_sync(kAll, in);
+                if (a.topk_group < a.n_group) {
+                    const float low = value_of(__reduce_min_sync(kAll, in ? key_of(s) : kAll));
+                    const float high = value_of(__reduce_max_sync(kAll, lane < a.n_group && !in ? key_of(s) : 0));
+                    sure = low - high > 4.0f * off + 0x1p-22f * fmaxf(fabsf(low), fabsf(high));
+                }
+#pragma unroll
+                for (int i = 0; i < EPL; i++) {
+                    const int e = i * 32 + lane;
+                    if (e < a.E && !(kept >> group_of(a, e) & 1)) key[i] = 0;
+                }
             }
         }
         if (sure) {
-            // one more than the chosen, to see that it lies apart (key 0: there is none)
-            unsigned found = 0;
-            const int left = a.E / a.n_group * a.topk_group, rounds = a.top_k < 32 && a.top_k < left ? a.top_k + 1 : a.top_k;
-            largest<EPL>(key, rounds, id, found);
-            const unsigned next = __shfl_down_sync(kAll, found, 1);
-            const bool apart = lane + 1 >= rounds || value_of(found) - value_of(next) > 2.0f * off;
-            sure = __all_sync(kAll, apart) && (rounds > a.top_k || a.top_k == left);
+#pragma unroll
+            for (int i = 0; i < EPL; i++) key[i] = key[i] ? (key[i] & ~kIndex) | (kIndex - i) : 0;
+            sort_keys(key);
+            // one more than the chosen, if there is one, to see that it lies apart
+            const int left = a.E / a.n_group * a.topk_group;
+            unsigned last = 0;
+            for (int k = 0; k <= a.top_k && k < left; k++) {
+                const unsigned best = __reduce_max_sync(kAll, key[0]);
+                const bool won = key[0] == best;
+                const unsigned who = __ballot_sync(kAll, won);
+                if (lane == r * a.seats + k && k < a.top_k) id = (int) (kIndex - (best & kIndex)) * 32 + __ffs(who) - 1;
+                if (k > 0) sure = sure && (BY_LOGIT ? (last | kIndex) > (best | kIndex) : value_of(last & ~kIndex) - value_of(best | kIndex) > 2.0f * off);
+                sure = sure && __popc(who) == 1;  // of equal keys one would be lost
+                last = best;
+#pragma unroll
+                for (int i = 0; i + 1 < EPL; i++) key[i] = won ? key[i + 1] : key[i];
+                key[EPL - 1] = won ? 0 : key[EPL - 1];
+            }
         }
-        if (!sure) id = choose_exactly<EPL>(a, row, bias, top);
+        if (!sure) {
+            int exact;
+            if constexpr (BY_LOGIT) exact = choose_by_logit<EPL>(a, row);
+            else exact = choose_exactly<EPL>(a, row, bias, top);
+            exact = __shfl_sync(kAll, exact, lane - r * a.seats);
+            if (lane >= r * a.seats && lane < r * a.seats + a.top_k) id = exact;
+        }
+        double total = 0.0;
+        if (!a.renorm && a.score == B200_ROUTER_SOFTMAX) {
+#pragma unroll
+            for (int i = 0; i < EPL; i++) total += term(a, x[i], top);
+            total = warp_sum_d(total);
+        }
+        if (lane >= r * a.seats) {
+            my_top = top;
+            my_total = total;
+        }
     }
 
-    // ---- weights: lane k's is the k-th chosen expert's ----
-    const bool chosen = lane < a.top_k;
-    double mine = chosen ? term(a, clean(row[id]), top) : 0.0;
+    // ---- weights, one expert of one row per lane ----
+    const int k = lane % a.seats;
+    const int64_t t = t0 + lane / a.seats;
+    const bool chosen = k < a.top_k && lane / a.seats < a.rows && t < T;
+    double mine = chosen ? term(a, clean(logits[t * a.E + id]), my_top) : 0.0;
     if (a.renorm) {
-        const double total = warp_sum_d(mine);
-        mine = total > 0.0 ? mine / total : 0.0;
-    } else if (a.score == B200_ROUTER_SOFTMAX) {
-        double total = 0.0;
-#pragma unroll
-        for (int i = 0; i < EPL; i++) total += term(a, x[i], top);
-        total = warp_sum_d(total);
-        mine = total > 0.0 ? mine / total : 0.0;
+        my_total = mine;
+        for (int o = a.seats >> 1; o > 0; o >>= 1) my_total += __shfl_xor_sync(kAll, my_total, o);
     }
+    if (a.renorm || a.score == B200_ROUTER_SOFTMAX) mine = my_total > 0.0 ? mine / my_total : 0.0;
     if (chosen) {
-        ids[t * a.top_k + lane] = id;
-        w[t * a.top_k + lane] = __double2float_rn(mine * (double) a.scale);
+        ids[t * a.top_k + k] = id;
+        w[t * a.top_k + k] = __double2float_rn(mine * (double) a.scale);
     }
 }
 
@@ -303,7 +357,11 @@ extern "C" b200_status b200_moe_router(b200_context * ctx, void * stream, const 
     if (T > (int64_t) INT32_MAX) return kv_fail(ctx, B200_ERR_INVALID, what, "more than 2^31 rows");
     DeviceScope scope(ctx->device);
     if (scope.status != cudaSuccess) return kv_cuda(ctx, scope.status, what);
-    RouterParams a{r->n_expert, r->top_k, r->score, r->n_group, r->topk_group, r->group_top, r->renorm, r->scale, 1, 0, 0};
+    RouterParams a{r->n_expert, r->top_k, r->score, r->n_group, r->topk_group, r->group_top, r->renorm, r->scale, 1, 0, 1, 1, 0};
+    // Several rows per warp share the double arithmetic of the weights (a row has top_k of them, a warp 32 lanes), as long as
+    // that leaves eight warps to each SM.
+    while (a.seats < a.top_k) a.seats *= 2;
+    while (2 * a.rows * a.seats <= 32 && T >= (int64_t) ctx->num_sms * 8 * 2 * a.rows) a.rows *= 2;
     size_t smem = 0;
     if (a.n_group > 1) {
         const int size = a.E / a.n_group;
@@ -313,7 +371,7 @@ extern "C" b200_status b200_moe_router(b200_context * ctx, void * stream, const 
         smem = (size_t) kWarps * a.n_group * a.pitch * sizeof(float);  // at most 4 * (1024 + 32 * 31) * 4 B < 32 KB
     }
     cudaStream_t st = stream ? (cudaStream_t) stream : ctx->stream;
-    const unsigned grid = (unsigned) ((T + kWarps - 1) / kWarps);
+    const unsigned grid = (unsigned) ((T + kWarps * a.rows - 1) / (kWarps * a.rows));
     const bool by_logit = !bias && a.n_group == 1;
     auto go = [&](auto epl) {
         constexpr int EPL = decltype(epl)::value;
