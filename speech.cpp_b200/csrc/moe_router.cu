@@ -7,7 +7,8 @@
 //  - without bias and groups the keys are the logits, and rows with equal truncated neighbours are done again with whole keys;
 //  - otherwise scores are computed in float32 first, with a bound on their error, and the row is accepted if every
 //    comparison that decides (neighbours among the chosen and the next one, the last group kept and the first one left) is
-//    wider than that. The rows that are not (some in a thousand), and rows with anything non-finite, are done in double.
+//    wider than that. Where neighbours are closer (some rows in a thousand) the few candidates are ordered by their scores in
+//    double; where groups are, or anything is not finite, the row is done again in double.
 // The weights of the chosen are double either way, one lane for each, of all the warp's rows at once. Reading the logits
 // takes 4 B per expert (2.7 us of HBM for 16384 rows of 256); the instructions decide the time.
 #include <cmath>
@@ -190,14 +191,37 @@ __device__ __forceinline__ void merge2(float & a1, float & a2, float b1, float b
     a1 = fmaxf(a1, b1);
 }
 
-// EPL: experts per lane (a power of two). BY_LOGIT: no bias and no groups.
-template <int EPL, bool BY_LOGIT>
+// The order of a row's candidates (lane j: expert e, j < n) by their scores in double; lane k gets the k-th. top, sum: the
+// softmax's (sum in double).
+__device__ __noinline__ int order_exactly(const RouterParams & a, const float * __restrict__ logits, const float * __restrict__ bias, float top, double sum,
+                                          int e, int n) {
+    const int lane = threadIdx.x & 31;
+    double c = 0.0;
+    if (lane < n) {
+        c = term(a, logits[e], top);
+        if (a.score == B200_ROUTER_SOFTMAX) c /= sum;
+        if (bias) c += (double) bias[e];
+    }
+    int rank = 0;
+    for (int j = 0; j < n; j++) rank += before(__shfl_sync(kAll, c, j), __shfl_sync(kAll, e, j), c, e);
+    int id = 0;
+    for (int j = 0; j < n; j++) {
+        const int to = __shfl_sync(kAll, rank, j), of = __shfl_sync(kAll, e, j);
+        if (lane == to) id = of;
+    }
+    return id;
+}
+
+// EPL: experts per lane (a power of two). BY_LOGIT: no bias and no groups. FULL: there are 32 EPL experts.
+template <int EPL, bool BY_LOGIT, bool FULL>
 __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a, const float * __restrict__ logits, const float * __restrict__ bias,
                                                                  int64_t T, int32_t * __restrict__ ids, float * __restrict__ w) {
     extern __shared__ float shared[];  // groups: each warp's scores, [n_group][pitch]
     constexpr unsigned kIndex = EPL - 1;  // a key's low bits give way to the expert's place in its lane, the first ones largest
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t t0 = (blockIdx.x * (int64_t) kWarps + warp) * a.rows;
+    const int mine = FULL ? EPL : (a.E - lane + 31) / 32;  // this lane's experts
+    const bool softmax = a.score == B200_ROUTER_SOFTMAX;
     int id = 0;                     // lane r * seats + k: the k-th expert of row t0 + r, and what its weight needs
     float my_top = -INFINITY;
     double my_total = 0.0;
@@ -206,7 +230,7 @@ __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a,
         float x[EPL], top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < EPL; i++) {
-            x[i] = i * 32 + lane < a.E ? clean(row[i * 32 + lane]) : -INFINITY;
+            x[i] = i < mine ? clean(row[i * 32 + lane]) : -INFINITY;
             top = fmaxf(top, x[i]);
         }
         top = value_of(__reduce_max_sync(kAll, key_of(top)));
@@ -216,47 +240,60 @@ __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a,
         bool sure = true;
         if constexpr (BY_LOGIT) {
 #pragma unroll
-            for (int i = 0; i < EPL; i++) key[i] = i * 32 + lane < a.E ? key_of(x[i]) : 0;
+            for (int i = 0; i < EPL; i++) key[i] = i < mine ? key_of(x[i]) : 0;
         } else {
             // float32 scores; `off` bounds the error of each. __expf(-d) is within 2 + 1.173 d units of its last place, so within
-            // 2^-22 absolutely; a sigmoid is that, a rounded sum and a quotient of two units: below 2^-20. A softmax's sum adds up
-            // to 32 terms per lane and five times over the warp (37 roundings, below 2^-18.7) of terms that are off by some
-            // 2^-20.7 of the sum at most: below 2^-17 of the largest term. The sum with the bias rounds once more.
-            float sum = 0.0f, c[EPL], far = 0.0f, flaw = 0.0f;  // flaw: NaN where a logit or a score is NaN or infinite
+            // 2^-22 absolutely. A sigmoid of x has p (1 - p) (2 + 1.173 |x|) < 0.63 times 2^-23 of that, half of one from the
+            // rounded sum and two units (2^-23) from the quotient: below 2^-21. A softmax's sum adds up to 32 terms per lane and
+            // five times over the warp (37 roundings, below 2^-18.7) of terms that are off by some 2^-20.7 of the sum at most:
+            // below 2^-17 of the largest term. The sum with the bias rounds once more.
+            float c[EPL], far = 0.0f, flaw = 0.0f;  // flaw: NaN where a logit or a score is NaN or infinite
+            if (softmax) {
+                float sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < EPL; i++) {
-                c[i] = a.score == B200_ROUTER_SIGMOID ? __fdividef(1.0f, 1.0f + __expf(-x[i])) : __expf(x[i] - top);
-                sum += i * 32 + lane < a.E ? c[i] : 0.0f;
+                for (int i = 0; i < EPL; i++) {
+                    c[i] = __expf(x[i] - top);
+                    if (i < mine) sum += c[i];
+                }
+                const float inv = __fdividef(1.0f, warp_sum(sum));
+                off = 0x1p-17f * inv;
+#pragma unroll
+                for (int i = 0; i < EPL; i++) c[i] *= inv;
+            } else {
+                off = 0x1p-21f;
+#pragma unroll
+                for (int i = 0; i < EPL; i++) c[i] = __fdividef(1.0f, 1.0f + __expf(-x[i]));
             }
-            const float inv = a.score == B200_ROUTER_SOFTMAX ? __fdividef(1.0f, warp_sum(sum)) : 1.0f;
+            if (bias) {
+#pragma unroll
+                for (int i = 0; i < EPL; i++)
+                    if (i < mine) c[i] += bias[i * 32 + lane];
+            }
 #pragma unroll
             for (int i = 0; i < EPL; i++) {
-                const int e = i * 32 + lane;
-                const bool there = e < a.E;
-                c[i] *= inv;
-                if (bias && there) c[i] += bias[e];
-                if (there) {
+                if (i < mine) {
                     far = fmaxf(far, fabsf(c[i]));
                     flaw = fmaf(0.0f, x[i], fmaf(0.0f, c[i], flaw));
                 }
-                key[i] = there ? key_of(c[i]) : 0;
+                key[i] = i < mine ? key_of(c[i]) : 0;
             }
             sure = __all_sync(kAll, flaw == 0.0f);
             far = value_of(__reduce_max_sync(kAll, key_of(far)));
-            off = (a.score == B200_ROUTER_SIGMOID ? 0x1p-20f : 0x1p-17f * inv) + 0x1p-23f * far;
+            off += 0x1p-23f * far;
             if (sure && a.n_group > 1) {
                 const int size = a.E / a.n_group;
-                float * mine = shared + warp * a.n_group * a.pitch;
+                float * scores = shared + warp * a.n_group * a.pitch;
+                int of[EPL];
 #pragma unroll
                 for (int i = 0; i < EPL; i++) {
-                    const int e = i * 32 + lane, of = group_of(a, e);
-                    if (e < a.E) mine[of * a.pitch + e - of * size] = c[i];
+                    of[i] = group_of(a, i * 32 + lane);
+                    if (i < mine) scores[i * 32 + lane + of[i] * (a.pitch - size)] = c[i];
                 }
                 __syncwarp();
                 const int g = lane / a.lanes;
                 float b1 = -INFINITY, b2 = -INFINITY;
                 if (g < a.n_group)
-                    for (int n = lane % a.lanes; n < size; n += a.lanes) merge2(b1, b2, mine[g * a.pitch + n], -INFINITY);
+                    for (int n = lane % a.lanes; n < size; n += a.lanes) merge2(b1, b2, scores[g * a.pitch + n], -INFINITY);
                 for (int o = a.lanes >> 1; o > 0; o >>= 1) {
                     const float o1 = __shfl_xor_sync(kAll, b1, o), o2 = __shfl_xor_sync(kAll, b2, o);
                     merge2(b1, b2, o1, o2);
@@ -278,64 +315,91 @@ __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a,
                     sure = low - high > 4.0f * off + 0x1p-22f * fmaxf(fabsf(low), fabsf(high));
                 }
 #pragma unroll
-                for (int i = 0; i < EPL; i++) {
-                    const int e = i * 32 + lane;
-                    if (e < a.E && !(kept >> group_of(a, e) & 1)) key[i] = 0;
-                }
+                for (int i = 0; i < EPL; i++) key[i] = kept >> of[i] & 1 ? key[i] : 0;
             }
         }
+        int chosen = 0;  // lane k: the k-th expert
         if (sure) {
 #pragma unroll
-            for (int i = 0; i < EPL; i++) key[i] = key[i] ? (key[i] & ~kIndex) | (kIndex - i) : 0;
+            for (int i = 0; i < EPL; i++) key[i] = FULL && BY_LOGIT || key[i] ? (key[i] & ~kIndex) | (kIndex - i) : 0;
             sort_keys(key);
-            // one more than the chosen, if there is one, to see that it lies apart
+            // Round n leaves the n-th key, and the lanes that had it, in lane n: top_k rounds and one more (if there is another
+            // expert and a lane for it) to see that it lies apart.
             const int left = a.E / a.n_group * a.topk_group;
-            unsigned last = 0;
-            for (int k = 0; k <= a.top_k && k < left; k++) {
+            unsigned found = 0, who = 0;
+            int n = 0;
+            auto round = [&] {
                 const unsigned best = __reduce_max_sync(kAll, key[0]);
                 const bool won = key[0] == best;
-                const unsigned who = __ballot_sync(kAll, won);
-                if (lane == r * a.seats + k && k < a.top_k) id = (int) (kIndex - (best & kIndex)) * 32 + __ffs(who) - 1;
-                if (k > 0) sure = sure && (BY_LOGIT ? (last | kIndex) > (best | kIndex) : value_of(last & ~kIndex) - value_of(best | kIndex) > 2.0f * off);
-                sure = sure && __popc(who) == 1;  // of equal keys one would be lost
-                last = best;
+                const unsigned winners = __ballot_sync(kAll, won);
+                if (lane == n) found = best, who = winners;
 #pragma unroll
                 for (int i = 0; i + 1 < EPL; i++) key[i] = won ? key[i + 1] : key[i];
                 key[EPL - 1] = won ? 0 : key[EPL - 1];
+                n++;
+                return best;
+            };
+            const int rounds = min(a.top_k + 1, min(left, 32));
+            while (n < rounds) round();
+            const unsigned next = __shfl_down_sync(kAll, found, 1);
+            const bool single = lane >= n || __popc(who) == 1;  // of equal keys one is lost
+            bool apart = lane + 1 >= n;
+            if constexpr (BY_LOGIT) apart = apart || (found | kIndex) > (next | kIndex);
+            else apart = apart || value_of(found & ~kIndex) - value_of(next | kIndex) > 2.0f * off;
+            sure = __all_sync(kAll, single) && (n > a.top_k || left == a.top_k);
+            chosen = (int) (kIndex - (found & kIndex)) * 32 + __ffs(who) - 1;
+            if (sure && !__all_sync(kAll, apart)) {
+                sure = false;
+                if constexpr (!BY_LOGIT) {
+                    // All that may be among the chosen: keys down to the last one's, less both their errors.
+                    const float least = value_of(__shfl_sync(kAll, found, a.top_k - 1) & ~kIndex) - 2.0f * off;
+                    bool enough = false;
+                    while (!enough && n < min(left, 32)) enough = value_of(round() | kIndex) < least;
+                    if (__all_sync(kAll, lane >= n || __popc(who) == 1) && (enough || n == left)) {
+                        double sum = 1.0;
+                        if (softmax) {
+                            sum = 0.0;
+#pragma unroll
+                            for (int i = 0; i < EPL; i++) sum += term(a, x[i], top);
+                            sum = warp_sum_d(sum);
+                        }
+                        chosen = order_exactly(a, row, bias, top, sum, (int) (kIndex - (found & kIndex)) * 32 + __ffs(who) - 1, n);
+                        sure = true;
+                    }
+                }
             }
         }
         if (!sure) {
-            int exact;
-            if constexpr (BY_LOGIT) exact = choose_by_logit<EPL>(a, row);
-            else exact = choose_exactly<EPL>(a, row, bias, top);
-            exact = __shfl_sync(kAll, exact, lane - r * a.seats);
-            if (lane >= r * a.seats && lane < r * a.seats + a.top_k) id = exact;
+            if constexpr (BY_LOGIT) chosen = choose_by_logit<EPL>(a, row);
+            else chosen = choose_exactly<EPL>(a, row, bias, top);
         }
+        chosen = __shfl_sync(kAll, chosen, lane - r * a.seats);
         double total = 0.0;
-        if (!a.renorm && a.score == B200_ROUTER_SOFTMAX) {
+        if (!a.renorm && softmax) {
 #pragma unroll
             for (int i = 0; i < EPL; i++) total += term(a, x[i], top);
             total = warp_sum_d(total);
         }
-        if (lane >= r * a.seats) {
+        if (lane >= r * a.seats) {  // the lanes behind this row's are the next rows'
+            id = chosen;
             my_top = top;
             my_total = total;
         }
     }
 
     // ---- weights, one expert of one row per lane ----
-    const int k = lane % a.seats;
+    const int k = lane & (a.seats - 1);
     const int64_t t = t0 + lane / a.seats;
-    const bool chosen = k < a.top_k && lane / a.seats < a.rows && t < T;
-    double mine = chosen ? term(a, clean(logits[t * a.E + id]), my_top) : 0.0;
+    const bool chosen = k < a.top_k && lane < a.rows * a.seats && t < T;
+    double weight = chosen ? term(a, clean(logits[t * a.E + id]), my_top) : 0.0;
     if (a.renorm) {
-        my_total = mine;
+        my_total = weight;
         for (int o = a.seats >> 1; o > 0; o >>= 1) my_total += __shfl_xor_sync(kAll, my_total, o);
     }
-    if (a.renorm || a.score == B200_ROUTER_SOFTMAX) mine = my_total > 0.0 ? mine / my_total : 0.0;
+    if (a.renorm || softmax) weight = my_total > 0.0 ? weight / my_total : 0.0;
     if (chosen) {
         ids[t * a.top_k + k] = id;
-        w[t * a.top_k + k] = __double2float_rn(mine * (double) a.scale);
+        w[t * a.top_k + k] = __double2float_rn(weight * (double) a.scale);
     }
 }
 
@@ -375,7 +439,9 @@ extern "C" b200_status b200_moe_router(b200_context * ctx, void * stream, const 
     const bool by_logit = !bias && a.n_group == 1;
     auto go = [&](auto epl) {
         constexpr int EPL = decltype(epl)::value;
-        auto kern = by_logit ? moe_router_kernel<EPL, true> : moe_router_kernel<EPL, false>;
+        const bool full = a.E == 32 * EPL;
+        auto kern = by_logit ? (full ? moe_router_kernel<EPL, true, true> : moe_router_kernel<EPL, true, false>)
+                             : (full ? moe_router_kernel<EPL, false, true> : moe_router_kernel<EPL, false, false>);
         kern<<<grid, 32 * kWarps, smem, st>>>(a, logits, bias, T, ids, w);
     };
     const int epl = (a.E + 31) / 32;
