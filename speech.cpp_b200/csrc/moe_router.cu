@@ -27,7 +27,8 @@ struct RouterParams {
     float scale;
     // groups in the float32 pass: `lanes` lanes (a power of two, n_group * lanes <= 32) for each, the scores of a group
     // `pitch` floats apart in shared memory so that a step's lanes read different banks
-    int lanes, pitch;
+    int lanes, pitch, size, left;  // size: a group's experts; left: the experts of the groups that are kept
+    int lane_shift, seat_shift;    // logarithms of lanes and seats
     // a warp takes `rows` rows; each has `seats` lanes (a power of two, at least top_k) for its weights
     int rows, seats;
     unsigned inv;  // expert e's group is e * inv >> 21 (e < 1024)
@@ -89,7 +90,7 @@ __device__ __noinline__ int choose_exactly(const RouterParams & a, const float *
         if (c[i] != c[i]) c[i] = ninf;
     }
     if (a.n_group > 1) {
-        const int size = a.E / a.n_group;
+        const int size = a.size;
         double mine = 0.0;  // lane g: group g's score
         for (int g = 0; g < a.n_group; g++) {
             double score = 0.0;
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a,
             far = value_of(__reduce_max_sync(kAll, key_of(far)));
             off += 0x1p-23f * far;
             if (sure && a.n_group > 1) {
-                const int size = a.E / a.n_group;
+                const int size = a.size;
                 float * scores = shared + warp * a.n_group * a.pitch;
                 int of[EPL];
 #pragma unroll
@@ -290,10 +291,10 @@ __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a,
                     if (i < mine) scores[i * 32 + lane + of[i] * (a.pitch - size)] = c[i];
                 }
                 __syncwarp();
-                const int g = lane / a.lanes;
+                const int g = lane >> a.lane_shift;
                 float b1 = -INFINITY, b2 = -INFINITY;
                 if (g < a.n_group)
-                    for (int n = lane % a.lanes; n < size; n += a.lanes) merge2(b1, b2, scores[g * a.pitch + n], -INFINITY);
+                    for (int n = lane & (a.lanes - 1); n < size; n += a.lanes) merge2(b1, b2, scores[g * a.pitch + n], -INFINITY);
                 for (int o = a.lanes >> 1; o > 0; o >>= 1) {
                     const float o1 = __shfl_xor_sync(kAll, b1, o), o2 = __shfl_xor_sync(kAll, b2, o);
                     merge2(b1, b2, o1, o2);
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a,
                 __syncwarp();
                 const float score = a.group_top == 2 && size > 1 ? b1 + b2 : b1;
                 // lane n: group n's score, and how many are before it
-                const float s = __shfl_sync(kAll, score, lane < a.n_group ? lane * a.lanes : 0);
+                const float s = __shfl_sync(kAll, score, lane < a.n_group ? lane << a.lane_shift : 0);
                 int ahead = 0;
                 for (int n = 0; n < a.n_group; n++) {
                     const float other = __shfl_sync(kAll, s, n);
@@ -325,7 +326,7 @@ __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a,
             sort_keys(key);
             // Round n leaves the n-th key, and the lanes that had it, in lane n: top_k rounds and one more (if there is another
             // expert and a lane for it) to see that it lies apart.
-            const int left = a.E / a.n_group * a.topk_group;
+            const int left = a.left;
             unsigned found = 0, who = 0;
             int n = 0;
             auto round = [&] {
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a,
 
     // ---- weights, one expert of one row per lane ----
     const int k = lane & (a.seats - 1);
-    const int64_t t = t0 + lane / a.seats;
+    const int64_t t = t0 + (lane >> a.seat_shift);
     const bool chosen = k < a.top_k && lane < a.rows * a.seats && t < T;
     double weight = chosen ? term(a, clean(logits[t * a.E + id]), my_top) : 0.0;
     if (a.renorm) {
@@ -421,17 +422,27 @@ extern "C" b200_status b200_moe_router(b200_context * ctx, void * stream, const 
     if (T > (int64_t) INT32_MAX) return kv_fail(ctx, B200_ERR_INVALID, what, "more than 2^31 rows");
     DeviceScope scope(ctx->device);
     if (scope.status != cudaSuccess) return kv_cuda(ctx, scope.status, what);
-    RouterParams a{r->n_expert, r->top_k, r->score, r->n_group, r->topk_group, r->group_top, r->renorm, r->scale, 1, 0, 1, 1, 0};
+    RouterParams a = {};
+    a.E = r->n_expert;
+    a.top_k = r->top_k;
+    a.score = r->score;
+    a.n_group = r->n_group;
+    a.topk_group = r->topk_group;
+    a.group_top = r->group_top;
+    a.renorm = r->renorm;
+    a.scale = r->scale;
+    a.size = a.E / a.n_group;
+    a.left = a.size * a.topk_group;
+    a.lanes = a.rows = a.seats = 1;
     // Several rows per warp share the double arithmetic of the weights (a row has top_k of them, a warp 32 lanes), as long as
     // that leaves eight warps to each SM.
-    while (a.seats < a.top_k) a.seats *= 2;
+    while (a.seats < a.top_k) a.seats *= 2, a.seat_shift++;
     while (2 * a.rows * a.seats <= 32 && T >= (int64_t) ctx->num_sms * 8 * 2 * a.rows) a.rows *= 2;
     size_t smem = 0;
     if (a.n_group > 1) {
-        const int size = a.E / a.n_group;
-        a.inv = ((1u << 21) + size - 1) / size;  // e * (inv * size - 2^21) < 2^10 2^10, so the quotient is exact
-        while (2 * a.lanes * a.n_group <= 32) a.lanes *= 2;
-        a.pitch = size + (a.lanes - size % 32 + 32) % 32;  // pitch mod 32 = lanes: lane l of a step reads bank l + const
+        a.inv = ((1u << 21) + a.size - 1) / a.size;  // e * (inv * size - 2^21) < 2^10 2^10, so the quotient is exact
+        while (2 * a.lanes * a.n_group <= 32) a.lanes *= 2, a.lane_shift++;
+        a.pitch = a.size + (a.lanes - a.size % 32 + 32) % 32;  // pitch mod 32 = lanes: lane l of a step reads bank l + const
         smem = (size_t) kWarps * a.n_group * a.pitch * sizeof(float);  // at most 4 * (1024 + 32 * 31) * 4 B < 32 KB
     }
     cudaStream_t st = stream ? (cudaStream_t) stream : ctx->stream;
