@@ -36,7 +36,7 @@ struct RouterParams {
 
 __device__ __forceinline__ int group_of(const RouterParams & a, int e) { return (int) ((unsigned) e * a.inv >> 21); }
 
-// Unsigned order of the keys = order of the values (NaN: not allowed). 0 is below every value's key.
+// Unsigned order of the keys = order of the values (NaN: not allowed). 0 is below every value's key, and value_of(0) is NaN.
 __device__ __forceinline__ unsigned key_of(float x) {
     const unsigned u = __float_as_uint(x + 0.0f);  // -0 as 0
     return u & 0x80000000u ? ~u : u | 0x80000000u;
@@ -49,13 +49,20 @@ __device__ __forceinline__ float value_of(unsigned k) { return __uint_as_float(k
 // (a, i) before (b, j): larger first, ties to the lower index.
 __device__ __forceinline__ bool before(double a, int i, double b, int j) { return a > b || (a == b && i < j); }
 
-__device__ __forceinline__ void warp_best(double & v, int & i) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const double ov = __shfl_xor_sync(kAll, v, o);
-        const int oi = __shfl_xor_sync(kAll, i, o);
-        if (before(ov, oi, v, i)) v = ov, i = oi;
-    }
+// The same order for doubles: integer comparisons and reductions are quicker than double ones.
+__device__ __forceinline__ unsigned long long key_of(double x) {
+    const long long u = __double_as_longlong(x + 0.0);
+    return u < 0 ? ~(unsigned long long) u : (unsigned long long) u | 1ull << 63;
+}
+
+__device__ __forceinline__ double value_of(unsigned long long k) {
+    return __longlong_as_double((long long) (k >> 63 ? k & ~(1ull << 63) : ~k));
+}
+
+__device__ __forceinline__ unsigned long long warp_largest(unsigned long long k) {
+    const unsigned high = __reduce_max_sync(kAll, (unsigned) (k >> 32));
+    const unsigned low = __reduce_max_sync(kAll, (unsigned) (k >> 32) == high ? (unsigned) k : 0);
+    return (unsigned long long) high << 32 | low;
 }
 
 __device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x; }
@@ -67,73 +74,87 @@ __device__ __forceinline__ double term(const RouterParams & a, float x, float to
     return x == top ? 1.0 : exp((double) x - (double) top);
 }
 
+// The sum of a row's softmax terms. (A function of its own, as the ones below: inlined, its registers would halve the number
+// of warps that are under way.)
+__device__ __noinline__ double softmax_sum(const RouterParams & a, const float * __restrict__ logits, float top) {
+    double sum = 0.0;
+    for (int e = threadIdx.x & 31; e < a.E; e += 32) sum += term(a, clean(logits[e]), top);
+    return warp_sum_d(sum);
+}
+
 // The experts of one row: lane k gets the k-th chosen. For rows that float32 does not decide.
 template <int EPL>
 __device__ __noinline__ int choose_exactly(const RouterParams & a, const float * __restrict__ logits, const float * __restrict__ bias, float top) {
     const int lane = threadIdx.x & 31;
-    const double ninf = -INFINITY;
-    double c[EPL], sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < EPL; i++) {
-        const int e = i * 32 + lane;
-        c[i] = e < a.E ? term(a, clean(logits[e]), top) : 0.0;
-        sum += c[i];
-    }
-    sum = warp_sum_d(sum);
-    unsigned taken = 0;  // bit i: this lane's expert i is out (past the last one, in a group that is not kept, or chosen)
-#pragma unroll
-    for (int i = 0; i < EPL; i++) {
-        const int e = i * 32 + lane;
-        if (a.score == B200_ROUTER_SOFTMAX) c[i] = sum > 0.0 ? c[i] / sum : 0.0;
-        if (e >= a.E) taken |= 1u << i, c[i] = ninf;
-        else if (bias) c[i] += (double) bias[e];
-        if (c[i] != c[i]) c[i] = ninf;
-    }
-    if (a.n_group > 1) {
-        const int size = a.size;
-        double mine = 0.0;  // lane g: group g's score
-        for (int g = 0; g < a.n_group; g++) {
-            double score = 0.0;
-            int skip = -1;
-            for (int n = 0; n < (a.group_top < size ? a.group_top : size); n++) {
-                double v = ninf;
-                int at = INT32_MAX;
-#pragma unroll
-                for (int i = 0; i < EPL; i++) {
-                    const int e = i * 32 + lane;
-                    if (e < a.E && group_of(a, e) == g && e != skip && before(c[i], e, v, at)) v = c[i], at = e;
-                }
-                warp_best(v, at);
-                score += v;
-                skip = at;
-            }
-            if (lane == g) mine = score != score ? ninf : score;
-        }
-        unsigned kept = 0;
-        for (int n = 0; n < a.topk_group; n++) {
-            const bool open = lane < a.n_group && !(kept >> lane & 1);
-            double v = open ? mine : ninf;
-            int at = open ? lane : 32 + lane;
-            warp_best(v, at);
-            kept |= 1u << at;
-        }
+    unsigned long long key[EPL];  // 0: past the last expert, in a group that is not kept, or chosen
+    {
+        double c[EPL], sum = 0.0;
 #pragma unroll
         for (int i = 0; i < EPL; i++) {
             const int e = i * 32 + lane;
-            if (e < a.E && !(kept >> group_of(a, e) & 1)) taken |= 1u << i;
+            c[i] = e < a.E ? term(a, clean(logits[e]), top) : 0.0;
+            sum += c[i];
         }
+        sum = warp_sum_d(sum);
+#pragma unroll
+        for (int i = 0; i < EPL; i++) {
+            const int e = i * 32 + lane;
+            if (a.score == B200_ROUTER_SOFTMAX) c[i] = sum > 0.0 ? c[i] / sum : 0.0;
+            if (bias && e < a.E) c[i] += (double) bias[e];
+            key[i] = e < a.E ? key_of(c[i] == c[i] ? c[i] : -(double) INFINITY) : 0;
+        }
+    }
+    // the lowest expert that has `best`
+    auto holder = [&](unsigned long long best) {
+        unsigned at = kAll;
+#pragma unroll
+        for (int i = EPL - 1; i >= 0; i--)
+            if (key[i] == best) at = i * 32 + lane;
+        return (int) __reduce_min_sync(kAll, at);
+    };
+    if (a.n_group > 1) {
+        unsigned long long mine = 0;  // lane g: group g's score
+        for (int g = 0; g < a.n_group; g++) {
+            unsigned long long best = 0;
+#pragma unroll
+            for (int i = 0; i < EPL; i++)
+                if (group_of(a, i * 32 + lane) == g && key[i] > best) best = key[i];
+            best = warp_largest(best);
+            double score = value_of(best);
+            if (a.group_top == 2 && a.size > 1) {
+                unsigned at = kAll;  // the lowest expert of the group that has it is left out
+#pragma unroll
+                for (int i = EPL - 1; i >= 0; i--)
+                    if (group_of(a, i * 32 + lane) == g && key[i] == best) at = i * 32 + lane;
+                at = __reduce_min_sync(kAll, at);
+                unsigned long long second = 0;
+#pragma unroll
+                for (int i = 0; i < EPL; i++)
+                    if (group_of(a, i * 32 + lane) == g && i * 32u + lane != at && key[i] > second) second = key[i];
+                score += value_of(warp_largest(second));
+            }
+            if (lane == g) mine = key_of(score == score ? score : -(double) INFINITY);
+        }
+        unsigned kept = 0;
+        for (int n = 0; n < a.topk_group; n++) {
+            const unsigned long long best = warp_largest(mine);
+            const int g = __ffs(__ballot_sync(kAll, mine == best)) - 1;
+            kept |= 1u << g;
+            if (lane == g) mine = 0;
+        }
+#pragma unroll
+        for (int i = 0; i < EPL; i++)
+            if (!(kept >> group_of(a, i * 32 + lane) & 1)) key[i] = 0;
     }
     int id = 0;
     for (int k = 0; k < a.top_k; k++) {
-        double v = ninf;
-        int at = INT32_MAX;
+        unsigned long long best = 0;
+#pragma unroll
+        for (int i = 0; i < EPL; i++) best = key[i] > best ? key[i] : best;
+        const int at = holder(warp_largest(best));
 #pragma unroll
         for (int i = 0; i < EPL; i++)
-            if (!(taken >> i & 1) && before(c[i], i * 32 + lane, v, at)) v = c[i], at = i * 32 + lane;
-        warp_best(v, at);
-#pragma unroll
-        for (int i = 0; i < EPL; i++)
-            if (at == i * 32 + lane) taken |= 1u << i;
+            if (at == i * 32 + lane) key[i] = 0;
         if (lane == k) id = at;
     }
     return id;
@@ -280,7 +301,7 @@ __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a,
             }
             sure = __all_sync(kAll, flaw == 0.0f);
             far = value_of(__reduce_max_sync(kAll, key_of(far)));
-            off += 0x1p-23f * far;
+            off += 0x1.1p-24f * far;
             if (sure && a.n_group > 1) {
                 const int size = a.size;
                 float * scores = shared + warp * a.n_group * a.pitch;
@@ -357,13 +378,7 @@ __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a,
                     bool enough = false;
                     while (!enough && n < min(left, 32)) enough = value_of(round() | kIndex) < least;
                     if (__all_sync(kAll, lane >= n || __popc(who) == 1) && (enough || n == left)) {
-                        double sum = 1.0;
-                        if (softmax) {
-                            sum = 0.0;
-#pragma unroll
-                            for (int i = 0; i < EPL; i++) sum += term(a, x[i], top);
-                            sum = warp_sum_d(sum);
-                        }
+                        const double sum = softmax ? softmax_sum(a, row, top) : 1.0;
                         chosen = order_exactly(a, row, bias, top, sum, (int) (kIndex - (found & kIndex)) * 32 + __ffs(who) - 1, n);
                         sure = true;
                     }
@@ -375,12 +390,7 @@ __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a,
             else chosen = choose_exactly<EPL>(a, row, bias, top);
         }
         chosen = __shfl_sync(kAll, chosen, lane - r * a.seats);
-        double total = 0.0;
-        if (!a.renorm && softmax) {
-#pragma unroll
-            for (int i = 0; i < EPL; i++) total += term(a, x[i], top);
-            total = warp_sum_d(total);
-        }
+        const double total = !a.renorm && softmax ? softmax_sum(a, row, top) : 0.0;
         if (lane >= r * a.seats) {  // the lanes behind this row's are the next rows'
             id = chosen;
             my_top = top;
