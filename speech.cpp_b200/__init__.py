@@ -545,7 +545,8 @@ class Context:
         qp, ldq = self._row_arg(q, "kv_attention q", (n_seq, n_tok, n_head, cache.head_dim))
         tp, mp, lp = self._kv_places(table, lens, n_seq, "kv_attention table and lens")
         if out is None:
-            out = torch.empty(shape, dtype=torch.float32, device=q.device)
+            # empty_like takes half of empty's time; rows that lie apart (columns of a wider product) need a shape of their own
+            out = torch.empty_like(q) if ldq == n_head * cache.head_dim and q.is_contiguous() else torch.empty(shape, dtype=torch.float32, device=q.device)
             op = out.data_ptr()
         else:
             op = self._arg(out, "kv_attention out", torch.float32, shape)
@@ -573,9 +574,16 @@ class Context:
         bp = None if bias is None else self._arg(bias, "moe_router bias", torch.float32, (E,))
         r = Router(E, top_k, ROUTER_SIGMOID if score == "sigmoid" else ROUTER_SOFTMAX, n_group, topk_group, group_top, bool(renorm), scale)
         chosen = (T, top_k)
-        ids = torch.empty(chosen, dtype=torch.int32, device=logits.device) if ids is None else ids
-        w = torch.empty(chosen, dtype=torch.float32, device=logits.device) if w is None else w
-        ip, wp = self._arg(ids, "moe_router ids", torch.int32, chosen), self._arg(w, "moe_router w", torch.float32, chosen)
+        if ids is None:
+            ids = torch.empty_strided(chosen, (top_k, 1), dtype=torch.int32, device=logits.device)
+            ip = ids.data_ptr()
+        else:
+            ip = self._arg(ids, "moe_router ids", torch.int32, chosen)
+        if w is None:
+            w = torch.empty_strided(chosen, (top_k, 1), dtype=torch.float32, device=logits.device)
+            wp = w.data_ptr()
+        else:
+            wp = self._arg(w, "moe_router w", torch.float32, chosen)
         self.check(self.L.b200_moe_router(self.h, self._stream(), ctypes.byref(r), lp, bp, T, ip, wp))
         return ids, w
 

@@ -39,20 +39,20 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kJoinWarps = 8;
-constexpr int kRows = 8;      // rows of a tile
 constexpr int kChunk = 64;    // positions of a chunk: one 16-position tile per warp
 constexpr int kItemChunks = 8;  // chunks per CTA up to which the work is cut by items
 constexpr float kShift = 14;  // weights are held times 2^14, so that their low halves reach 2^-38 of the largest
 
 struct Geometry {
-    int n_tok, n_head, group, tiles;  // tiles: row tiles of a key/value head
+    int n_tok, n_head, group;
+    int rows, tiles;                  // rows of an item; items of a key/value head
     int64_t items;                    // n_kv_head * tiles, per sequence
     int64_t n_seq;
     int64_t ctas;                     // CTAs among which the chunks are divided, or
     int cluster;                      // CTAs that share an item (0: the work is cut by positions)
 };
 
-constexpr int64_t partial_floats(int D) { return (int64_t) kRows * (D + 2); }  // o [kRows][D], m [kRows], l [kRows]
+constexpr int64_t partial_floats(int D, int rows) { return (int64_t) rows * (D + 2); }  // o [rows][D], m [rows], l [rows]
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -126,8 +126,10 @@ __device__ __forceinline__ float half_of(const uint32_t * w, int i) {
 
 // How a head's rows are taken apart. The n index of O = P V runs through the dimensions in groups of 8 kRun, lane quad g
 // holding kRun contiguous ones of each.
-template <bool Q8, int D>
+template <bool Q8, int D, int TILES>
 struct Shape {
+    static constexpr bool kQ8 = Q8;
+    static constexpr int kDim = D, kTiles = TILES, kRows = 8 * TILES;  // kRows: rows of an item
     static constexpr int kBlocks = D / 32;
     static constexpr int kRun = !Q8 && D % 64 == 0 ? 8 : 4;
     static constexpr int kGroups = D / (8 * kRun);
@@ -139,8 +141,8 @@ struct Shape {
     static constexpr int kRowBytes = Q8 ? D : 2 * D;
     static constexpr int kScaleBytes = Q8 ? D / 16 : 0;    // of a row
     static constexpr int kPiece = 32 * (kRowBytes + kScaleBytes);
-    static constexpr int kStages = Q8 ? (D == 128 ? 2 : 3) : (D == 64 ? 4 : D == 256 ? 2 : 3);
-    static constexpr int kCtas = Q8 ? (D == 64 || D == 128 ? 3 : 2) : (D == 256 ? 1 : D == 128 ? 2 : 3);
+    static constexpr int kStages = Q8 ? (D == 128 && TILES == 1 ? 2 : 3) : (D == 64 ? 4 : D == 256 ? 2 : 3);
+    static constexpr int kCtas = Q8 ? (TILES == 1 && (D == 64 || D == 128) ? 3 : 2) : (D == 256 ? 1 : D == 128 || TILES == 2 ? 2 : 3);
     static_assert(D == 96 || kPiece % 128 == 0, "swizzled pieces keep the ring's alignment");
     static constexpr int kStage = kSub * kPiece, kBytes = kWarps * kStages * kStage;
     // The 16-byte chunks of a row are stored at chunk ^ swizzle(row), so that the lanes that read together read different
@@ -219,47 +221,53 @@ __device__ __forceinline__ void find_sequence(const KvView & c, const Geometry &
     start = red[kWarps + 1];
 }
 
-// Rows of a tile: row i is query head h * group + (tile * 8 + i) % group of token (tile * 8 + i) / group.
+// Rows of an item: row i is query head h * group + n % group of token n / group, n = tile * rows + i.
 struct Row {
     int token, head;
     bool there;
 };
 
+template <int ROWS>
 __device__ __forceinline__ Row row_of(const Geometry & g, int h, int tile, int i) {
-    const int n = tile * kRows + i;
+    const int n = tile * ROWS + i;
     return {n / g.group, h * g.group + n % g.group, n < g.n_tok * g.group};
 }
 
 // A CTA's shared memory: the warps' rings of pieces, and, at the ring's place once a run is done, each warp's o.
-template <bool Q8, int D>
+template <class S>
 struct Shared {
     uint8_t * ring;  // dynamic: [kWarps][kStages][kSub][kPiece]
-    float (*sm)[kRows];
-    float (*sl)[kRows];
-    static constexpr int kRingBytes = Shape<Q8, D>::kStages * Shape<Q8, D>::kStage;
-    static constexpr int kPitch = D + 4;
-    static_assert(kRows * kPitch * 4 <= kRingBytes, "a warp's o fits its ring");
+    float (*sm)[S::kRows];
+    float (*sl)[S::kRows];
+    static constexpr int kRingBytes = S::kStages * S::kStage;
+    static constexpr int kPitch = S::kDim + 4;
+    static_assert(S::kRows * kPitch * 4 <= kRingBytes, "a warp's o fits its ring");
     __device__ __forceinline__ float & o(int w, int row, int d) const {
         return reinterpret_cast<float *>(ring + w * kRingBytes)[row * kPitch + d];
     }
 };
 
 // Chunks [c0, c1) of one item: the warps' m, l and o are left in shared memory (synchronised).
-template <bool Q8, int D>
+template <class S>
 __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, const float * __restrict__ q, int64_t ldq, float scale,
-                                       const Shared<Q8, D> & sh, int64_t seq, int64_t len, int h, int tile, int64_t c0, int64_t c1) {
-    using S = Shape<Q8, D>;
+                                       const Shared<S> & sh, int64_t seq, int64_t len, int h, int tile, int64_t c0, int64_t c1) {
+    constexpr bool Q8 = S::kQ8;
+    constexpr int D = S::kDim, TILES = S::kTiles;
     constexpr int kRowBytes = S::kRowBytes, kValues = 16 * kRowBytes, kKeyScales = 32 * kRowBytes, kValueScales = kKeyScales + 16 * S::kScaleBytes;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int gq = lane >> 2, t = lane & 3;  // the fragment's group and thread in it
-    const Row row = row_of(g, h, tile, gq);
+    Row row[TILES];
+#pragma unroll
+    for (int y = 0; y < TILES; y++) row[y] = row_of<S::kRows>(g, h, tile, 8 * y + gq);
     const int p_end = (int) (c1 * kChunk < len ? c1 * kChunk : len);
     const int all_see = (int) len - g.n_tok + 1;  // positions below are seen by every row
-    const int seen = row.there ? all_see + row.token : 0;
+    int seen[TILES];
+#pragma unroll
+    for (int y = 0; y < TILES; y++) seen[y] = row[y].there ? all_see + row[y].token : 0;
 
     // ---- the ring: steps of kSub pieces, the warps in turn through [c0 * 64, c1 * 64), copied kStages - 1 ahead ----
     constexpr int kSub = S::kSub, kStep = kWarps * 16 * kSub;
-    const uint32_t ring = smem_addr(sh.ring) + warp * Shared<Q8, D>::kRingBytes;
+    const uint32_t ring = smem_addr(sh.ring) + warp * Shared<S>::kRingBytes;
     const int64_t page_bytes = (int64_t) c.n_kv_head * c.page_size * kRowBytes;
     const uint8_t * kh = c.k + (int64_t) h * c.page_size * kRowBytes + lane * 16;
     const int64_t to_values = c.v - c.k;
@@ -337,15 +345,16 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
     // 1 and 3. The row is scaled by 2^k to a largest magnitude in [2^14, 2^15).
     // Q8_0: key bytes enter as q + 128 in the low byte of an F16, which is (q + 128) 2^-24 (a subnormal, and exact); `bias` is
     // what the 128 adds to a block's sum.
-    uint32_t qf[D / 16][4];
-    float bias[Q8 ? S::kBlocks : 1];
-    float factor;  // what a raw score is multiplied by: scale log2(e) 2^-k
-    {
-        const float * src = q + (seq * g.n_tok + row.token) * ldq + (int64_t) row.head * D + 8 * t;
+    uint32_t qf[TILES][D / 16][4];
+    float bias[TILES][Q8 ? S::kBlocks : 1];
+    float factor[TILES];  // what a raw score is multiplied by: scale log2(e) 2^-k
+#pragma unroll
+    for (int y = 0; y < TILES; y++) {
+        const float * src = q + (seq * g.n_tok + row[y].token) * ldq + (int64_t) row[y].head * D + 8 * t;
         float x[D / 4], top = 0.0f;
 #pragma unroll
         for (int i = 0; i < D / 4; i++) {
-            x[i] = row.there ? src[(i / 8) * 32 + i % 8] : 0.0f;
+            x[i] = row[y].there ? src[(i / 8) * 32 + i % 8] : 0.0f;
             top = fmaxf(top, fabsf(x[i]));
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -353,14 +362,14 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
         const int e = (int) (__float_as_uint(top) >> 23);
         const int k = e == 255 || top == 0.0f ? 0 : 141 - e < 126 ? 141 - e : 126;
         const float up = __uint_as_float((uint32_t) (k + 127) << 23);
-        factor = scale * 1.4426950408889634f * __uint_as_float((uint32_t) (127 - k) << 23);
+        factor[y] = scale * 1.4426950408889634f * __uint_as_float((uint32_t) (127 - k) << 23);
 #pragma unroll
         for (int j = 0; j < D / 16; j++) {
-            split(x[4 * j] * up, x[4 * j + 1] * up, qf[j][0], qf[j][1]);
-            split(x[4 * j + 2] * up, x[4 * j + 3] * up, qf[j][2], qf[j][3]);
+            split(x[4 * j] * up, x[4 * j + 1] * up, qf[y][j][0], qf[y][j][1]);
+            split(x[4 * j + 2] * up, x[4 * j + 3] * up, qf[y][j][2], qf[y][j][3]);
         }
         if constexpr (Q8) {
-            factor *= 0x1p24f;
+            factor[y] *= 0x1p24f;
 #pragma unroll
             for (int b = 0; b < S::kBlocks; b++) {
                 float sum = 0.0f;
@@ -368,7 +377,7 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                 for (int i = 0; i < 8; i++) sum = fmaf(x[8 * b + i], up, sum);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                bias[b] = sum * -0x1p-17f;
+                bias[y][b] = sum * -0x1p-17f;
             }
         }
     }
@@ -378,8 +387,10 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
     const uint32_t key_at = gq * kRowBytes + ((t * (Q8 ? 8 : 16)) ^ (S::key_swizzle(gq) * 16));
     const uint32_t value_at = kValues + 2 * t * kRowBytes + ((gq * S::kRun * (Q8 ? 1 : 2)) ^ (S::value_swizzle(2 * t) * 16));
 
-    float2 o[S::kGroups][S::kRun] = {};
-    float m = -INFINITY, l = 0.0f;
+    float2 o[TILES][S::kGroups][S::kRun] = {};
+    float m[TILES], l[TILES];
+#pragma unroll
+    for (int y = 0; y < TILES; y++) m[y] = -INFINITY, l[y] = 0.0f;
     int stage = 0;
     for (int p0 = (int) c0 * kChunk + warp * 16 * kSub; p0 < p_end; p0 += kStep) {
         asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
@@ -395,8 +406,8 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
         stage = stage + 1 == S::kStages ? 0 : stage + 1;
         copy_step();
 
-        // ---- scores: s[u][2 i + j] is position 16 u + 2 t + j + 8 i of row gq ----
-        float s[kSub][4];
+        // ---- scores: s[y][u][2 i + j] is position 16 u + 2 t + j + 8 i of row 8 y + gq ----
+        float s[TILES][kSub][4];
 #pragma unroll
         for (int u = 0; u < kSub; u++) {
             const uint32_t keys = at + u * S::kPiece + key_at;
@@ -405,8 +416,8 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
 #pragma unroll
                 for (int i = 0; i < 2; i++) lds(kd[i], at + u * S::kPiece + kKeyScales + (2 * t + 8 * i) * S::kScaleBytes);
             }
-            float sum[2][4] = {};
-            float2 part[2] = {};
+            float sum[TILES][2][4] = {};
+            float2 part[TILES][2] = {};
 #pragma unroll
             for (int b = 0; b < S::kBlocks; b++)
 #pragma unroll
@@ -414,57 +425,75 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                     uint32_t w[S::kKeyWords];
                     lds(w, S::along(keys, b * (Q8 ? 32 : 64)) + i * 8 * kRowBytes);
                     if constexpr (Q8) {
-                        float r[4];
                         const uint32_t w0 = w[0] ^ 0x80808080u, w1 = w[1] ^ 0x80808080u;
-                        mma(r, qf[2 * b], __byte_perm(w0, 0, 0x4140), __byte_perm(w0, 0, 0x4342));
-                        mma(r, qf[2 * b + 1], __byte_perm(w1, 0, 0x4140), __byte_perm(w1, 0, 0x4342), r);
-                        const float2 whole = __fadd2_rn(make_float2(r[0], r[1]), __fadd2_rn(make_float2(r[2], r[3]), make_float2(bias[b], bias[b])));
-                        part[i] = __ffma2_rn(make_float2(half_of(kd[i], b), half_of(kd[i], S::kBlocks + b)), whole, part[i]);
+                        const uint32_t f[4] = {__byte_perm(w0, 0, 0x4140), __byte_perm(w0, 0, 0x4342), __byte_perm(w1, 0, 0x4140), __byte_perm(w1, 0, 0x4342)};
+                        const float2 d = make_float2(half_of(kd[i], b), half_of(kd[i], S::kBlocks + b));
+#pragma unroll
+                        for (int y = 0; y < TILES; y++) {
+                            float r[4];
+                            mma(r, qf[y][2 * b], f[0], f[1]);
+                            mma(r, qf[y][2 * b + 1], f[2], f[3], r);
+                            const float2 whole =
+                                __fadd2_rn(make_float2(r[0], r[1]), __fadd2_rn(make_float2(r[2], r[3]), make_float2(bias[y][b], bias[y][b])));
+                            part[y][i] = __ffma2_rn(d, whole, part[y][i]);
+                        }
                     } else {
-                        mma(sum[i], qf[2 * b], w[0], w[1], sum[i]);
-                        mma(sum[i], qf[2 * b + 1], w[2], w[3], sum[i]);
+#pragma unroll
+                        for (int y = 0; y < TILES; y++) {
+                            mma(sum[y][i], qf[y][2 * b], w[0], w[1], sum[y][i]);
+                            mma(sum[y][i], qf[y][2 * b + 1], w[2], w[3], sum[y][i]);
+                        }
                     }
                 }
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                if constexpr (!Q8) part[i] = __fadd2_rn(make_float2(sum[i][0], sum[i][1]), make_float2(sum[i][2], sum[i][3]));
-                s[u][2 * i] = part[i].x * factor;
-                s[u][2 * i + 1] = part[i].y * factor;
-            }
+            for (int y = 0; y < TILES; y++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    if constexpr (!Q8)
+                        part[y][i] = __fadd2_rn(make_float2(sum[y][i][0], sum[y][i][1]), make_float2(sum[y][i][2], sum[y][i][3]));
+                    s[y][u][2 * i] = part[y][i].x * factor[y];
+                    s[y][u][2 * i + 1] = part[y][i].y * factor[y];
+                }
         }
         if (edge) {
 #pragma unroll
-            for (int u = 0; u < kSub; u++)
+            for (int y = 0; y < TILES; y++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int j = 2 * t + (i & 1) + 8 * (i >> 1);
-                    if (j >= here[u] || p0 + 16 * u + j >= seen) s[u][i] = -INFINITY;
-                }
+                for (int u = 0; u < kSub; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int j = 2 * t + (i & 1) + 8 * (i >> 1);
+                        if (j >= here[u] || p0 + 16 * u + j >= seen[y]) s[y][u][i] = -INFINITY;
+                    }
         }
 
         // ---- weights: m is the running maximum less kShift (-infinity before any score) ----
-        float top = -INFINITY;
+        float2 keep[TILES];
+        uint32_t pf[TILES][kSub][4];  // the weights' fragments: hi, lo of positions 2 t, 2 t + 1, then of 2 t + 8, 2 t + 9
 #pragma unroll
-        for (int u = 0; u < kSub; u++) top = fmaxf(top, fmaxf(fmaxf(s[u][0], s[u][1]), fmaxf(s[u][2], s[u][3])));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float m_new = fmaxf(m, top - kShift);
-        const float base = m_new == -INFINITY ? 0.0f : m_new;
-        const float keep = ex2(m - base);
-        m = m_new;
-        l *= keep;
-        uint32_t pf[kSub][4];  // the weights' fragments: hi, lo of positions 2 t, 2 t + 1, then of 2 t + 8, 2 t + 9
+        for (int y = 0; y < TILES; y++) {
+            float top = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < kSub; u++) {
+            for (int u = 0; u < kSub; u++) top = fmaxf(top, fmaxf(fmaxf(s[y][u][0], s[y][u][1]), fmaxf(s[y][u][2], s[y][u][3])));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float m_new = fmaxf(m[y], top - kShift);
+            const float base = m_new == -INFINITY ? 0.0f : m_new;
+            const float k = ex2(m[y] - base);
+            keep[y] = make_float2(k, k);
+            m[y] = m_new;
+            l[y] *= k;
 #pragma unroll
-            for (int i = 0; i < 4; i++) s[u][i] = ex2(s[u][i] - base);
-            l += (s[u][0] + s[u][1]) + (s[u][2] + s[u][3]);
-            split(s[u][0], s[u][1], pf[u][0], pf[u][1]);
-            split(s[u][2], s[u][3], pf[u][2], pf[u][3]);
+            for (int u = 0; u < kSub; u++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[y][u][i] = ex2(s[y][u][i] - base);
+                l[y] += (s[y][u][0] + s[y][u][1]) + (s[y][u][2] + s[y][u][3]);
+                split(s[y][u][0], s[y][u][1], pf[y][u][0], pf[y][u][1]);
+                split(s[y][u][2], s[y][u][3], pf[y][u][2], pf[y][u][3]);
+            }
         }
 
         // ---- o = o keep + P V: values of rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9, the positions whose weights this lane holds ----
-        const float2 keep2 = make_float2(keep, keep);
         using Words = uint32_t[4][S::kValueWords];
         auto values = [&](Words & w, int u, int n) {
             const uint32_t first = at + u * S::kPiece + value_at;
@@ -491,7 +520,7 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                         }
                     }
             }
-            using Fragments = uint32_t[S::kSub][4];
+            using Fragments = uint32_t[S::kTiles][S::kSub][4];
             // one block of 32 dimensions: weights times scales (fragments a), times 2^k and back where `down` is not 1
             auto block = [&](int b, const Fragments & a, auto scaled, float down) {
                 uint32_t x[S::kSub][2][2];  // two rows' four bytes each, interleaved: (row, row + 1) pairs
@@ -507,14 +536,20 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                 }
 #pragma unroll
                 for (int n = 0; n < 4; n++) {
-                    float r[4];
                     const uint32_t sel = n & 1 ? 0x4342 : 0x4140;
-                    mma(r, a[0], halves(x[0][0][n / 2], sel), halves(x[0][1][n / 2], sel));
+                    uint32_t f[S::kSub][2];
 #pragma unroll
-                    for (int u = 1; u < kSub; u++) mma(r, a[u], halves(x[u][0][n / 2], sel), halves(x[u][1][n / 2], sel), r);
-                    float2 part = __fadd2_rn(make_float2(r[0], r[1]), make_float2(r[2], r[3]));
-                    if constexpr (decltype(scaled)::value) part.x *= down, part.y *= down;
-                    o[b][n] = __ffma2_rn(o[b][n], keep2, part);
+                    for (int u = 0; u < kSub; u++) f[u][0] = halves(x[u][0][n / 2], sel), f[u][1] = halves(x[u][1][n / 2], sel);
+#pragma unroll
+                    for (int y = 0; y < TILES; y++) {
+                        float r[4];
+                        mma(r, a[y][0], f[0][0], f[0][1]);
+#pragma unroll
+                        for (int u = 1; u < kSub; u++) mma(r, a[y][u], f[u][0], f[u][1], r);
+                        float2 part = __fadd2_rn(make_float2(r[0], r[1]), make_float2(r[2], r[3]));
+                        if constexpr (decltype(scaled)::value) part.x *= down, part.y *= down;
+                        o[y][b][n] = __ffma2_rn(o[y][b][n], keep[y], part);
+                    }
                 }
             };
             // Scales between 2^-14 and 2 (nearly always all of them) multiply the weights' halves in F16 pairs: the
@@ -537,9 +572,13 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                         for (int u = 0; u < kSub; u++)
 #pragma unroll
                             for (int i = 0; i < 2; i++) {
-                                const __half2 d = h2(pair_of<b, S::kBlocks + b>(vd[u][i])), hi = h2(pf[u][2 * i]), w = __hmul2_rn(hi, d);
-                                a[u][2 * i] = u32(w);
-                                a[u][2 * i + 1] = u32(__hfma2(h2(pf[u][2 * i + 1]), d, __hfma2(hi, d, __hneg2(w))));
+                                const __half2 d = h2(pair_of<b, S::kBlocks + b>(vd[u][i]));
+#pragma unroll
+                                for (int y = 0; y < TILES; y++) {
+                                    const __half2 hi = h2(pf[y][u][2 * i]), w = __hmul2_rn(hi, d);
+                                    a[y][u][2 * i] = u32(w);
+                                    a[y][u][2 * i + 1] = u32(__hfma2(h2(pf[y][u][2 * i + 1]), d, __hfma2(hi, d, __hneg2(w))));
+                                }
                             }
                         block(b, a, std::false_type{}, 1.0f);
                     }
@@ -566,20 +605,22 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                     const float up = __uint_as_float((uint32_t) (253 - e) << 23), down = __uint_as_float((uint32_t) (e + 1) << 23);
                     Fragments a;
 #pragma unroll
-                    for (int u = 0; u < kSub; u++) {
-                        float w[4];
+                    for (int y = 0; y < TILES; y++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) w[i] = edge && s[u][i] == 0.0f ? 0.0f : s[u][i] * (d[u][i] * up);
-                        split(w[0], w[1], a[u][0], a[u][1]);
-                        split(w[2], w[3], a[u][2], a[u][3]);
-                    }
+                        for (int u = 0; u < kSub; u++) {
+                            float w[4];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) w[i] = edge && s[y][u][i] == 0.0f ? 0.0f : s[y][u][i] * (d[u][i] * up);
+                            split(w[0], w[1], a[y][u][0], a[y][u][1]);
+                            split(w[2], w[3], a[y][u][2], a[y][u][3]);
+                        }
                     block(b, a, std::true_type{}, down);
                 }
             }
         } else {
             static_assert(Q8 || kSub == 1, "an F16 step is one piece");
             // `below`: rows from this place in the piece on enter as zeros
-            auto product = [&](int below, bool mine) {
+            auto product = [&](int below, int token) {  // token: only its rows' results count (-1: every row's)
 #pragma unroll
                 for (int n = 0; n < S::kGroups; n++) {
                     Words w;
@@ -593,20 +634,25 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                     }
 #pragma unroll
                     for (int r = 0; r < S::kRun; r++) {
-                        float part[4];
                         const uint32_t sel = r & 1 ? 0x7632 : 0x5410;
-                        mma(part, pf[0], __byte_perm(w[0][r / 2], w[1][r / 2], sel), __byte_perm(w[2][r / 2], w[3][r / 2], sel));
-                        if (mine) o[n][r] = __ffma2_rn(o[n][r], keep2, __fadd2_rn(make_float2(part[0], part[1]), make_float2(part[2], part[3])));
+                        const uint32_t f0 = __byte_perm(w[0][r / 2], w[1][r / 2], sel), f1 = __byte_perm(w[2][r / 2], w[3][r / 2], sel);
+#pragma unroll
+                        for (int y = 0; y < TILES; y++) {
+                            float part[4];
+                            mma(part, pf[y][0], f0, f1);
+                            if (token < 0 || row[y].token == token)
+                                o[y][n][r] = __ffma2_rn(o[y][n][r], keep[y], __fadd2_rn(make_float2(part[0], part[1]), make_float2(part[2], part[3])));
+                        }
                     }
                 }
             };
             if (edge && g.n_tok > 1) {
                 // Where rows see different positions, a value that is NaN or infinite must not meet the weight 0 of a row
                 // that does not see it: one product per token, with the values behind its position zeroed.
-                const int last = min((tile * kRows + kRows - 1) / g.group, g.n_tok - 1);
-                for (int token = tile * kRows / g.group; token <= last; token++) product(all_see + token - p0, row.token == token);
+                const int last = min((tile * S::kRows + S::kRows - 1) / g.group, g.n_tok - 1);
+                for (int token = tile * S::kRows / g.group; token <= last; token++) product(all_see + token - p0, token);
             } else {
-                product(16, true);
+                product(16, -1);
             }
         }
     }
@@ -614,27 +660,30 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
     // ---- join the warps ----
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();  // the ring is read no more: o takes its place
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (t == 0) {
-        sh.sm[warp][gq] = m;
-        sh.sl[warp][gq] = l;
-    }
 #pragma unroll
-    for (int n = 0; n < S::kGroups; n++)
-#pragma unroll
-        for (int r = 0; r < S::kRun; r++) {
-            sh.o(warp, gq, n * 8 * S::kRun + 2 * t * S::kRun + r) = o[n][r].x;
-            sh.o(warp, gq, n * 8 * S::kRun + (2 * t + 1) * S::kRun + r) = o[n][r].y;
+    for (int y = 0; y < TILES; y++) {
+        l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
+        l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
+        if (t == 0) {
+            sh.sm[warp][8 * y + gq] = m[y];
+            sh.sl[warp][8 * y + gq] = l[y];
         }
+#pragma unroll
+        for (int n = 0; n < S::kGroups; n++)
+#pragma unroll
+            for (int r = 0; r < S::kRun; r++) {
+                sh.o(warp, 8 * y + gq, n * 8 * S::kRun + 2 * t * S::kRun + r) = o[y][n][r].x;
+                sh.o(warp, 8 * y + gq, n * 8 * S::kRun + (2 * t + 1) * S::kRun + r) = o[y][n][r].y;
+            }
+    }
     __syncthreads();
 }
 
 // The CTA's sum of the warps' results for one row: the factors of the warps, and m and l.
-template <bool Q8, int D>
+template <class S>
 struct Joined {
     float f[kWarps], m, l;
-    __device__ __forceinline__ Joined(const Shared<Q8, D> & sh, int i) {
+    __device__ __forceinline__ Joined(const Shared<S> & sh, int i) {
         m = -INFINITY;
         l = 0.0f;
 #pragma unroll
@@ -646,7 +695,7 @@ struct Joined {
             l = fmaf(sh.sl[w][i], f[w], l);
         }
     }
-    __device__ __forceinline__ float value(const Shared<Q8, D> & sh, int i, int d) const {
+    __device__ __forceinline__ float value(const Shared<S> & sh, int i, int d) const {
         float v = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWarps; w++) v = fmaf(sh.o(w, i, d), f[w], v);
@@ -655,13 +704,14 @@ struct Joined {
 };
 
 // The work cut by positions: CTA b takes chunks [b share, (b + 1) share) of all items' chunks.
-template <bool Q8, int D>
-__global__ void __launch_bounds__(kThreads, Shape<Q8, D>::kCtas)
+template <class S>
+__global__ void __launch_bounds__(kThreads, S::kCtas)
     kv_attention_kernel(KvView c, Geometry g, const float * __restrict__ q, int64_t ldq, float scale, float * __restrict__ out, float * __restrict__ ws) {
+    constexpr int D = S::kDim, kRows = S::kRows;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
-    const Shared<Q8, D> sh{ring, sm, sl};
     __shared__ int64_t red[kWarps + 2];
+    const Shared<S> sh{ring, sm, sl};
     const int tid = threadIdx.x;
     pdl_launch_dependents();
 
@@ -685,21 +735,22 @@ __global__ void __launch_bounds__(kThreads, Shape<Q8, D>::kCtas)
         const int64_t c1 = c0 + (end - at) < chunks ? c0 + (end - at) : chunks;
         at += c1 - c0;
         const int h = (int) (item / g.tiles), tile = (int) (item % g.tiles);
-        attend<Q8, D>(c, g, q, ldq, scale, sh, seq, len, h, tile, c0, c1);
+        attend<S>(c, g, q, ldq, scale, sh, seq, len, h, tile, c0, c1);
 
-        const int i = tid / 16;  // a row per 16 threads
-        const Joined<Q8, D> all(sh, i);
-        const Row row = row_of(g, h, tile, i);
-        if (c0 == 0 && c1 == chunks) {  // the whole item
-            const float inv = all.l != 0.0f ? 1.0f / all.l : 0.0f;
-            if (row.there)
-                for (int d = tid & 15; d < D; d += 16) out[((seq * g.n_tok + row.token) * g.n_head + row.head) * D + d] = all.value(sh, i, d) * inv;
-        } else {  // the CTA's first partial (of an item begun before it) or its last
-            float * to = ws + (2 * blockIdx.x + (c0 == 0 ? 1 : 0)) * partial_floats(D);
-            for (int d = tid & 15; d < D; d += 16) to[i * D + d] = all.value(sh, i, d);
-            if ((tid & 15) == 0) {
-                to[kRows * D + i] = all.m;
-                to[kRows * D + kRows + i] = all.l;
+        for (int i = tid / 16; i < kRows; i += kThreads / 16) {  // a row per 16 threads
+            const Joined<S> all(sh, i);
+            const Row row = row_of<kRows>(g, h, tile, i);
+            if (c0 == 0 && c1 == chunks) {  // the whole item
+                const float inv = all.l != 0.0f ? 1.0f / all.l : 0.0f;
+                if (row.there)
+                    for (int d = tid & 15; d < D; d += 16) out[((seq * g.n_tok + row.token) * g.n_head + row.head) * D + d] = all.value(sh, i, d) * inv;
+            } else {  // the CTA's first partial (of an item begun before it) or its last
+                float * to = ws + (2 * blockIdx.x + (c0 == 0 ? 1 : 0)) * partial_floats(D, kRows);
+                for (int d = tid & 15; d < D; d += 16) to[i * D + d] = all.value(sh, i, d);
+                if ((tid & 15) == 0) {
+                    to[kRows * D + i] = all.m;
+                    to[kRows * D + kRows + i] = all.l;
+                }
             }
         }
         __syncthreads();  // the shared memory is written again by the next run
@@ -708,22 +759,22 @@ __global__ void __launch_bounds__(kThreads, Shape<Q8, D>::kCtas)
 
 // The work cut by items: a cluster of `cluster` CTAs per item, each an equal run of its chunks, joined over distributed
 // shared memory: the CTA of rank r writes rows r, r + cluster, ... One launch, and no length but the item's own is read.
-template <bool Q8, int D>
-__global__ void __launch_bounds__(kThreads, Shape<Q8, D>::kCtas)
+template <class S>
+__global__ void __launch_bounds__(kThreads, S::kCtas)
     kv_attention_item_kernel(KvView c, Geometry g, int cluster, const float * __restrict__ q, int64_t ldq, float scale, float * __restrict__ out) {
+    constexpr int D = S::kDim, kRows = S::kRows;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
-    const Shared<Q8, D> sh{ring, sm, sl};
     __shared__ float jm[kRows], jl[kRows];
+    const Shared<S> sh{ring, sm, sl};
     const int tid = threadIdx.x, rank = blockIdx.x % cluster;
     const int64_t unit = blockIdx.x / cluster, seq = unit / g.items;
     const int item = (int) (unit % g.items), h = item / g.tiles, tile = item % g.tiles;
     const int64_t len = kv_len(c, seq, tid == 0), chunks = (len + kChunk - 1) / kChunk, per = (chunks + cluster - 1) / cluster;
     const int64_t c0 = rank * per < chunks ? rank * per : chunks, c1 = c0 + per < chunks ? c0 + per : chunks;
-    attend<Q8, D>(c, g, q, ldq, scale, sh, seq, len, h, tile, c0, c1);
-    {
-        const int i = tid / 16;
-        const Joined<Q8, D> all(sh, i);
+    attend<S>(c, g, q, ldq, scale, sh, seq, len, h, tile, c0, c1);
+    for (int i = tid / 16; i < kRows; i += kThreads / 16) {
+        const Joined<S> all(sh, i);
         for (int d = tid & 15; d < D; d += 16) sh.o(0, i, d) = all.value(sh, i, d);  // read and written by this thread alone
         if ((tid & 15) == 0) jm[i] = all.m, jl[i] = all.l;
     }
@@ -731,7 +782,7 @@ __global__ void __launch_bounds__(kThreads, Shape<Q8, D>::kCtas)
     group.sync();
     for (int e = tid; e < kRows / cluster * D; e += kThreads) {
         const int i = e / D * cluster + rank, d = e % D;
-        const Row row = row_of(g, h, tile, i);
+        const Row row = row_of<kRows>(g, h, tile, i);
         if (!row.there) continue;
         float m = -INFINITY, l = 0.0f, v = 0.0f;
         for (int r = 0; r < cluster; r++) m = fmaxf(m, *group.map_shared_rank(&jm[i], r));
@@ -748,13 +799,13 @@ __global__ void __launch_bounds__(kThreads, Shape<Q8, D>::kCtas)
 
 // Joins the partials of items that several CTAs worked on, and writes the zeros of empty sequences. One CTA per row of an
 // item: a warp takes every kJoinWarps-th partial, a lane D / 32 dimensions, and the warps join in shared memory.
-template <int D>
+template <int D, int ROWS>
 __global__ void __launch_bounds__(32 * kJoinWarps) kv_attention_join_kernel(KvView c, Geometry g, float * __restrict__ out, const float * __restrict__ ws) {
     __shared__ int64_t red[2 * kJoinWarps];
     __shared__ float so[kJoinWarps][D], sm[kJoinWarps], sl[kJoinWarps];
-    const int i = blockIdx.x % kRows, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t seq = blockIdx.x / kRows / g.items, item = blockIdx.x / kRows % g.items;
-    const Row mine = row_of(g, (int) (item / g.tiles), (int) (item % g.tiles), i);
+    const int i = blockIdx.x % ROWS, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t seq = blockIdx.x / ROWS / g.items, item = blockIdx.x / ROWS % g.items;
+    const Row mine = row_of<ROWS>(g, (int) (item / g.tiles), (int) (item % g.tiles), i);
     if (!mine.there) return;
     int64_t sums[2] = {0, 0};  // the chunks of an item in all sequences, and in those before this one
     for (int64_t s = tid; s < g.n_seq; s += 32 * kJoinWarps) {
@@ -794,9 +845,9 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv_attention_join_kernel(KvVi
 #pragma unroll
         for (int n = 0; n < kStep; n++) {
             const int k = k0 + n * kJoinWarps;
-            const float * src = ws + (2 * k + (k == first ? 1 : 0)) * partial_floats(D);
-            pm[n] = k <= last ? src[kRows * D + i] : -INFINITY;
-            pl[n] = k <= last ? src[kRows * D + kRows + i] : 0.0f;
+            const float * src = ws + (2 * k + (k == first ? 1 : 0)) * partial_floats(D, ROWS);
+            pm[n] = k <= last ? src[ROWS * D + i] : -INFINITY;
+            pl[n] = k <= last ? src[ROWS * D + ROWS + i] : 0.0f;
 #pragma unroll
             for (int d = 0; d < D / 32; d++) po[n][d] = k <= last ? src[i * D + lane + 32 * d] : 0.0f;
         }
@@ -842,15 +893,22 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv_attention_join_kernel(KvVi
     }
 }
 
-// Calls f with the Shape of a cache's type and head_dim.
+// Calls f with the Shape for a cache's type and head_dim and a key/value head's rows: sixteen rows at a time where there are
+// more than eight and the registers hold them (each key and value is then read and converted once for all sixteen).
 template <class F>
-void with_shape(bool q8, int D, F f) {
-    switch (D) {
-    case 64: q8 ? f(Shape<true, 64>{}) : f(Shape<false, 64>{}); break;
-    case 96: q8 ? f(Shape<true, 96>{}) : f(Shape<false, 96>{}); break;
-    case 128: q8 ? f(Shape<true, 128>{}) : f(Shape<false, 128>{}); break;
-    default: q8 ? f(Shape<true, 256>{}) : f(Shape<false, 256>{}); break;
-    }
+void with_shape(bool q8, int D, int rows, F f) {
+    auto pick = [&](auto type) {
+        constexpr bool Q8 = decltype(type)::value;
+        const bool two = rows > 8;
+        switch (D) {
+        case 64: two ? f(Shape<Q8, 64, 2>{}) : f(Shape<Q8, 64, 1>{}); break;
+        case 96: two ? f(Shape<Q8, 96, 2>{}) : f(Shape<Q8, 96, 1>{}); break;
+        case 128: two ? f(Shape<Q8, 128, 2>{}) : f(Shape<Q8, 128, 1>{}); break;
+        default: f(Shape<Q8, 256, 1>{}); break;
+        }
+    };
+    if (q8) pick(std::true_type{});
+    else pick(std::false_type{});
 }
 
 Geometry geometry(const b200_context * ctx, const b200_kv_cache * c, int64_t max_pages, int64_t n_seq, int64_t n_tok, int64_t n_head) {
@@ -858,10 +916,14 @@ Geometry geometry(const b200_context * ctx, const b200_kv_cache * c, int64_t max
     g.n_tok = (int) n_tok;
     g.n_head = (int) n_head;
     g.group = (int) (n_head / c->n_kv_head);
-    g.tiles = (g.n_tok * g.group + kRows - 1) / kRows;
+    with_shape(c->type == B200_TYPE_Q8_0, c->head_dim, g.n_tok * g.group, [&](auto shape) {
+        using S = decltype(shape);
+        g.rows = S::kRows;
+        g.ctas = (int64_t) ctx->num_sms * S::kCtas;
+    });
+    g.tiles = (g.n_tok * g.group + g.rows - 1) / g.rows;
     g.items = (int64_t) c->n_kv_head * g.tiles;
     g.n_seq = n_seq;
-    with_shape(c->type == B200_TYPE_Q8_0, c->head_dim, [&](auto shape) { g.ctas = (int64_t) ctx->num_sms * decltype(shape)::kCtas; });
     // By items when the lengths that the table allows are short: the cluster (1 to 8 CTAs) is the largest that all items fit
     // on the GPU with at once.
     const int64_t most = (max_pages * c->page_size + kChunk - 1) / kChunk;  // chunks of the longest sequence there can be
@@ -873,13 +935,12 @@ Geometry geometry(const b200_context * ctx, const b200_kv_cache * c, int64_t max
 }
 
 // ready: the kernels of this shape may use their shared memory on this device (set once per context).
-template <bool Q8, int D>
+template <class S>
 cudaError_t launch(const KvView & c, const Geometry & g, const float * q, int64_t ldq, float scale, float * out, float * ws, cudaStream_t st,
                    bool ready) {
-    constexpr int kBytes = Shape<Q8, D>::kBytes;
     if (!ready) {
-        cudaError_t e = cudaFuncSetAttribute(kv_attention_kernel<Q8, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kv_attention_item_kernel<Q8, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+        cudaError_t e = cudaFuncSetAttribute(kv_attention_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kv_attention_item_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg = {};
@@ -890,27 +951,27 @@ cudaError_t launch(const KvView & c, const Geometry & g, const float * q, int64_
     if (g.cluster) {
         cfg.gridDim = dim3((unsigned) (g.n_seq * g.items * g.cluster), 1, 1);
         cfg.blockDim = dim3(kThreads, 1, 1);
-        cfg.dynamicSmemBytes = kBytes;
+        cfg.dynamicSmemBytes = S::kBytes;
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = (unsigned) g.cluster;
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-        return cudaLaunchKernelEx(&cfg, kv_attention_item_kernel<Q8, D>, c, g, g.cluster, q, ldq, scale, out);
+        return cudaLaunchKernelEx(&cfg, kv_attention_item_kernel<S>, c, g, g.cluster, q, ldq, scale, out);
     }
-    kv_attention_kernel<Q8, D><<<(unsigned) g.ctas, kThreads, kBytes, st>>>(c, g, q, ldq, scale, out, ws);
+    kv_attention_kernel<S><<<(unsigned) g.ctas, kThreads, S::kBytes, st>>>(c, g, q, ldq, scale, out, ws);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    cfg.gridDim = dim3((unsigned) (g.n_seq * g.items * kRows), 1, 1);
+    cfg.gridDim = dim3((unsigned) (g.n_seq * g.items * g.rows), 1, 1);
     cfg.blockDim = dim3(32 * kJoinWarps, 1, 1);
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    return cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<D>, c, g, out, (const float *) ws);
+    return cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<S::kDim, S::kRows>, c, g, out, (const float *) ws);
 }
 
-size_t workspace_bytes_of(const Geometry & g, int D) { return g.cluster ? 0 : (size_t) (2 * g.ctas * partial_floats(D)) * sizeof(float); }
+size_t workspace_bytes_of(const Geometry & g, int D) { return g.cluster ? 0 : (size_t) (2 * g.ctas * partial_floats(D, g.rows)) * sizeof(float); }
 
 bool fits(const b200_kv_cache * c, int64_t max_pages, int64_t n_seq, int64_t n_tok, int64_t n_head) {
     return c && c->n_kv_head > 0 && c->page_size > 0 && max_pages >= 0 && n_seq > 0 && n_tok > 0 && n_tok <= 16 && n_head > 0 && n_head <= 65535 &&
-           n_head % c->n_kv_head == 0 && max_pages <= (1 << 30) / c->page_size && n_seq * n_tok <= INT32_MAX / kRows / n_head;
+           n_head % c->n_kv_head == 0 && max_pages <= (1 << 30) / c->page_size && n_seq * n_tok <= INT32_MAX / 16 / n_head;
 }
 
 }  // namespace
@@ -933,7 +994,7 @@ b200_status b200_kv_attention(b200_context * ctx, void * stream, const b200_kv_c
     if (n_tok > 16) return kv_fail(ctx, B200_ERR_UNSUPPORTED, what, "more than 16 tokens per sequence");
     if (n_head <= 0 || n_head > 65535 || n_head % c.n_kv_head) return kv_fail(ctx, B200_ERR_INVALID, what, "n_head is not a multiple of n_kv_head");
     if (n_seq == 0 || n_tok == 0) return B200_OK;
-    if (!fits(cache, max_pages, n_seq, n_tok, n_head)) return kv_fail(ctx, B200_ERR_INVALID, what, "n_seq * n_tok * n_head passes 2^28");
+    if (!fits(cache, max_pages, n_seq, n_tok, n_head)) return kv_fail(ctx, B200_ERR_INVALID, what, "n_seq * n_tok * n_head passes 2^27");
     if (ldq < n_head * c.head_dim) return kv_fail(ctx, B200_ERR_INVALID, what, "the row stride is below n_head * head_dim");
     if (!q || !out || ((uintptr_t) q & 3) || ((uintptr_t) out & 3)) return kv_fail(ctx, B200_ERR_INVALID, what, "NULL or misaligned q or out");
     const Geometry g = geometry(ctx, cache, max_pages, n_seq, n_tok, n_head);
@@ -944,12 +1005,10 @@ b200_status b200_kv_attention(b200_context * ctx, void * stream, const b200_kv_c
     if (scope.status != cudaSuccess) return kv_cuda(ctx, scope.status, what);
     cudaStream_t st = stream ? (cudaStream_t) stream : ctx->stream;
     const bool q8 = cache->type == B200_TYPE_Q8_0;
-    const unsigned bit = 1u << ((c.head_dim / 32) + (q8 ? 16 : 0));
+    const unsigned bit = 1u << (c.head_dim / 32 + (q8 ? 8 : 0) + (g.rows == 8 ? 0 : 16));
     cudaError_t e = cudaErrorInvalidValue;
-    with_shape(q8, c.head_dim, [&](auto shape) {
-        using S = decltype(shape);
-        e = launch<S::kKeyWords == 2, 32 * S::kBlocks>(c, g, q, ldq, scale, out, (float *) workspace, st, ctx->kv_shapes & bit);
-    });
+    with_shape(q8, c.head_dim, g.n_tok * g.group,
+               [&](auto shape) { e = launch<decltype(shape)>(c, g, q, ldq, scale, out, (float *) workspace, st, ctx->kv_shapes & bit); });
     if (e == cudaSuccess) ctx->kv_shapes |= bit;
     return kv_cuda(ctx, e, what);
 }
