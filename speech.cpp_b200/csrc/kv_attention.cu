@@ -646,9 +646,24 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                     }
                 }
             };
-            if (edge && g.n_tok > 1) {
-                // Where rows see different positions, a value that is NaN or infinite must not meet the weight 0 of a row
-                // that does not see it: one product per token, with the values behind its position zeroed.
+            bool flaw = false;
+            if (edge && g.n_tok > 1) {  // is a value that not every row sees NaN or infinite?
+                uint32_t high = 0;
+#pragma unroll
+                for (int n = 0; n < S::kGroups; n++) {
+                    Words w;
+                    values(w, 0, n);
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int r = 0; r < S::kValueWords; r++)
+                            if (p0 + 2 * t + (i & 1) + 8 * (i >> 1) >= all_see) high = __vmaxu2(high, w[i][r] & 0x7c007c00u);
+                }
+                flaw = __any_sync(0xffffffffu, (high & 0xffffu) == 0x7c00u || high >= 0x7c000000u);
+            }
+            if (flaw) {
+                // It must not meet the weight 0 of a row that does not see it: one product per token, with the values behind
+                // its position zeroed. (With finite values this gives the bits that one product for all gives.)
                 const int last = min((tile * S::kRows + S::kRows - 1) / g.group, g.n_tok - 1);
                 for (int token = tile * S::kRows / g.group; token <= last; token++) product(all_see + token - p0, token);
             } else {
