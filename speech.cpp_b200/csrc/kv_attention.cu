@@ -46,6 +46,7 @@ constexpr float kShift = 14;  // weights are held times 2^14, so that their low 
 struct Geometry {
     int n_tok, n_head, group;
     int rows, tiles;                  // rows of an item; items of a key/value head
+    int vec;                          // q's rows and out are 16-byte aligned
     int64_t items;                    // n_kv_head * tiles, per sequence
     int64_t n_seq;
     int64_t ctas;                     // CTAs among which the chunks are divided, or
@@ -171,28 +172,35 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
     return v;
 }
 
-// Chunks of sequences [0, n), summed by the block (red: one value per warp).
-__device__ __forceinline__ int64_t block_chunks(const KvView & c, int64_t n, int64_t * red) {
-    int64_t sum = 0;
-    for (int64_t s = threadIdx.x; s < n; s += kThreads) sum += chunks_of(c, s, blockIdx.x == 0);
-    sum = warp_sum64(sum);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
-    __syncthreads();
-    sum = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; w++) sum += red[w];
-    return sum;
-}
+// Where a CTA's share of the chunks lies: chunk numbers count the sequences' chunks one after the other, each `items` times.
+struct Place {
+    int64_t at, end;     // the chunks [at, end) of all
+    int64_t seq, start;  // the sequence that chunk `at` lies in, and its first chunk (when at < end)
+};
 
-// The sequence that holds chunk number `at` (of one item; chunk numbers count each sequence's chunks `items` times), and
-// where it starts. at < the total.
-__device__ __forceinline__ void find_sequence(const KvView & c, const Geometry & g, int64_t at, int64_t * red, int64_t & seq, int64_t & start) {
+// Block-wide (every thread gets the result): the lengths are read kThreads at a time, summed for the share and scanned for
+// the sequence; up to kThreads of them stay in registers in between.
+__device__ __forceinline__ Place find_place(const KvView & c, const Geometry & g, int64_t * red) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t first = threadIdx.x < g.n_seq ? chunks_of(c, threadIdx.x, blockIdx.x == 0) * g.items : 0;
+    int64_t sum = first;
+    for (int64_t s = threadIdx.x + kThreads; s < g.n_seq; s += kThreads) sum += chunks_of(c, s, blockIdx.x == 0) * g.items;
+    sum = warp_sum64(sum);
+    if (lane == 0) red[warp] = sum;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) total += red[w];
+    const int64_t share = (total + g.ctas - 1) / g.ctas;
+    Place p;
+    p.at = blockIdx.x * share;
+    p.end = p.at + share < total ? p.at + share : total;
+    p.seq = p.start = 0;
+    if (p.at >= p.end) return p;  // the same for all threads
     int64_t base = 0;
     for (int64_t s0 = 0; s0 < g.n_seq; s0 += kThreads) {
         const int64_t s = s0 + threadIdx.x;
-        const int64_t mine = s < g.n_seq ? chunks_of(c, s, false) * g.items : 0;
+        const int64_t mine = s0 == 0 ? first : s < g.n_seq ? chunks_of(c, s, false) * g.items : 0;
         int64_t incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -202,23 +210,24 @@ __device__ __forceinline__ void find_sequence(const KvView & c, const Geometry &
         __syncthreads();
         if (lane == 31) red[warp] = incl;
         __syncthreads();
-        int64_t first = base, all = 0;
+        int64_t before = base, all = 0;
 #pragma unroll
         for (int w = 0; w < kWarps; w++) {
-            if (w < warp) first += red[w];
+            if (w < warp) before += red[w];
             all += red[w];
         }
-        const int64_t begin = first + incl - mine;
-        if (mine > 0 && at >= begin && at < begin + mine) {
+        const int64_t begin = before + incl - mine;
+        if (mine > 0 && p.at >= begin && p.at < begin + mine) {
             red[kWarps] = s;
             red[kWarps + 1] = begin;
         }
         base += all;
-        if (at < base) break;  // the same for all threads
+        if (p.at < base) break;  // the same for all threads
     }
     __syncthreads();
-    seq = red[kWarps];
-    start = red[kWarps + 1];
+    p.seq = red[kWarps];
+    p.start = red[kWarps + 1];
+    return p;
 }
 
 // Rows of an item: row i is query head h * group + n % group of token n / group, n = tile * rows + i.
@@ -242,8 +251,9 @@ struct Shared {
     static constexpr int kRingBytes = S::kStages * S::kStage;
     static constexpr int kPitch = S::kDim + 4;
     static_assert(S::kRows * kPitch * 4 <= kRingBytes, "a warp's o fits its ring");
-    __device__ __forceinline__ float & o(int w, int row, int d) const {
-        return reinterpret_cast<float *>(ring + w * kRingBytes)[row * kPitch + d];
+    // dimensions d to d + 3 of a row (d % 4 == 0)
+    __device__ __forceinline__ float4 & o(int w, int row, int d) const {
+        return reinterpret_cast<float4 *>(ring + w * kRingBytes)[(row * kPitch + d) / 4];
     }
 };
 
@@ -352,11 +362,18 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
     for (int y = 0; y < TILES; y++) {
         const float * src = q + (seq * g.n_tok + row[y].token) * ldq + (int64_t) row[y].head * D + 8 * t;
         float x[D / 4], top = 0.0f;
+        if (g.vec && row[y].there) {
 #pragma unroll
-        for (int i = 0; i < D / 4; i++) {
-            x[i] = row[y].there ? src[(i / 8) * 32 + i % 8] : 0.0f;
-            top = fmaxf(top, fabsf(x[i]));
+            for (int i = 0; i < D / 4; i += 4) {
+                const float4 v = *reinterpret_cast<const float4 *>(src + (i / 8) * 32 + i % 8);
+                x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < D / 4; i++) x[i] = row[y].there ? src[(i / 8) * 32 + i % 8] : 0.0f;
         }
+#pragma unroll
+        for (int i = 0; i < D / 4; i++) top = fmaxf(top, fabsf(x[i]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int e = (int) (__float_as_uint(top) >> 23);
@@ -686,12 +703,24 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
 #pragma unroll
         for (int n = 0; n < S::kGroups; n++)
 #pragma unroll
-            for (int r = 0; r < S::kRun; r++) {
-                sh.o(warp, 8 * y + gq, n * 8 * S::kRun + 2 * t * S::kRun + r) = o[y][n][r].x;
-                sh.o(warp, 8 * y + gq, n * 8 * S::kRun + (2 * t + 1) * S::kRun + r) = o[y][n][r].y;
+            for (int r = 0; r < S::kRun; r += 4) {
+                const float2 * v = &o[y][n][r];
+                sh.o(warp, 8 * y + gq, n * 8 * S::kRun + 2 * t * S::kRun + r) = make_float4(v[0].x, v[1].x, v[2].x, v[3].x);
+                sh.o(warp, 8 * y + gq, n * 8 * S::kRun + (2 * t + 1) * S::kRun + r) = make_float4(v[0].y, v[1].y, v[2].y, v[3].y);
             }
     }
     __syncthreads();
+}
+
+__device__ __forceinline__ float4 fma4(float4 a, float b, float4 c) {
+    return make_float4(fmaf(a.x, b, c.x), fmaf(a.y, b, c.y), fmaf(a.z, b, c.z), fmaf(a.w, b, c.w));
+}
+
+// Four results times f to p.
+__device__ __forceinline__ void put4(float * p, float4 v, float f, bool vec) {
+    v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+    if (vec) *reinterpret_cast<float4 *>(p) = v;
+    else p[0] = v.x, p[1] = v.y, p[2] = v.z, p[3] = v.w;
 }
 
 // The CTA's sum of the warps' results for one row: the factors of the warps, and m and l.
@@ -710,10 +739,10 @@ struct Joined {
             l = fmaf(sh.sl[w][i], f[w], l);
         }
     }
-    __device__ __forceinline__ float value(const Shared<S> & sh, int i, int d) const {
-        float v = 0.0f;
+    __device__ __forceinline__ float4 value(const Shared<S> & sh, int i, int d) const {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) v = fmaf(sh.o(w, i, d), f[w], v);
+        for (int w = 0; w < kWarps; w++) v = fma4(sh.o(w, i, d), f[w], v);
         return v;
     }
 };
@@ -730,13 +759,10 @@ __global__ void __launch_bounds__(kThreads, S::kCtas)
     const int tid = threadIdx.x;
     pdl_launch_dependents();
 
-    const int64_t total = block_chunks(c, g.n_seq, red) * g.items;
-    const int64_t share = (total + g.ctas - 1) / g.ctas;
-    int64_t at = blockIdx.x * share;
-    const int64_t end = at + share < total ? at + share : total;
+    const Place place = find_place(c, g, red);
+    int64_t at = place.at, seq = place.seq, start = place.start;
+    const int64_t end = place.end;
     if (at >= end) return;
-    int64_t seq, start;
-    find_sequence(c, g, at, red, seq, start);
     int64_t len = kv_len(c, seq, false), chunks = (len + kChunk - 1) / kChunk;
 
     while (at < end) {
@@ -758,10 +784,11 @@ __global__ void __launch_bounds__(kThreads, S::kCtas)
             if (c0 == 0 && c1 == chunks) {  // the whole item
                 const float inv = all.l != 0.0f ? 1.0f / all.l : 0.0f;
                 if (row.there)
-                    for (int d = tid & 15; d < D; d += 16) out[((seq * g.n_tok + row.token) * g.n_head + row.head) * D + d] = all.value(sh, i, d) * inv;
+                    for (int d = 4 * (tid & 15); d < D; d += 64)
+                        put4(out + ((seq * g.n_tok + row.token) * g.n_head + row.head) * D + d, all.value(sh, i, d), inv, g.vec);
             } else {  // the CTA's first partial (of an item begun before it) or its last
                 float * to = ws + (2 * blockIdx.x + (c0 == 0 ? 1 : 0)) * partial_floats(D, kRows);
-                for (int d = tid & 15; d < D; d += 16) to[i * D + d] = all.value(sh, i, d);
+                for (int d = 4 * (tid & 15); d < D; d += 64) put4(to + i * D + d, all.value(sh, i, d), 1.0f, true);
                 if ((tid & 15) == 0) {
                     to[kRows * D + i] = all.m;
                     to[kRows * D + kRows + i] = all.l;
@@ -790,24 +817,25 @@ __global__ void __launch_bounds__(kThreads, S::kCtas)
     attend<S>(c, g, q, ldq, scale, sh, seq, len, h, tile, c0, c1);
     for (int i = tid / 16; i < kRows; i += kThreads / 16) {
         const Joined<S> all(sh, i);
-        for (int d = tid & 15; d < D; d += 16) sh.o(0, i, d) = all.value(sh, i, d);  // read and written by this thread alone
+        for (int d = 4 * (tid & 15); d < D; d += 64) sh.o(0, i, d) = all.value(sh, i, d);  // read and written by this thread alone
         if ((tid & 15) == 0) jm[i] = all.m, jl[i] = all.l;
     }
     const cooperative_groups::cluster_group group = cooperative_groups::this_cluster();
     group.sync();
-    for (int e = tid; e < kRows / cluster * D; e += kThreads) {
-        const int i = e / D * cluster + rank, d = e % D;
+    for (int e = tid; e < kRows / cluster * (D / 4); e += kThreads) {
+        const int i = e / (D / 4) * cluster + rank, d = e % (D / 4) * 4;
         const Row row = row_of<kRows>(g, h, tile, i);
         if (!row.there) continue;
-        float m = -INFINITY, l = 0.0f, v = 0.0f;
+        float m = -INFINITY, l = 0.0f;
         for (int r = 0; r < cluster; r++) m = fmaxf(m, *group.map_shared_rank(&jm[i], r));
         const float base = m == -INFINITY ? 0.0f : m;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int r = 0; r < cluster; r++) {
             const float f = ex2(*group.map_shared_rank(&jm[i], r) - base);
             l = fmaf(*group.map_shared_rank(&jl[i], r), f, l);
-            v = fmaf(*group.map_shared_rank(&sh.o(0, i, d), r), f, v);
+            v = fma4(*group.map_shared_rank(&sh.o(0, i, d), r), f, v);
         }
-        out[((seq * g.n_tok + row.token) * g.n_head + row.head) * D + d] = l != 0.0f ? v * (1.0f / l) : 0.0f;
+        put4(out + ((seq * g.n_tok + row.token) * g.n_head + row.head) * D + d, v, l != 0.0f ? 1.0f / l : 0.0f, g.vec);
     }
     group.sync();  // the others read this CTA's shared memory until here
 }
@@ -927,7 +955,7 @@ void with_shape(bool q8, int D, int rows, F f) {
 }
 
 Geometry geometry(const b200_context * ctx, const b200_kv_cache * c, int64_t max_pages, int64_t n_seq, int64_t n_tok, int64_t n_head) {
-    Geometry g;
+    Geometry g = {};
     g.n_tok = (int) n_tok;
     g.n_head = (int) n_head;
     g.group = (int) (n_head / c->n_kv_head);
@@ -1012,7 +1040,8 @@ b200_status b200_kv_attention(b200_context * ctx, void * stream, const b200_kv_c
     if (!fits(cache, max_pages, n_seq, n_tok, n_head)) return kv_fail(ctx, B200_ERR_INVALID, what, "n_seq * n_tok * n_head passes 2^27");
     if (ldq < n_head * c.head_dim) return kv_fail(ctx, B200_ERR_INVALID, what, "the row stride is below n_head * head_dim");
     if (!q || !out || ((uintptr_t) q & 3) || ((uintptr_t) out & 3)) return kv_fail(ctx, B200_ERR_INVALID, what, "NULL or misaligned q or out");
-    const Geometry g = geometry(ctx, cache, max_pages, n_seq, n_tok, n_head);
+    Geometry g = geometry(ctx, cache, max_pages, n_seq, n_tok, n_head);
+    g.vec = ((uintptr_t) q & 15) == 0 && ((uintptr_t) out & 15) == 0 && ldq % 4 == 0;
     const size_t need = workspace_bytes_of(g, c.head_dim);
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t) workspace & 255)))
         return kv_fail(ctx, B200_ERR_INVALID, what, "the workspace is missing, misaligned or too small");
