@@ -11,8 +11,7 @@ struct KvView {
     const uint8_t * v;
     const __half * kd;   // Q8_0 scales [n_pages][n_kv_head][page_size][head_dim / 32]
     const __half * vd;
-    int n_kv_head, head_dim, page_size;
-    int64_t n_pages;
+    int n_kv_head, head_dim, page_size, n_pages;
     const int32_t * table;  // [n_seq][max_pages]
     const int32_t * lens;   // [n_seq]
     int64_t max_pages;
@@ -31,7 +30,7 @@ __device__ __forceinline__ int64_t kv_len(const KvView & c, int64_t s, bool tell
 // Page number i of sequence s, or -1 (reported) when the table holds one outside the cache.
 __device__ __forceinline__ int kv_page(const KvView & c, int64_t s, int64_t i, bool tell) {
     const int p = c.table[s * c.max_pages + i];
-    if (p >= 0 && p < c.n_pages) return p;
+    if ((unsigned) p < (unsigned) c.n_pages) return p;
     if (tell) atomicOr(c.err, B200_DEVERR_PAGE);
     return -1;
 }

@@ -278,7 +278,9 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
     // ---- the ring: steps of kSub pieces, the warps in turn through [c0 * 64, c1 * 64), copied kStages - 1 ahead ----
     constexpr int kSub = S::kSub, kStep = kWarps * 16 * kSub;
     const uint32_t ring = smem_addr(sh.ring) + warp * Shared<S>::kRingBytes;
-    const int64_t page_bytes = (int64_t) c.n_kv_head * c.page_size * kRowBytes;
+    // a page's bytes: a multiple of 512 (16 rows of a multiple of 32 bytes), and 32 bits hold them in such units
+    const uint32_t page_units = (uint32_t) ((int64_t) c.n_kv_head * c.page_size * kRowBytes / 512);
+    const int32_t * pages = c.table + seq * c.max_pages;
     const uint8_t * kh = c.k + (int64_t) h * c.page_size * kRowBytes + lane * 16;
     const int64_t to_values = c.v - c.k;
     const uint8_t * scales = nullptr;  // this lane's 16 bytes of a piece's scales: the keys', then the values'
@@ -292,7 +294,7 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
     auto find_pages = [&] {
 #pragma unroll
         for (int u = 0; u < kSub; u++)
-            page[u] = p_copy + 16 * u < p_end ? kv_page(c, seq, in_table + (slot + 16 * u >= c.page_size), lane == 0) : -1;
+            page[u] = p_copy + 16 * u < p_end ? pages[in_table + (slot + 16 * u >= c.page_size)] : -1;
     };
     find_pages();
     // where this lane's first 16 bytes of a piece go: row lane / (chunks of a row), chunk lane % (chunks of a row)
@@ -303,9 +305,11 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
         if (p_copy < p_end) {
 #pragma unroll
             for (int u = 0; u < kSub; u++) {
-                const int here = page[u] < 0 ? 0 : p_end - p_copy - 16 * u;  // rows of the piece; the others are zeros
+                const bool exists = (unsigned) page[u] < (unsigned) c.n_pages;
+                const int here = exists ? p_end - p_copy - 16 * u : 0;  // rows of the piece; the others are zeros
+                if (!exists && p_copy + 16 * u < p_end && lane == 0) atomicOr(c.err, B200_DEVERR_PAGE);
                 const int in_page = slot + 16 * u - (slot + 16 * u >= c.page_size ? c.page_size : 0);
-                const int64_t at = max(page[u], 0) * page_bytes + in_page * kRowBytes;
+                const int64_t at = (int64_t) ((uint64_t) (exists ? page[u] : 0) * page_units << 9) + in_page * kRowBytes;
                 const uint8_t * from = kh + at;
                 const uint32_t to = ring + stage_copy * S::kStage + u * S::kPiece;
                 constexpr int kRowChunks = kRowBytes / 16, kCopies = kRowChunks / 2;  // a piece's rows are contiguous: 16 kRowChunks chunks
@@ -333,10 +337,10 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                 if (here >= 16) each(std::true_type{});
                 else each(std::false_type{});
                 if constexpr (Q8) {  // whole, rows behind the end too: they lie in the page
-                    if (lane < 2 * S::kScaleBytes) copy16(to + kKeyScales + lane * 16, scales + at / 16, page[u] >= 0);
+                    if (lane < 2 * S::kScaleBytes) copy16(to + kKeyScales + lane * 16, scales + at / 16, exists);
                 }
                 const unsigned bit = 1u << (kSub * stage_copy + u);
-                found = page[u] < 0 ? found & ~bit : found | bit;
+                found = exists ? found | bit : found & ~bit;
             }
             p_copy += kStep;
             in_table += page_step;

@@ -46,7 +46,7 @@ b200_status kv_checked_view(b200_context * ctx, const char * what, const b200_kv
     out->n_kv_head = c->n_kv_head;
     out->head_dim = c->head_dim;
     out->page_size = c->page_size;
-    out->n_pages = c->n_pages;
+    out->n_pages = (int) c->n_pages;  // at most INT32_MAX (kv_sizes)
     out->table = table;
     out->lens = lens;
     out->max_pages = max_pages;
