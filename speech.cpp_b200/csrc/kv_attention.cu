@@ -357,10 +357,7 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
     // ---- the query tile's fragments ----
     // k step 2 j + b of lane (gq, t) holds dimensions 32 j + 8 t + 4 b .. + 3 of row gq: hi in registers 0 and 2, lo in
     // 1 and 3. The row is scaled by 2^k to a largest magnitude in [2^14, 2^15).
-    // Q8_0: key bytes enter as q + 128 in the low byte of an F16, which is (q + 128) 2^-24 (a subnormal, and exact); `bias` is
-    // what the 128 adds to a block's sum.
     uint32_t qf[TILES][D / 16][4];
-    float bias[TILES][Q8 ? S::kBlocks : 1];
     float factor[TILES];  // what a raw score is multiplied by: scale log2(e) 2^-k
 #pragma unroll
     for (int y = 0; y < TILES; y++) {
@@ -388,18 +385,6 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
         for (int j = 0; j < D / 16; j++) {
             split(x[4 * j] * up, x[4 * j + 1] * up, qf[y][j][0], qf[y][j][1]);
             split(x[4 * j + 2] * up, x[4 * j + 3] * up, qf[y][j][2], qf[y][j][3]);
-        }
-        if constexpr (Q8) {
-            factor[y] *= 0x1p24f;
-#pragma unroll
-            for (int b = 0; b < S::kBlocks; b++) {
-                float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; i++) sum = fmaf(x[8 * b + i], up, sum);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                bias[y][b] = sum * -0x1p-17f;
-            }
         }
     }
 
@@ -437,7 +422,6 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
 #pragma unroll
                 for (int i = 0; i < 2; i++) lds(kd[i], at + u * S::kPiece + kKeyScales + (2 * t + 8 * i) * S::kScaleBytes);
             }
-            float sum[TILES][2][4] = {};
             float2 part[TILES][2] = {};
 #pragma unroll
             for (int b = 0; b < S::kBlocks; b++)
@@ -447,22 +431,23 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                     lds(w, S::along(keys, b * (Q8 ? 32 : 64)) + i * 8 * kRowBytes);
                     if constexpr (Q8) {
                         const uint32_t w0 = w[0] ^ 0x80808080u, w1 = w[1] ^ 0x80808080u;
-                        const uint32_t f[4] = {__byte_perm(w0, 0, 0x4140), __byte_perm(w0, 0, 0x4342), __byte_perm(w1, 0, 0x4140), __byte_perm(w1, 0, 0x4342)};
+                        const uint32_t f[4] = {halves(w0, 0x4140), halves(w0, 0x4342), halves(w1, 0x4140), halves(w1, 0x4342)};
                         const float2 d = make_float2(half_of(kd[i], b), half_of(kd[i], S::kBlocks + b));
 #pragma unroll
                         for (int y = 0; y < TILES; y++) {
                             float r[4];
                             mma(r, qf[y][2 * b], f[0], f[1]);
                             mma(r, qf[y][2 * b + 1], f[2], f[3], r);
-                            const float2 whole =
-                                __fadd2_rn(make_float2(r[0], r[1]), __fadd2_rn(make_float2(r[2], r[3]), make_float2(bias[y][b], bias[y][b])));
+                            const float2 whole = __fadd2_rn(make_float2(r[0], r[1]), make_float2(r[2], r[3]));
                             part[y][i] = __ffma2_rn(d, whole, part[y][i]);
                         }
                     } else {
 #pragma unroll
                         for (int y = 0; y < TILES; y++) {
-                            mma(sum[y][i], qf[y][2 * b], w[0], w[1], sum[y][i]);
-                            mma(sum[y][i], qf[y][2 * b + 1], w[2], w[3], sum[y][i]);
+                            float r[4];
+                            mma(r, qf[y][2 * b], w[0], w[1]);
+                            mma(r, qf[y][2 * b + 1], w[2], w[3], r);
+                            part[y][i] = __fadd2_rn(part[y][i], __fadd2_rn(make_float2(r[0], r[1]), make_float2(r[2], r[3])));
                         }
                     }
                 }
@@ -470,8 +455,6 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
             for (int y = 0; y < TILES; y++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    if constexpr (!Q8)
-                        part[y][i] = __fadd2_rn(make_float2(sum[y][i][0], sum[y][i][1]), make_float2(sum[y][i][2], sum[y][i][3]));
                     s[y][u][2 * i] = part[y][i].x * factor[y];
                     s[y][u][2 * i + 1] = part[y][i].y * factor[y];
                 }
