@@ -40,7 +40,8 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kJoinWarps = 8;
 constexpr int kChunk = 64;    // positions of a chunk: one 16-position tile per warp
-constexpr int kItemChunks = 8;  // chunks per CTA up to which the work is cut by items
+constexpr int kItemChunks = 16;  // the work is cut by items up to this many chunks per CTA,
+constexpr int kItemMost = 64;    // and this many per sequence
 constexpr float kShift = 14;  // weights are held times 2^14, so that their low halves reach 2^-38 of the largest
 
 struct Geometry {
@@ -955,11 +956,14 @@ Geometry geometry(const b200_context * ctx, const b200_kv_cache * c, int64_t max
     g.items = (int64_t) c->n_kv_head * g.tiles;
     g.n_seq = n_seq;
     // By items when the lengths that the table allows are short: the cluster (1 to 8 CTAs) is the largest that all items fit
-    // on the GPU with at once.
+    // on the GPU with at once. One launch instead of two, and no scan of the lengths, against CTAs with equal work. Measured
+    // (F16, 16 and 8 heads of 128, lengths from a quarter of the table's width to all of it), by items and by positions: 1
+    // sequence of 512: 5.6 and 6.4 us, 4096: 10.5 and 8.4 (where the second launch costs the host as much again); 8 sequences of
+    // 1024: 8.3 and 11.2, 4096: 18.3 and 18.2; 64 sequences of 1024: 33.6 and 41.0, 2048: 64.0 and 65.2.
     const int64_t most = (max_pages * c->page_size + kChunk - 1) / kChunk;  // chunks of the longest sequence there can be
     g.cluster = 8;
     while (g.cluster > 1 && n_seq * g.items * g.cluster > g.ctas) g.cluster /= 2;
-    if (most > kItemChunks * g.cluster) g.cluster = 0;
+    if (most > kItemChunks * g.cluster || most > kItemMost) g.cluster = 0;
     if (g.ctas > most * n_seq * g.items) g.ctas = most > 0 ? most * n_seq * g.items : 1;
     return g;
 }
