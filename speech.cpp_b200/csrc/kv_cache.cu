@@ -30,11 +30,12 @@ b200_status kv_cuda(b200_context * ctx, cudaError_t e, const char * what) {
 b200_status kv_checked_view(b200_context * ctx, const char * what, const b200_kv_cache * c, const int32_t * table, int64_t max_pages,
                             const int32_t * lens, int64_t n_seq, int64_t n_tok, KvView * out) {
     if (!ctx) return kv_fail(ctx, B200_ERR_INVALID, what, "NULL context");
-    if (!c || !c->data || c->nbytes < b200_kv_cache_nbytes(c->type, c->n_kv_head, c->head_dim, c->page_size, c->n_pages) || c->nbytes == 0)
-        return kv_fail(ctx, B200_ERR_INVALID, what, "not a cache");
+    const size_t need = c ? b200_kv_cache_nbytes(c->type, c->n_kv_head, c->head_dim, c->page_size, c->n_pages) : 0;
+    if (!need || !c->data || c->nbytes < need) return kv_fail(ctx, B200_ERR_INVALID, what, "not a cache");
     if (c->device != ctx->device) return kv_fail(ctx, B200_ERR_INVALID, what, "the cache lies on another device than the context");
     if (n_seq < 0 || n_tok < 0 || max_pages < 0) return kv_fail(ctx, B200_ERR_INVALID, what, "a negative size");
-    if (n_seq > 0 && n_tok > 0 && (!lens || (max_pages > 0 && !table))) return kv_fail(ctx, B200_ERR_INVALID, what, "NULL table or lens");
+    if (n_seq > 0 && n_tok > 0 && (!lens || (max_pages > 0 && !table) || ((uintptr_t) lens & 3) || ((uintptr_t) table & 3)))
+        return kv_fail(ctx, B200_ERR_INVALID, what, "NULL or misaligned table or lens");
     if (max_pages > (1 << 30) / c->page_size) return kv_fail(ctx, B200_ERR_INVALID, what, "max_pages * page_size passes 2^30");
     // one CTA per row (or fewer) in a one-dimensional grid
     if (n_tok > 0 && n_seq > INT32_MAX / n_tok) return kv_fail(ctx, B200_ERR_INVALID, what, "n_seq * n_tok passes 2^31");
@@ -345,7 +346,8 @@ b200_status b200_kv_read(b200_context * ctx, void * stream, const b200_kv_cache 
     if (out_type != B200_TYPE_F32 && out_type != B200_TYPE_F16) return kv_fail(ctx, B200_ERR_UNSUPPORTED, "kv_read", "rows are read as F32 or F16");
     if (n_seq == 0 || n_tok == 0) return B200_OK;
     const size_t elem = out_type == B200_TYPE_F16 ? 2 : 4;
-    if (!k || !v || !aligned(k, elem) || !aligned(v, elem)) return kv_fail(ctx, B200_ERR_INVALID, "kv_read", "NULL or misaligned k or v");
+    if (!k || !v || !aligned(k, elem) || !aligned(v, elem) || !aligned(start, 4))
+        return kv_fail(ctx, B200_ERR_INVALID, "kv_read", "NULL or misaligned k or v, or a misaligned start");
     DeviceScope scope(ctx->device);
     if (scope.status != cudaSuccess) return kv_cuda(ctx, scope.status, "kv_read");
     const bool vec = aligned(k, 4 * elem) && aligned(v, 4 * elem);

@@ -428,7 +428,8 @@ extern "C" b200_status b200_moe_router(b200_context * ctx, void * stream, const 
         return kv_fail(ctx, B200_ERR_INVALID, what, "bad groups");
     if (r->top_k > r->n_expert / r->n_group * r->topk_group) return kv_fail(ctx, B200_ERR_INVALID, what, "top_k passes the experts that stay");
     if (T == 0) return B200_OK;
-    if (!logits || !ids || !w) return kv_fail(ctx, B200_ERR_INVALID, what, "NULL argument");
+    if (!logits || !ids || !w || (((uintptr_t) logits | (uintptr_t) bias | (uintptr_t) ids | (uintptr_t) w) & 3))
+        return kv_fail(ctx, B200_ERR_INVALID, what, "a NULL or misaligned argument");
     if (T > (int64_t) INT32_MAX) return kv_fail(ctx, B200_ERR_INVALID, what, "more than 2^31 rows");
     DeviceScope scope(ctx->device);
     if (scope.status != cudaSuccess) return kv_cuda(ctx, scope.status, what);

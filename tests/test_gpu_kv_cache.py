@@ -1,6 +1,8 @@
 """The paged key/value cache on the GPU: rows written, read back and attended to, against plain 64-bit restatements
 (tests/kv_reference.py) and, for Q8_0, against the oracle's row quantizer bit for bit."""
 
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -157,6 +159,14 @@ def test_refusals(b200, ctx):
     assert L.b200_kv_write(*args, 1 << 20, 1 << 20, vp, 128, vp, 128) == b200.ERR_INVALID
     assert L.b200_kv_write(ctx.h, None, cache.ref, table.data_ptr(), 1 << 30, lens.data_ptr(), 2, 1, vp, 128, vp, 128) == b200.ERR_INVALID
     assert L.b200_kv_write(ctx.h, None, cache.ref, None, 2, lens.data_ptr(), 2, 1, vp, 128, vp, 128) == b200.ERR_INVALID
+    assert L.b200_kv_write(ctx.h, None, cache.ref, table.data_ptr() + 2, 2, lens.data_ptr(), 2, 1, vp, 128, vp, 128) == b200.ERR_INVALID
+    assert L.b200_kv_read(ctx.h, None, cache.ref, table.data_ptr(), 2, lens.data_ptr(), lens.data_ptr() + 1, 2, 1, b200.F32, vp, vp) == b200.ERR_INVALID
+    for name, value in (("page_size", 0), ("head_dim", 100), ("n_pages", 1 << 40), ("type", b200.F32), ("n_kv_head", 0), ("device", 1)):
+        bad = b200.KvCacheStruct.from_buffer_copy(cache.s)
+        setattr(bad, name, value)
+        call = (ctx.h, None, ctypes.byref(bad), table.data_ptr(), 2, lens.data_ptr(), 2, 1)
+        assert L.b200_kv_write(*call, vp, 128, vp, 128) == b200.ERR_INVALID
+        assert L.b200_kv_attention(*call, 2, vp, 128, 1.0, vp, None, 0) == b200.ERR_INVALID
     assert L.b200_kv_read(*args, None, 2, 1, b200.Q8_0, vp, vp) == b200.ERR_UNSUPPORTED
     assert L.b200_kv_read(*args, None, 2, 1, b200.F32, vp, None) == b200.ERR_INVALID
     assert L.b200_kv_attention(*args, 2, 1, 2, vp, 64, 1.0, vp, None, 0) == b200.ERR_INVALID
@@ -334,6 +344,37 @@ def test_attention_is_split_over_a_long_cache(b200, ctx, qname):
 
 
 @pytest.mark.parametrize("qname", ["F16", "Q8_0"])
+@pytest.mark.parametrize("D,Hkv,group,page,n_tok,lens", [
+    (64, 3, 5, 48, 2, [777, 1, 0, 48, 49, 600, 95]),
+    (64, 2, 2, 16, 1, [130, 5]),
+    (96, 2, 3, 16, 1, [100, 1000, 0]),
+    (96, 1, 4, 80, 4, [81, 333, 2]),
+    (128, 8, 2, 32, 5, [1, 5, 300, 64, 0, 4, 65, 127]),
+    (128, 2, 1, 16, 1, [1, 2, 15, 16, 17, 31, 32, 33]),
+    (128, 1, 20, 16, 2, [400, 64]),
+    (256, 2, 4, 32, 3, [260, 31, 1]),
+])
+def test_attention_with_a_wide_table(b200, ctx, qname, D, Hkv, group, page, n_tok, lens):
+    """The same with a table that allows long sequences: the work is cut by positions and joined by a second kernel."""
+    import torch
+
+    p = Pool(b200, ctx, getattr(b200, qname), Hkv, D, page, lens, seed=D + len(lens), width=-(-5000 // page)).fill()
+    assert ctx.L.b200_kv_attention_workspace(ctx.h, p.cache.ref, p.width, len(lens), n_tok, Hkv * group) > 0
+    out = torch.full((len(lens), n_tok, Hkv * group, D), float("nan"), device="cuda")
+    got = p.check_attention(Hkv * group, n_tok, out=out)
+    for s, n in enumerate(lens):
+        assert not got[s, :max(0, n_tok - n)].any()
+
+
+def test_attention_of_many_sequences(b200, ctx):
+    """More sequences than a CTA has threads: their lengths are scanned in several steps."""
+    rng = np.random.default_rng(20)
+    lens = rng.integers(0, 40, 300).tolist()
+    lens[131] = 5000
+    Pool(b200, ctx, b200.F16, 1, 64, 16, lens, seed=20).fill().check_attention(2, 1)
+
+
+@pytest.mark.parametrize("qname", ["F16", "Q8_0"])
 @pytest.mark.parametrize("width", [1, 2, 300])
 def test_attention_whatever_the_tables_width(b200, ctx, qname, width):
     """The table's width bounds the lengths, not what is computed: a wide table of short sequences, an exactly full one."""
@@ -357,12 +398,13 @@ def test_attention_with_scores_far_apart(b200, ctx, qname):
     p.check_attention(4, 1, q=q)  # the mean of the values
 
 
-def test_attention_does_not_see_what_lies_behind_a_row(b200, ctx):
+@pytest.mark.parametrize("width", [None, 300])
+def test_attention_does_not_see_what_lies_behind_a_row(b200, ctx, width):
     """Positions that later rows of the call see, but an earlier one does not, hold NaN and infinities: the earlier rows
     come out as if these were not there; the later ones are NaN where the definition is."""
     import torch
 
-    p = Pool(b200, ctx, b200.F16, 2, 128, 16, [50, 17], seed=9).fill()
+    p = Pool(b200, ctx, b200.F16, 2, 128, 16, [50, 17], seed=9, width=width).fill()
     q = p.rng.normal(0, 1, (2, 4, 4, 128)).astype(np.float32)
     clean = ctx.kv_attention(p.cache, cu(q), p.table, p.lens_t, 0.1)
     for which, value in ((0, float("nan")), (1, float("nan")), (1, float("inf")), (0, float("inf"))):
@@ -391,10 +433,11 @@ def test_non_finite_queries_stay_in_their_rows(b200, ctx):
         assert torch.equal(got[same], clean[same]) and torch.isnan(got[0, 1, 2]).all()
 
 
-def test_attention_gives_the_same_bits_every_time(b200, ctx):
+@pytest.mark.parametrize("longest", [3000, 7000])
+def test_attention_gives_the_same_bits_every_time(b200, ctx, longest):
     import torch
 
-    p = Pool(b200, ctx, b200.Q8_0, 2, 128, 16, [3000, 1, 700, 2999], seed=11).fill()
+    p = Pool(b200, ctx, b200.Q8_0, 2, 128, 16, [longest, 1, 700, 2999], seed=11).fill()
     q = cu(p.rng.normal(0, 1, (4, 2, 8, 128)).astype(np.float32))
     first = ctx.kv_attention(p.cache, q, p.table, p.lens_t, 0.1)
     for _ in range(5):
@@ -427,11 +470,12 @@ def test_places_past_4_gib(b200, ctx):
 # ---- streams and graphs ------------------------------------------------------------------------------------------------
 
 
-def test_calls_run_on_torchs_current_stream(b200, ctx):
+@pytest.mark.parametrize("lens", [[4000, 3500], [6000, 5500]])  # by items; by positions, with a workspace
+def test_calls_run_on_torchs_current_stream(b200, ctx, lens):
     """Two streams at once, each with its own sequences of one pool: no call waits for or reads the other's workspace."""
     import torch
 
-    p = Pool(b200, ctx, b200.F16, 2, 128, 16, [4000, 3500], seed=13).fill()
+    p = Pool(b200, ctx, b200.F16, 2, 128, 16, lens, seed=13).fill()
     q = cu(p.rng.normal(0, 1, (2, 1, 8, 128)).astype(np.float32))
     want = [ctx.kv_attention(p.cache, q[i:i + 1], p.table[i:i + 1], p.lens_t[i:i + 1], 0.1) for i in (0, 1)]
     torch.cuda.synchronize()
@@ -455,13 +499,35 @@ def test_calls_run_on_torchs_current_stream(b200, ctx):
     assert torch.equal(out, want[0])
 
 
+def test_the_first_call_of_a_context_may_be_captured(b200):
+    import torch
+
+    for lens in ([300, 5], [6000, 5]):  # by items, by positions
+        fresh = b200.Context(0)
+        p = Pool(b200, fresh, b200.F16, 2, 64, 16, lens, seed=21)
+        n = max(lens)
+        k, v = (torch.randn(2, n, 2, 64, device="cuda") for _ in range(2))
+        q, out = torch.randn(2, 1, 4, 64, device="cuda"), torch.zeros(2, 1, 4, 64, device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            fresh.kv_write(p.cache, k, v, p.table, p.lens_t)
+            fresh.kv_attention(p.cache, q, p.table, p.lens_t, 0.2, out=out)
+        graph.replay()
+        assert torch.equal(out, fresh.kv_attention(p.cache, q, p.table, p.lens_t, 0.2)) and out.any()
+        fresh.synchronize()
+        del graph
+        fresh.close()
+
+
+@pytest.mark.parametrize("longest", [700, 5000])
 @pytest.mark.parametrize("qname", ["F16", "Q8_0"])
-def test_a_captured_step_replays_with_new_rows_and_lengths(b200, ctx, qname):
+def test_a_captured_step_replays_with_new_rows_and_lengths(b200, ctx, qname, longest):
     """Write and attention captured once, replayed while the sequences grow over page ends; two graphs replayed at once."""
     import torch
 
     page, steps = 16, 40
-    lens0 = [1, 10, 700]
+    lens0 = [1, 10, longest]
     p = Pool(b200, ctx, getattr(b200, qname), 2, 64, page, [n + steps for n in lens0], seed=14).fill()
     graphs = []
     for _ in range(2):
