@@ -454,7 +454,7 @@ class Context:
 
     def _arg(self, t, what, dtype, shape):
         """The address of a contiguous CUDA tensor of this device, type and shape."""
-        if not t.is_cuda or t.get_device() != self.device or t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        if t.get_device() != self.device or t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
             self._refuse(t, what, f"a contiguous {dtype} tensor of shape {tuple(shape)}")
         return t.data_ptr()
 
@@ -465,7 +465,7 @@ class Context:
 
         n_seq, n_tok, heads, dim = shape
         width = heads * dim
-        if t.dtype == torch.float32 and t.shape == shape and t.is_cuda and t.get_device() == self.device:
+        if t.dtype is torch.float32 and t.shape == shape and t.get_device() == self.device:
             if t.is_contiguous():
                 return t.data_ptr(), width
             s = t.stride()
@@ -489,10 +489,12 @@ class Context:
         """(table's address, its width, the lengths' address)."""
         import torch
 
-        if table.dim() != 2:
-            self._refuse(table, what + " table", "int32 [n_seq, max_pages]")
-        width = table.shape[1]
-        return self._arg(table, what, torch.int32, (n_seq, width)), width, self._arg(lens, what, torch.int32, (n_seq,))
+        i32, device, shape = torch.int32, self.device, table.shape
+        if (len(shape) == 2 and shape[0] == n_seq and table.dtype is i32 and table.get_device() == device and table.is_contiguous()
+                and lens.dtype is i32 and lens.shape == (n_seq,) and lens.get_device() == device and lens.is_contiguous()):
+            return table.data_ptr(), shape[1], lens.data_ptr()
+        self._arg(lens, what + " lens", i32, (n_seq,))
+        self._refuse(table, what + " table", f"a contiguous int32 tensor [{n_seq}, max_pages]")
 
     def kv_write(self, cache, k, v, table, lens):
         """Writes rows k, v float32 [n_seq, n_tok, n_kv_head, head_dim] at positions lens[s] - n_tok + r (b200_kv_write);
@@ -502,7 +504,7 @@ class Context:
         shape = (n_seq, n_tok, cache.n_kv_head, cache.head_dim)
         kp, ldk = self._row_arg(k, "kv_write k", shape)
         vp, ldv = self._row_arg(v, "kv_write v", shape)
-        tp, mp, lp = self._kv_places(table, lens, n_seq, "kv_write table and lens")
+        tp, mp, lp = self._kv_places(table, lens, n_seq, "kv_write")
         self.check(self.L.b200_kv_write(self.h, self._stream(), cache.ref, tp, mp, lp, n_seq, n_tok, kp, ldk, vp, ldv))
 
     def kv_read(self, cache, table, lens, n_tok=None, start=None, dtype=None, k=None, v=None):
@@ -528,7 +530,7 @@ class Context:
             raise ValueError(f"kv_read: rows are float32 or float16, not {kind}")
         kp, vp = self._arg(k, "kv_read k", kind, shape), self._arg(v, "kv_read v", kind, shape)
         sp = None if start is None else self._arg(start, "kv_read start", torch.int32, (n_seq,))
-        tp, mp, lp = self._kv_places(table, lens, n_seq, "kv_read table and lens")
+        tp, mp, lp = self._kv_places(table, lens, n_seq, "kv_read")
         self.check(self.L.b200_kv_read(self.h, self._stream(), cache.ref, tp, mp, lp, sp, n_seq, n_tok, F16 if kind == torch.float16 else F32, kp, vp))
         return k, v
 
@@ -543,7 +545,7 @@ class Context:
             raise ValueError(f"kv_attention: expected q [n_seq, n_tok, n_head, head_dim], got {tuple(shape)}")
         n_seq, n_tok, n_head = shape[:3]
         qp, ldq = self._row_arg(q, "kv_attention q", (n_seq, n_tok, n_head, cache.head_dim))
-        tp, mp, lp = self._kv_places(table, lens, n_seq, "kv_attention table and lens")
+        tp, mp, lp = self._kv_places(table, lens, n_seq, "kv_attention")
         if out is None:
             # empty_like takes half of empty's time; rows that lie apart (columns of a wider product) need a shape of their own
             out = torch.empty_like(q) if ldq == n_head * cache.head_dim and q.is_contiguous() else torch.empty(shape, dtype=torch.float32, device=q.device)
