@@ -343,7 +343,7 @@ int b200_graph_supports(const b200_tensor * tensors, int64_t n, int64_t i);
 /* ------------------------------------------------------------------------------------------------------------
  * Paged key/value cache: one layer's keys and values of many sequences in pages of one pool, written (and quantized)
  * row by row, read back, and attended to. The reference keeps one dense F16 cache per request
- * (src/common/qwen3-decoder.cpp:300-346) and attends to a view of it; this is the form for a program that serves many
+ * (src/common/qwen3-decoder.cpp:320-321) and attends to a view of it; this is the form for a program that serves many
  * requests with one set of weights: sequence s's position p lies in page table[s][p / page_size], slot p % page_size.
  *
  * Layout of the cache's memory, arrays in this order, each starting at a multiple of 256 bytes (field_off):

@@ -1,31 +1,41 @@
 // kv_attention.cu — attention of a few new tokens per sequence over the paged key/value cache (b200_kv_attention).
 //
 // Mathematics. The rows of one key/value head (its group of query heads, times the call's tokens) share every key and value,
-// so they are taken eight at a time: S = Q K^T and O = P V over 16 positions at a time, with a running maximum and sum per
-// row (o and l are rescaled by 2^(m_old - m_new) when a larger score appears; exponentials to base 2, their scale folded into
-// the scores'). Bytes decide: a position costs 4 D bytes (F16) or 2.125 D (Q8_0) of HBM and 4 D multiply-adds per row, so
-// the arithmetic has to cost next to nothing beside the stream of the cache.
+// so they are taken eight (or twice eight) at a time: S = Q K^T and O = P V over 16 positions at a time, with a running maximum
+// and sum per row (o and l are rescaled by 2^(m_old - m_new) when a larger score appears; exponentials to base 2, their scale
+// folded into the scores'). Bytes decide: a position costs 4 D bytes (F16) or 2.125 D (Q8_0) of HBM and 4 D multiply-adds
+// per row, so the arithmetic has to cost next to nothing beside the stream of the cache.
 //
 // Float32 results from F16 matrix instructions. mma.m16n8k16 multiplies F16 exactly and adds in float32, but takes 16 rows
 // where there are at most eight: rows 0-7 of the tile hold the high half of the operand and rows 8-15 the low half (x = hi +
 // lo in F16, 22 bits; q scaled by a power of two per row first), and the two results of a row lie in the same lane's
 // registers, where one addition joins them. So q and the weights enter with 22 bits at the price of the padding. Q8_0's
 // values are whole numbers and exact in F16; their scales stay outside: a key block's multiplies its partial score, a value
-// block's multiplies the weight before it is split (times a power of two per 16 positions that keeps it in F16's range).
-// Each instruction's sum starts at zero and is added to the float32 result with an ordinary rounded addition (the
-// instruction's own accumulation truncates, which over thousands of positions would add up).
+// block's multiplies the weight's two halves. An instruction's own accumulation truncates, which over thousands of positions
+// would add up: at most two are chained, and their sum is added to the float32 result with a rounded addition. (Errors
+// against 64 bits: 2e-7 to 4e-7 of the result, a plain float32 computation's being 4e-7 to 2e-6.)
 //
-// Operands without shared memory. The k index of S = Q K^T may run through a row's dimensions in any order that both operands
-// share, and the n index of O = P V through any order that the output is written back in. They are chosen such that a lane's
-// fragment is 16 (F16 keys and values), 8 or 4 (Q8_0) contiguous bytes of a row: keys and values go from HBM to the matrix
-// instruction's registers with wide loads that use every byte of each sector, and the scores' registers are the weights'
-// fragment as they stand.
+// Operands. The k index of S = Q K^T may run through a row's dimensions in any order that both operands share, and the n index
+// of O = P V through any order that the output is written back in. They are chosen such that a lane's fragment is 16 (F16
+// keys and values), 8 or 4 (Q8_0) contiguous bytes of a row, read from shared memory without bank conflicts (the 16-byte chunks
+// are swizzled as they are copied), and the scores' registers are the weights' fragment as they stand. Each warp copies its own
+// pieces of 16 positions into its own ring with cp.async, one or more ahead, so no warp waits for another before the end.
+// (Fragments loaded from HBM straight into registers need no copies, but what a warp has under way is then bound by its
+// registers: at its best that form took 105 us for F16 and 168 us for Q8_0, below; the ring took 103 and 142 us at once.)
 //
-// Split. Sequences differ in length and there may be one of them, so the work is cut by positions: all (sequence, key/value
-// head, row tile) items laid end to end in chunks of 64 positions, and each CTA takes an equal run of chunks. A CTA's four
-// warps take turns at 16-position tiles of a run and join at its end. Items that lie within one CTA's run are finished by it;
-// of the others each CTA leaves a partial (m, l, o) in the workspace, and a second kernel, launched with programmatic
-// dependent launch, joins them.
+// Split. Sequences differ in length and there may be one of them. By positions: all (sequence, key/value head, row tile)
+// items are laid end to end in chunks of 64 positions, and each CTA takes an equal run of chunks; a CTA's four warps take
+// turns at a run's pieces and join at its end. Items that lie within one CTA's run are finished by it; of the others each CTA
+// leaves a partial (m, l, o) in the workspace, and a second kernel, launched with programmatic dependent launch, joins them.
+// By items, where a table allows short sequences only: a cluster per item, joined over distributed shared memory, in one
+// launch (geometry() has the rule and both sides' times).
+//
+// Measured on one B200, device time (a CUDA graph of calls on the same inputs), 16 heads on 8 of 128 unless said otherwise: 64
+// sequences of 512 to 4096 positions over F16 (612 MB) 104 us, 5.9 TB/s, bound by HBM; 32 of 2048 to 16384 over Q8_0 (658 MB)
+// 128 us, 5.1 TB/s, bound by the instructions that turn bytes into F16 and scale them (ALU pipe 48 % busy, matrix pipe 30 %,
+// some 490 instructions per 16 positions; on inputs that change from call to call, under the power limit, 147 us); one of
+// 131071 positions over Q8_0, 32 heads on 4, 41 us; one of 517 over F16 6.2 us, a chain of latencies: length, page number,
+// rows, two or three pieces, the cluster's join.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -39,10 +49,10 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kJoinWarps = 8;
-constexpr int kChunk = 64;    // positions of a chunk: one 16-position tile per warp
+constexpr int kChunk = 64;       // positions of a chunk: one piece per warp
 constexpr int kItemChunks = 16;  // the work is cut by items up to this many chunks per CTA,
 constexpr int kItemMost = 64;    // and this many per sequence
-constexpr float kShift = 14;  // weights are held times 2^14, so that their low halves reach 2^-38 of the largest
+constexpr float kShift = 14;     // weights are held times 2^14, so that their low halves reach 2^-38 of the largest
 
 struct Geometry {
     int n_tok, n_head, group;
@@ -137,8 +147,10 @@ struct Shape {
     static constexpr int kGroups = D / (8 * kRun);
     static constexpr int kKeyWords = Q8 ? 2 : 4;           // a lane's words of a row's 32 dimensions
     static constexpr int kValueWords = Q8 ? 1 : kRun / 2;  // a lane's words of a row's group
-    // A piece is 16 positions: its key rows, value rows, and their scales. A warp takes kSub pieces at a time, from a ring of
-    // kStages such in shared memory; the ring's depth and the CTAs per SM fill its 227 KB.
+    // A piece is 16 positions: its key rows, value rows, and their scales. A warp takes kSub pieces at a time (two of Q8_0 share
+    // the running maximum's and sum's arithmetic and one addition to o: 142 -> 134 us for the batch above), from a ring of
+    // kStages such in shared memory; the ring's depth and the CTAs per SM fill its 227 KB and the registers. (F16, D = 128: two
+    // CTAs with three stages 103 us, three with two 106 us. Q8_0, D = 128: three with two 131 us, two with three 134 us.)
     static constexpr int kSub = Q8 && D <= 128 ? 2 : 1;
     static constexpr int kRowBytes = Q8 ? D : 2 * D;
     static constexpr int kScaleBytes = Q8 ? D / 16 : 0;    // of a row

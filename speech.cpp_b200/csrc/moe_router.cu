@@ -10,7 +10,9 @@
 //    wider than that. Where neighbours are closer (some rows in a thousand) the few candidates are ordered by their scores in
 //    double; where groups are, or anything is not finite, the row is done again in double.
 // The weights of the chosen are double either way, one lane for each, of all the warp's rows at once. Reading the logits
-// takes 4 B per expert (2.7 us of HBM for 16384 rows of 256); the instructions decide the time.
+// takes 4 B per expert (2.7 us of HBM for 16384 rows of 256); the instructions decide the time. Measured on one B200, device
+// time: 16384 rows of 256, eight chosen, by logits 11 us, by sigmoid and bias 17 us, with four of eight groups kept 23 to 27 us
+// (in double throughout: 167 us); one row of 128 2.3 us, a launch.
 #include <cmath>
 
 #include "kv.cuh"
