@@ -249,6 +249,7 @@ class Context:
     """One B200 device, one stream, a scratch pool (b200_context)."""
 
     _raw_stream = None
+    _on_torchs = False  # calls have run on torch's current stream since the last synchronize()
 
     def __init__(self, device=0):
         self.L = lib()
@@ -274,6 +275,11 @@ class Context:
         return torch.cuda.ExternalStream(self.stream_handle, device=torch.device("cuda", self.device))
 
     def synchronize(self):
+        """Waits for the context's stream and, after calls that ran on torch's current stream, for that one; raises the first
+        error that a kernel recorded."""
+        if self._on_torchs:
+            self._sync_in()
+            self._on_torchs = False
         self.check(self.L.b200_synchronize(self.h))
 
     def close(self):
@@ -445,6 +451,7 @@ class Context:
 
             # the handle alone, where torch has it: a Stream object costs a microsecond more per call
             self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+        self._on_torchs = True
         return self._raw_stream(self.device) or 1
 
     def _refuse(self, t, what, wanted):

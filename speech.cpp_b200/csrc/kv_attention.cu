@@ -538,8 +538,8 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                     }
             }
             using Fragments = uint32_t[S::kTiles][S::kSub][4];
-            // one block of 32 dimensions: weights times scales (fragments a), times 2^k and back where `down` is not 1
-            auto block = [&](int b, const Fragments & a, auto scaled, float down) {
+            // one block of 32 dimensions: weights times scales (fragments a), which where `scaled` come times 1 / down
+            auto block = [&](int b, const Fragments & a, auto scaled, const float * down) {
                 uint32_t x[S::kSub][2][2];  // two rows' four bytes each, interleaved: (row, row + 1) pairs
 #pragma unroll
                 for (int u = 0; u < kSub; u++) {
@@ -564,7 +564,7 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
 #pragma unroll
                         for (int u = 1; u < kSub; u++) mma(r, a[y][u], f[u][0], f[u][1], r);
                         float2 part = __fadd2_rn(make_float2(r[0], r[1]), make_float2(r[2], r[3]));
-                        if constexpr (decltype(scaled)::value) part.x *= down, part.y *= down;
+                        if constexpr (decltype(scaled)::value) part.x *= down[y], part.y *= down[y];
                         o[y][b][n] = __ffma2_rn(o[y][b][n], keep[y], part);
                     }
                 }
@@ -597,40 +597,41 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                                     a[y][u][2 * i + 1] = u32(__hfma2(h2(pf[y][u][2 * i + 1]), d, __hfma2(hi, d, __hneg2(w))));
                                 }
                             }
-                        block(b, a, std::false_type{}, 1.0f);
+                        block(b, a, std::false_type{}, nullptr);
                     }
                 };
                 go(std::integral_constant<int, 0>{}), go(std::integral_constant<int, 1>{}), go(std::integral_constant<int, 2>{});
                 go(std::integral_constant<int, 3>{}), go(std::integral_constant<int, 4>{}), go(std::integral_constant<int, 5>{});
                 go(std::integral_constant<int, 6>{}), go(std::integral_constant<int, 7>{});
             } else {
-                // any scales: the product in float32, times a power of two that brings the step's largest scale below 1
+                // any scales: the product in float32, times a power of two that brings a row's largest to [2^13, 2^14)
 #pragma unroll
                 for (int b = 0; b < S::kBlocks; b++) {
-                    float d[kSub][4], big = 0.0f;
-#pragma unroll
-                    for (int u = 0; u < kSub; u++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            d[u][i] = half_of(vd[u][i >> 1], (i & 1) * S::kBlocks + b);
-                            big = fmaxf(big, fabsf(d[u][i]));
-                        }
-                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-                    int e = (int) (__float_as_uint(big) >> 23);
-                    if (e == 0 || e == 255) e = 126;
-                    const float up = __uint_as_float((uint32_t) (253 - e) << 23), down = __uint_as_float((uint32_t) (e + 1) << 23);
                     Fragments a;
+                    float down[TILES];
 #pragma unroll
-                    for (int y = 0; y < TILES; y++)
+                    for (int y = 0; y < TILES; y++) {
+                        float w[kSub][4], big = 0.0f;
+#pragma unroll
+                        for (int u = 0; u < kSub; u++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                const float d = half_of(vd[u][i >> 1], (i & 1) * S::kBlocks + b);
+                                w[u][i] = edge && s[y][u][i] == 0.0f ? 0.0f : s[y][u][i] * d;
+                                big = fmaxf(big, fabsf(w[u][i]));
+                            }
+                        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                        const int e = (int) (__float_as_uint(big) >> 23);
+                        const int k = e == 255 ? 0 : min(140 - e, 126);  // at least -114
+                        const float up = __uint_as_float((uint32_t) (127 + k) << 23);
+                        down[y] = __uint_as_float((uint32_t) (127 - k) << 23);
 #pragma unroll
                         for (int u = 0; u < kSub; u++) {
-                            float w[4];
-#pragma unroll
-                            for (int i = 0; i < 4; i++) w[i] = edge && s[y][u][i] == 0.0f ? 0.0f : s[y][u][i] * (d[u][i] * up);
-                            split(w[0], w[1], a[y][u][0], a[y][u][1]);
-                            split(w[2], w[3], a[y][u][2], a[y][u][3]);
+                            split(w[u][0] * up, w[u][1] * up, a[y][u][0], a[y][u][1]);
+                            split(w[u][2] * up, w[u][3] * up, a[y][u][2], a[y][u][3]);
                         }
+                    }
                     block(b, a, std::true_type{}, down);
                 }
             }

@@ -398,6 +398,20 @@ def test_attention_with_scores_far_apart(b200, ctx, qname):
     p.check_attention(4, 1, q=q)  # the mean of the values
 
 
+@pytest.mark.parametrize("n_tok", [1, 3])
+def test_values_that_a_weight_all_but_leaves_out(b200, ctx, n_tok):
+    """In one piece of the cache lie values of 1e6 whose weights are some e^-40 and values of 1e-4 whose weights are most of
+    the sum; in another the scales are 0."""
+    p = Pool(b200, ctx, b200.Q8_0, 2, 128, 16, [90], seed=22)
+    k = p.rng.normal(0, 0.1, (1, 90, 2, 128)).astype(np.float32)
+    v = (p.rng.normal(0, 1, (1, 90, 2, 128)) * 1e-4).astype(np.float32)
+    k[:, ::7], v[:, ::7] = -1.0, v[:, ::7] * 1e10
+    v[:, 30:41] = 0.0
+    ctx.kv_write(p.cache, cu(k), cu(v), p.table, p.lens_t)
+    q = np.ones((1, n_tok, 4, 128), np.float32)
+    p.check_attention(4, n_tok, scale=0.3125, q=q)  # scores of -40 beside +-0.35
+
+
 @pytest.mark.parametrize("width", [None, 300])
 def test_attention_does_not_see_what_lies_behind_a_row(b200, ctx, width):
     """Positions that later rows of the call see, but an earlier one does not, hold NaN and infinities: the earlier rows
