@@ -277,7 +277,8 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
     constexpr bool Q8 = S::kQ8;
     constexpr int D = S::kDim, TILES = S::kTiles;
     constexpr int kRowBytes = S::kRowBytes, kValues = 16 * kRowBytes, kKeyScales = 32 * kRowBytes, kValueScales = kKeyScales + 16 * S::kScaleBytes;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // so that the compiler knows it is one for the warp
     const int gq = lane >> 2, t = lane & 3;  // the fragment's group and thread in it
     Row row[TILES];
 #pragma unroll
@@ -313,8 +314,9 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
     // where this lane's first 16 bytes of a piece go: row lane / (chunks of a row), chunk lane % (chunks of a row)
     const uint32_t copy_key = lane * 16 ^ S::key_swizzle(lane / (kRowBytes / 16)) * 16;
     const uint32_t copy_value = lane * 16 ^ S::value_swizzle(lane / (kRowBytes / 16)) * 16;
-    unsigned found = 0;  // bit kSub stage + u: the piece has a page
+    unsigned found = 0;  // of the steps copied, the last in the lowest kSub bits: which pieces have a page
     auto copy_step = [&] {
+        found <<= kSub;
         if (p_copy < p_end) {
 #pragma unroll
             for (int u = 0; u < kSub; u++) {
@@ -352,8 +354,7 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                 if constexpr (Q8) {  // whole, rows behind the end too: they lie in the page
                     if (lane < 2 * S::kScaleBytes) copy16(to + kKeyScales + lane * 16, scales + at / 16, exists);
                 }
-                const unsigned bit = 1u << (kSub * stage_copy + u);
-                found = exists ? found | bit : found & ~bit;
+                if (exists) found |= 1u << u;
             }
             p_copy += kStep;
             in_table += page_step;
@@ -406,6 +407,7 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
     const uint32_t key_at = gq * kRowBytes + ((t * (Q8 ? 8 : 16)) ^ (S::key_swizzle(gq) * 16));
     const uint32_t value_at = kValues + 2 * t * kRowBytes + ((gq * S::kRun * (Q8 ? 1 : 2)) ^ (S::value_swizzle(2 * t) * 16));
 
+    const int plain_end = min(p_end, all_see);  // steps that end here or before have all their positions, seen by every row
     float2 o[TILES][S::kGroups][S::kRun] = {};
     float m[TILES], l[TILES];
 #pragma unroll
@@ -415,13 +417,9 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
         asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
         __syncwarp();  // the step is here for every lane, and every lane is done with the one before, whose place is refilled
         const uint32_t at = ring + stage * S::kStage;
-        int here[kSub];  // positions of the pieces
-        bool edge = p0 + 16 * kSub > all_see;
-#pragma unroll
-        for (int u = 0; u < kSub; u++) {
-            here[u] = found >> (kSub * stage + u) & 1 ? p_end - p0 - 16 * u : 0;
-            edge = edge || here[u] < 16;
-        }
+        const unsigned pages_here = found >> (kSub * (S::kStages - 2)) & ((1u << kSub) - 1);
+        const bool edge = p0 + 16 * kSub > plain_end || pages_here != (1u << kSub) - 1;
+        auto here = [&](int u) { return pages_here >> u & 1 ? p_end - p0 - 16 * u : 0; };  // positions of a piece
         stage = stage + 1 == S::kStages ? 0 : stage + 1;
         copy_step();
 
@@ -480,7 +478,7 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int j = 2 * t + (i & 1) + 8 * (i >> 1);
-                        if (j >= here[u] || p0 + 16 * u + j >= seen[y]) s[y][u][i] = -INFINITY;
+                        if (j >= here(u) || p0 + 16 * u + j >= seen[y]) s[y][u][i] = -INFINITY;
                     }
         }
 
@@ -528,7 +526,7 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                 for (int u = 0; u < kSub; u++)
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        const uint32_t a = 2 * t + 8 * i < here[u] ? 0 : 0x3c00, b = 2 * t + 1 + 8 * i < here[u] ? 0 : 0x3c00;
+                        const uint32_t a = 2 * t + 8 * i < here(u) ? 0 : 0x3c00, b = 2 * t + 1 + 8 * i < here(u) ? 0 : 0x3c00;
 #pragma unroll
                         for (int n = 0; n < S::kBlocks; n++) {  // halves 2 n and 2 n + 1: the first kBlocks are row 2 t's
                             const uint32_t low = 2 * n < S::kBlocks ? a : b, high = 2 * n + 1 < S::kBlocks ? a : b;
