@@ -72,6 +72,9 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+template <class T>
+__device__ __forceinline__ T first_lane(T x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 // d = A B + c, and d = A B.
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
@@ -278,7 +281,10 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
     constexpr int D = S::kDim, TILES = S::kTiles;
     constexpr int kRowBytes = S::kRowBytes, kValues = 16 * kRowBytes, kKeyScales = 32 * kRowBytes, kValueScales = kKeyScales + 16 * S::kScaleBytes;
     const int tid = threadIdx.x, lane = tid & 31;
-    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // so that the compiler knows it is one for the warp
+    // What is the same for a whole warp comes from its first lane, so that the compiler knows it and computes with it once.
+    const int warp = first_lane(tid >> 5);
+    seq = first_lane(seq), len = first_lane(len), c0 = first_lane(c0), c1 = first_lane(c1);
+    h = first_lane(h), tile = first_lane(tile);
     const int gq = lane >> 2, t = lane & 3;  // the fragment's group and thread in it
     Row row[TILES];
 #pragma unroll
@@ -320,11 +326,12 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
         if (p_copy < p_end) {
 #pragma unroll
             for (int u = 0; u < kSub; u++) {
-                const bool exists = (unsigned) page[u] < (unsigned) c.n_pages;
+                const unsigned number = (unsigned) first_lane(page[u]);
+                const bool exists = number < (unsigned) c.n_pages;
                 const int here = exists ? p_end - p_copy - 16 * u : 0;  // rows of the piece; the others are zeros
                 if (!exists && p_copy + 16 * u < p_end && lane == 0) atomicOr(c.err, B200_DEVERR_PAGE);
                 const int in_page = slot + 16 * u - (slot + 16 * u >= c.page_size ? c.page_size : 0);
-                const int64_t at = (int64_t) ((uint64_t) (exists ? page[u] : 0) * page_units << 9) + in_page * kRowBytes;
+                const int64_t at = (int64_t) ((uint64_t) (exists ? number : 0) * page_units << 9) + in_page * kRowBytes;
                 const uint8_t * from = kh + at;
                 const uint32_t to = ring + stage_copy * S::kStage + u * S::kPiece;
                 constexpr int kRowChunks = kRowBytes / 16, kCopies = kRowChunks / 2;  // a piece's rows are contiguous: 16 kRowChunks chunks
