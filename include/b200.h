@@ -402,8 +402,8 @@ b200_status b200_kv_read(b200_context * ctx, void * stream, const b200_kv_cache 
  * contiguous in it; out float32 [n_seq][n_tok][n_head][head_dim]. Rows with no position to see (or whose scores are all
  * -infinity) become zeros; what the cache holds past a row's last position does not reach it, NaN and infinities included.
  * Unlike B200_OP_FLASH_ATTN (which rounds q to F16 as ggml does), q and the weights enter with 22 bits and sums are float32;
- * weights below 2^-38 of a row's largest count as 0. A row that sees a key or value that is not finite is not finite. workspace:
- * device memory of b200_kv_attention_workspace bytes (256-byte aligned, contents arbitrary; NULL when that is 0), in use
+ * weights below 2^-38 of a row's largest count as 0 in front of their values. A key or value that is not finite can make
+ * every row that sees it NaN. workspace: device memory of b200_kv_attention_workspace bytes (256-byte aligned, contents arbitrary; NULL when that is 0), in use
  * until the call's work is done: calls that may overlap on the GPU need one each. */
 size_t b200_kv_attention_workspace(b200_context * ctx, const b200_kv_cache * cache, int64_t max_pages, int64_t n_seq, int64_t n_tok,
                                    int64_t n_head);
