@@ -359,7 +359,7 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                 if (here >= 16) each(std::true_type{});
                 else each(std::false_type{});
                 if constexpr (Q8) {  // whole, rows behind the end too: they lie in the page
-                    if (lane < 2 * S::kScaleBytes) copy16(to + kKeyScales + lane * 16, scales + at / 16, exists);
+                    if (lane < 2 * S::kScaleBytes) copy16(to + kKeyScales + lane * 16, scales + (at >> 4), exists);
                 }
                 if (exists) found |= 1u << u;
             }

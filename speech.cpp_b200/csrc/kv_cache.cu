@@ -91,7 +91,7 @@ struct RowSplit {
     int64_t rows;
 };
 
-constexpr int kUnroll = 4;  // four-value pieces of a row that a thread has in flight
+constexpr int kUnroll = 2;  // steps of a row that a thread has in flight, each four values of k and four of v
 
 // The row of this thread (-1: none) and its place among the row's threads, a multiple of 32 to the warp.
 __device__ __forceinline__ int64_t my_row(const RowSplit & p, int & i0) {
@@ -99,6 +99,35 @@ __device__ __forceinline__ int64_t my_row(const RowSplit & p, int & i0) {
     i0 = threadIdx.x % p.per_row;
     return row < p.rows ? row : -1;
 }
+
+// A thread's way through a row of n_kv_head heads of Q = head_dim / 4 quads (four values), `per_row` quads further each step.
+template <int Q>
+struct Walk {
+    int i, h, q, step, step_h, step_q;  // quad i of the row: quad q of head h
+    __device__ __forceinline__ Walk(int i0, int per_row) : i(i0), h(i0 / Q), q(i0 % Q), step(per_row), step_h(per_row / Q), step_q(per_row % Q) {}
+    __device__ __forceinline__ void next() {
+        i += step;
+        h += step_h;
+        q += step_q;
+        if (q >= Q) q -= Q, h++;
+    }
+};
+
+// Where a row lies: its first head's bytes in k and v and in the scales, and what each head further adds.
+template <bool Q8, int D>
+struct RowPlace {
+    int64_t at, scale_at;
+    int head, scale_head;
+    __device__ __forceinline__ RowPlace(const KvView & c, int page, int64_t pos) {
+        const int64_t row = (int64_t) page * c.n_kv_head * c.page_size + pos % c.page_size;
+        at = row * (Q8 ? D : 2 * D);
+        head = c.page_size * (Q8 ? D : 2 * D);
+        scale_at = row * (D / 32);
+        scale_head = c.page_size * (D / 32);
+    }
+    __device__ __forceinline__ int64_t quad(int h, int q) const { return at + (int64_t) h * head + q * (Q8 ? 4 : 8); }
+    __device__ __forceinline__ int64_t scale(int h, int q) const { return scale_at + (int64_t) h * scale_head + (q >> 3); }
+};
 
 // Row (s, r) of k and v to its slot. Q8_0: eight lanes hold a block's 32 values (quantize_q8_0_quad), so the warp's lanes
 // all take part in every step, those past the row's end on its last values without storing.
@@ -113,38 +142,76 @@ __global__ void __launch_bounds__(512) kv_write_kernel(KvView c, RowSplit p, int
     if (pos < 0) return;
     const int page = kv_page(c, s, pos / c.page_size, i0 == 0);
     if (page < 0) return;
-    const int64_t at0 = (int64_t) page * c.n_kv_head * c.page_size + pos % c.page_size;  // head 0's row in the arrays
-    const int quads = c.n_kv_head * (D / 4);  // of k, and of v
+    const RowPlace<Q8, D> place(c, page, pos);
+    const int quads = c.n_kv_head * (D / 4);
     const float * kr = k + row * ldk, * vr = v + row * ldv;
-    for (int j0 = i0; (j0 & ~31) < 2 * quads; j0 += kUnroll * p.per_row) {
-        float4 x[kUnroll];
+    uint8_t * to_k = const_cast<uint8_t *>(c.k), * to_v = const_cast<uint8_t *>(c.v);
+    __half * to_kd = const_cast<__half *>(c.kd), * to_vd = const_cast<__half *>(c.vd);
+    for (Walk<D / 4> w(i0, p.per_row); (w.i & ~31) < quads;) {
+        float4 xk[kUnroll], xv[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; u++) {
-            const int j = j0 + u * p.per_row, i = j < 2 * quads ? j : 2 * quads - 1;
-            if ((j & ~31) >= 2 * quads) break;  // the whole warp
-            x[u] = load4<VEC>(i >= quads ? vr + (i - quads) * 4 : kr + i * 4);
+            const int i = min(w.i + u * w.step, quads - 1);
+            if (u > 0 && ((w.i + u * w.step) & ~31) >= quads) break;  // the whole warp
+            xk[u] = load4<VEC>(kr + i * 4);
+            xv[u] = load4<VEC>(vr + i * 4);
         }
 #pragma unroll
         for (int u = 0; u < kUnroll; u++) {
-            const int j = j0 + u * p.per_row;
-            if ((j & ~31) >= 2 * quads) break;
-            const bool here = j < 2 * quads;
-            const int i = here ? j : 2 * quads - 1;
-            const bool is_v = i >= quads;
-            const int e = (is_v ? i - quads : i) * 4, h = e / D, d = e % D;
-            const int64_t at = at0 + (int64_t) h * c.page_size;
-            uint8_t * to = const_cast<uint8_t *>(is_v ? c.v : c.k);
+            if (u > 0 && (w.i & ~31) >= quads) break;
+            const bool here = w.i < quads;
             if constexpr (Q8) {
-                float df;
-                const uint32_t q = quantize_q8_0_quad(x[u], &df);
+                float dk, dv;
+                const uint32_t qk = quantize_q8_0_quad(xk[u], &dk), qv = quantize_q8_0_quad(xv[u], &dv);
                 if (here) {
-                    *reinterpret_cast<uint32_t *>(to + at * D + d) = q;
-                    if ((i & 7) == 0) const_cast<__half *>(is_v ? c.vd : c.kd)[at * (D / 32) + d / 32] = __float2half_rn(df);
+                    const int64_t at = place.quad(w.h, w.q);
+                    *reinterpret_cast<uint32_t *>(to_k + at) = qk;
+                    *reinterpret_cast<uint32_t *>(to_v + at) = qv;
+                    if ((w.q & 7) == 0) {
+                        const int64_t sc = place.scale(w.h, w.q);
+                        to_kd[sc] = __float2half_rn(dk);
+                        to_vd[sc] = __float2half_rn(dv);
+                    }
                 }
             } else if (here) {
-                *reinterpret_cast<uint2 *>(to + (at * D + d) * 2) = pack4(x[u]);
+                const int64_t at = place.quad(w.h, w.q);
+                *reinterpret_cast<uint2 *>(to_k + at) = pack4(xk[u]);
+                *reinterpret_cast<uint2 *>(to_v + at) = pack4(xv[u]);
             }
+            w.next();
         }
+    }
+}
+
+// Four values of the cache as float32.
+template <bool Q8>
+__device__ __forceinline__ float4 widen(uint2 raw, __half scale) {
+    if constexpr (Q8) {
+        const char4 q = *reinterpret_cast<const char4 *>(&raw.x);
+        const float f = __half2float(scale);
+        return make_float4(__fmul_rn(f, (float) q.x), __fmul_rn(f, (float) q.y), __fmul_rn(f, (float) q.z), __fmul_rn(f, (float) q.w));
+    } else {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&raw.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&raw.y));
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+}
+
+// Four values to element o of an output.
+template <bool HALF, bool VEC>
+__device__ __forceinline__ void store4(void * out, int64_t o, float4 x) {
+    if constexpr (HALF) {
+        const uint2 w = pack4(x);
+        if constexpr (VEC) {
+            *reinterpret_cast<uint2 *>((__half *) out + o) = w;
+        } else {
+            uint16_t * to = (uint16_t *) out + o;
+            to[0] = (uint16_t) w.x, to[1] = (uint16_t) (w.x >> 16), to[2] = (uint16_t) w.y, to[3] = (uint16_t) (w.y >> 16);
+        }
+    } else if constexpr (VEC) {
+        *reinterpret_cast<float4 *>((float *) out + o) = x;
+    } else {
+        float * to = (float *) out + o;
+        to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
     }
 }
 
@@ -160,64 +227,43 @@ __global__ void __launch_bounds__(512) kv_read_kernel(KvView c, RowSplit p, cons
     if (pos < 0 || pos >= kv_len(c, s, i0 == 0)) return;
     const int page = kv_page(c, s, pos / c.page_size, i0 == 0);
     if (page < 0) return;
-    const int64_t at0 = (int64_t) page * c.n_kv_head * c.page_size + pos % c.page_size;
+    const RowPlace<Q8, D> place(c, page, pos);
     const int quads = c.n_kv_head * (D / 4);
-    for (int j0 = i0; j0 < 2 * quads; j0 += kUnroll * p.per_row) {
-        uint2 raw[kUnroll];
-        __half scale[kUnroll];
+    const int64_t out = row * 4 * quads;
+    for (Walk<D / 4> w(i0, p.per_row); w.i < quads;) {
+        uint2 rk[kUnroll], rv[kUnroll];
+        __half dk[kUnroll], dv[kUnroll];
+        const int i = w.i;
 #pragma unroll
         for (int u = 0; u < kUnroll; u++) {
-            const int i = j0 + u * p.per_row;
-            if (i >= 2 * quads) break;
-            const bool is_v = i >= quads;
-            const int e = (is_v ? i - quads : i) * 4, h = e / D, d = e % D;
-            const int64_t at = at0 + (int64_t) h * c.page_size;
-            const uint8_t * from = is_v ? c.v : c.k;
+            if (u > 0 && w.i >= quads) break;
+            const int64_t at = place.quad(w.h, w.q);
             if constexpr (Q8) {
-                raw[u].x = *reinterpret_cast<const uint32_t *>(from + at * D + d);
-                scale[u] = (is_v ? c.vd : c.kd)[at * (D / 32) + d / 32];
+                rk[u].x = *reinterpret_cast<const uint32_t *>(c.k + at);
+                rv[u].x = *reinterpret_cast<const uint32_t *>(c.v + at);
+                const int64_t sc = place.scale(w.h, w.q);
+                dk[u] = c.kd[sc];
+                dv[u] = c.vd[sc];
             } else {
-                raw[u] = *reinterpret_cast<const uint2 *>(from + (at * D + d) * 2);
+                rk[u] = *reinterpret_cast<const uint2 *>(c.k + at);
+                rv[u] = *reinterpret_cast<const uint2 *>(c.v + at);
             }
+            w.next();
         }
 #pragma unroll
         for (int u = 0; u < kUnroll; u++) {
-            const int i = j0 + u * p.per_row;
-            if (i >= 2 * quads) break;
-            float4 x;
-            if constexpr (Q8) {
-                const char4 q = *reinterpret_cast<const char4 *>(&raw[u].x);
-                const float f = __half2float(scale[u]);
-                x = make_float4(__fmul_rn(f, (float) q.x), __fmul_rn(f, (float) q.y), __fmul_rn(f, (float) q.z), __fmul_rn(f, (float) q.w));
-            } else {
-                const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&raw[u].x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&raw[u].y));
-                x = make_float4(a.x, a.y, b.x, b.y);
-            }
-            const int64_t o = row * 4 * quads + (i >= quads ? i - quads : i) * 4;
-            void * out = i >= quads ? v : k;
-            if constexpr (HALF) {
-                const uint2 w = pack4(x);
-                if constexpr (VEC) {
-                    *reinterpret_cast<uint2 *>((__half *) out + o) = w;
-                } else {
-                    uint16_t * to = (uint16_t *) out + o;
-                    to[0] = (uint16_t) w.x, to[1] = (uint16_t) (w.x >> 16), to[2] = (uint16_t) w.y, to[3] = (uint16_t) (w.y >> 16);
-                }
-            } else if constexpr (VEC) {
-                *reinterpret_cast<float4 *>((float *) out + o) = x;
-            } else {
-                float * to = (float *) out + o;
-                to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
-            }
+            if (u > 0 && i + u * w.step >= quads) break;
+            store4<HALF, VEC>(k, out + (i + u * w.step) * 4, widen<Q8>(rk[u], dk[u]));
+            store4<HALF, VEC>(v, out + (i + u * w.step) * 4, widen<Q8>(rv[u], dv[u]));
         }
     }
 }
 
-// Threads per row: a power of two from 32 to 512, at most one per four values of the row, such that all rows together come to
+// Threads per row: a power of two from 32 to 512, at most one per four values of k, such that all rows together come to
 // some 512 threads per SM. With more (2048 per SM) 1500 rows of 8 x 128 are written in 6.0 instead of 4.7 us and 1031 read in
 // 6.6 instead of 4.1: the threads' values are then not enough to keep their loads under way.
 RowSplit split_rows(const b200_context * ctx, const KvView & c, int64_t rows) {
-    const int64_t fill = (int64_t) ctx->num_sms * 512, most = c.n_kv_head * c.head_dim / 2;
+    const int64_t fill = (int64_t) ctx->num_sms * 512, most = c.n_kv_head * c.head_dim / 4;
     int n = 32;
     while (n < 512 && n < most && rows * n < fill) n *= 2;
     return {n, rows};
