@@ -48,7 +48,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kJoinWarps = 8;
+constexpr int kJoinWarps = 8;  // 2^3
 constexpr int kChunk = 64;       // positions of a chunk: one piece per warp
 constexpr int kItemChunks = 16;  // the work is cut by items up to this many chunks per CTA,
 constexpr int kItemMost = 64;    // and this many per sequence
@@ -62,6 +62,8 @@ struct Geometry {
     int64_t n_seq;
     int64_t ctas;                     // CTAs among which the chunks are divided, or
     int cluster;                      // CTAs that share an item (0: the work is cut by positions)
+    int64_t units;                    // what may have to be joined: items, or CTAs (each begins at most one item that others end)
+    int by_item, join_shift;          // which of the two; logarithm of the warps per row of the join
 };
 
 constexpr int64_t partial_floats(int D, int rows) { return (int64_t) rows * (D + 2); }  // o [rows][D], m [rows], l [rows]
@@ -191,30 +193,34 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
 // Where a CTA's share of the chunks lies: chunk numbers count the sequences' chunks one after the other, each `items` times.
 struct Place {
     int64_t at, end;     // the chunks [at, end) of all
-    int64_t seq, start;  // the sequence that chunk `at` lies in, and its first chunk (when at < end)
+    int64_t share;       // end - at, but for the last one
+    int64_t seq, start;  // the sequence that chunk `at` (LAST: the share's last one) lies in, and its first chunk (when at < end)
 };
 
-// Block-wide (every thread gets the result): the lengths are read kThreads at a time, summed for the share and scanned for
-// the sequence; up to kThreads of them stay in registers in between.
-__device__ __forceinline__ Place find_place(const KvView & c, const Geometry & g, int64_t * red) {
+// CTA b's place, block-wide (every thread gets the result): the lengths are read 32 WARPS at a time, summed for the share and
+// scanned for the sequence; up to that many of them stay in registers in between.
+template <int WARPS, bool LAST>
+__device__ __forceinline__ Place find_place(const KvView & c, const Geometry & g, int64_t b, bool tell, int64_t (&red)[WARPS + 2]) {
+    constexpr int kStep = 32 * WARPS;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t first = threadIdx.x < g.n_seq ? chunks_of(c, threadIdx.x, blockIdx.x == 0) * g.items : 0;
+    const int64_t first = threadIdx.x < g.n_seq ? chunks_of(c, threadIdx.x, tell) * g.items : 0;
     int64_t sum = first;
-    for (int64_t s = threadIdx.x + kThreads; s < g.n_seq; s += kThreads) sum += chunks_of(c, s, blockIdx.x == 0) * g.items;
+    for (int64_t s = threadIdx.x + kStep; s < g.n_seq; s += kStep) sum += chunks_of(c, s, tell) * g.items;
     sum = warp_sum64(sum);
     if (lane == 0) red[warp] = sum;
     __syncthreads();
     int64_t total = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; w++) total += red[w];
-    const int64_t share = (total + g.ctas - 1) / g.ctas;
+    for (int w = 0; w < WARPS; w++) total += red[w];
     Place p;
-    p.at = blockIdx.x * share;
-    p.end = p.at + share < total ? p.at + share : total;
+    p.share = (total + g.ctas - 1) / g.ctas;
+    p.at = b * p.share;
+    p.end = p.at + p.share < total ? p.at + p.share : total;
     p.seq = p.start = 0;
     if (p.at >= p.end) return p;  // the same for all threads
+    const int64_t to = LAST ? p.end - 1 : p.at;
     int64_t base = 0;
-    for (int64_t s0 = 0; s0 < g.n_seq; s0 += kThreads) {
+    for (int64_t s0 = 0; s0 < g.n_seq; s0 += kStep) {
         const int64_t s = s0 + threadIdx.x;
         const int64_t mine = s0 == 0 ? first : s < g.n_seq ? chunks_of(c, s, false) * g.items : 0;
         int64_t incl = mine;
@@ -228,21 +234,21 @@ __device__ __forceinline__ Place find_place(const KvView & c, const Geometry & g
         __syncthreads();
         int64_t before = base, all = 0;
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) {
+        for (int w = 0; w < WARPS; w++) {
             if (w < warp) before += red[w];
             all += red[w];
         }
         const int64_t begin = before + incl - mine;
-        if (mine > 0 && p.at >= begin && p.at < begin + mine) {
-            red[kWarps] = s;
-            red[kWarps + 1] = begin;
+        if (mine > 0 && to >= begin && to < begin + mine) {
+            red[WARPS] = s;
+            red[WARPS + 1] = begin;
         }
         base += all;
-        if (p.at < base) break;  // the same for all threads
+        if (to < base) break;  // the same for all threads
     }
     __syncthreads();
-    p.seq = red[kWarps];
-    p.start = red[kWarps + 1];
+    p.seq = red[WARPS];
+    p.start = red[WARPS + 1];
     return p;
 }
 
@@ -765,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, S::kCtas)
     const int tid = threadIdx.x;
     pdl_launch_dependents();
 
-    const Place place = find_place(c, g, red);
+    const Place place = find_place<kWarps, false>(c, g, blockIdx.x, blockIdx.x == 0, red);
     int64_t at = place.at, seq = place.seq, start = place.start;
     const int64_t end = place.end;
     if (at >= end) return;
@@ -846,55 +852,80 @@ __global__ void __launch_bounds__(kThreads, S::kCtas)
     group.sync();  // the others read this CTA's shared memory until here
 }
 
-// Joins the partials of items that several CTAs worked on, and writes the zeros of empty sequences. One CTA per row of an
-// item: a warp takes every kJoinWarps-th partial, a lane D / 32 dimensions, and the warps join in shared memory.
+// Joins the partials of the items that several CTAs worked on, and writes the zeros of empty sequences. A unit of work is an
+// item, or a CTA of the first kernel: the item that it begins and others end. A row has 2^join_shift warps (up to
+// kJoinWarps): each takes every so many-th partial, a lane D / 32 dimensions, and they join in shared memory.
 template <int D, int ROWS>
 __global__ void __launch_bounds__(32 * kJoinWarps) kv_attention_join_kernel(KvView c, Geometry g, float * __restrict__ out, const float * __restrict__ ws) {
-    __shared__ int64_t red[2 * kJoinWarps];
+    __shared__ int64_t red[kJoinWarps + 2], before[kJoinWarps];
     __shared__ float so[kJoinWarps][D], sm[kJoinWarps], sl[kJoinWarps];
-    const int i = blockIdx.x % ROWS, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t seq = blockIdx.x / ROWS / g.items, item = blockIdx.x / ROWS % g.items;
-    const Row mine = row_of<ROWS>(g, (int) (item / g.tiles), (int) (item % g.tiles), i);
-    if (!mine.there) return;
-    int64_t sums[2] = {0, 0};  // the chunks of an item in all sequences, and in those before this one
-    for (int64_t s = tid; s < g.n_seq; s += 32 * kJoinWarps) {
-        const int64_t n = chunks_of(c, s, false);
-        sums[0] += n;
-        if (s < seq) sums[1] += n;
-    }
-    sums[0] = warp_sum64(sums[0]);
-    sums[1] = warp_sum64(sums[1]);
-    if (lane == 0) {
-        red[2 * warp] = sums[0];
-        red[2 * warp + 1] = sums[1];
-    }
-    const int64_t chunks = chunks_of(c, seq, false);
-    __syncthreads();
-    int64_t total = 0, a = 0;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = 1 << g.join_shift;
+    const int parts_shift = (ROWS == 8 ? 0 : 1) + g.join_shift, part = (int) (blockIdx.x & ((1 << parts_shift) - 1));  // a unit's CTAs
+    const int i = part * (kJoinWarps >> g.join_shift) + (warp >> g.join_shift), sub = warp & (warps - 1);
+    const int64_t unit = blockIdx.x >> parts_shift;
+    int64_t seq, item;
+    int first = 0, last = 0;  // the CTAs that worked on it
+    auto zero = [&](int64_t s) {  // before the wait: only the kernels before the first one could still use these rows, and they ended
+        const int64_t n = (int64_t) g.n_tok * g.n_head * D;
+        for (int64_t d = tid; d < n; d += 32 * kJoinWarps) out[s * n + d] = 0.0f;
+    };
+    if (g.by_item) {
+        int64_t sums[2] = {0, 0};  // the chunks of an item in all sequences, and in those before this one
+        seq = unit / g.items;
+        item = unit % g.items;
+        for (int64_t s = tid; s < g.n_seq; s += 32 * kJoinWarps) {
+            const int64_t n = chunks_of(c, s, false);
+            sums[0] += n;
+            if (s < seq) sums[1] += n;
+        }
+        sums[0] = warp_sum64(sums[0]);
+        sums[1] = warp_sum64(sums[1]);
+        if (lane == 0) {
+            red[warp] = sums[0];
+            before[warp] = sums[1];
+        }
+        const int64_t chunks = chunks_of(c, seq, false);
+        __syncthreads();
+        int64_t total = 0, a = 0;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; w++) {
-        total += red[2 * w];
-        a += red[2 * w + 1];
+        for (int w = 0; w < kJoinWarps; w++) {
+            total += red[w];
+            a += before[w];
+        }
+        a = a * g.items + item * chunks;
+        const int64_t share = (total * g.items + g.ctas - 1) / g.ctas;
+        if (chunks > 0) {
+            first = (int) (a / share);
+            last = (int) ((a + chunks - 1) / share);
+        } else if (item == 0 && part == 0) {
+            zero(seq);
+        }
+    } else {
+        if (part == 0)
+            for (int64_t s = unit; s < g.n_seq; s += g.units)
+                if (kv_len(c, s, false) == 0) zero(s);
+        const Place p = find_place<kJoinWarps, true>(c, g, unit, false, red);
+        seq = p.seq;
+        item = 0;
+        if (p.at < p.end) {
+            const int64_t chunks = chunks_of(c, seq, false), a = p.end - 1 - (p.end - 1 - p.start) % chunks;
+            item = (a - p.start) / chunks;
+            if (a >= p.at && a + chunks > p.end) {
+                first = (int) unit;
+                last = (int) ((a + chunks - 1) / p.share);
+            }
+        }
     }
-    total *= g.items;
-    a = a * g.items + item * chunks;
-    float * to = out + ((seq * g.n_tok + mine.token) * g.n_head + mine.head) * D;
     pdl_wait();
-    if (chunks == 0) {
-        for (int d = tid; d < D; d += 32 * kJoinWarps) to[d] = 0.0f;
-        return;
-    }
-    const int64_t share = (total + g.ctas - 1) / g.ctas;
-    const int first = (int) (a / share), last = (int) ((a + chunks - 1) / share);
-    if (first == last) return;
+    if (first == last) return;  // the same for all threads
     constexpr int kStep = 4;  // partials of a warp in flight
     float v[D / 32] = {}, m = -INFINITY, l = 0.0f;
-    for (int k0 = first + warp; k0 <= last; k0 += kStep * kJoinWarps) {
+    for (int k0 = first + sub; k0 <= last; k0 += kStep * warps) {
         float pm[kStep], pl[kStep], po[kStep][D / 32];
 #pragma unroll
         for (int n = 0; n < kStep; n++) {
-            const int k = k0 + n * kJoinWarps;
-            const float * src = ws + (2 * k + (k == first ? 1 : 0)) * partial_floats(D, ROWS);
+            const int k = k0 + n * warps;
+            const float * src = ws + (2 * (int64_t) k + (k == first ? 1 : 0)) * partial_floats(D, ROWS);
             pm[n] = k <= last ? src[ROWS * D + i] : -INFINITY;
             pl[n] = k <= last ? src[ROWS * D + ROWS + i] : 0.0f;
 #pragma unroll
@@ -923,21 +954,29 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv_attention_join_kernel(KvVi
 #pragma unroll
     for (int d = 0; d < D / 32; d++) so[warp][lane + 32 * d] = v[d];
     __syncthreads();
+    const Row mine = row_of<ROWS>(g, (int) (item / g.tiles), (int) (item % g.tiles), i);
+    if (!mine.there) return;
     float top = -INFINITY;
+    bool in[kJoinWarps];  // the row's warps
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; w++) top = fmaxf(top, sm[w]);
+    for (int w = 0; w < kJoinWarps; w++) {
+        in[w] = w >> g.join_shift == warp >> g.join_shift;
+        if (in[w]) top = fmaxf(top, sm[w]);
+    }
     const float base = top == -INFINITY ? 0.0f : top;
     float f[kJoinWarps], sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < kJoinWarps; w++) {
         f[w] = ex2(sm[w] - base);
-        sum = fmaf(sl[w], f[w], sum);
+        if (in[w]) sum = fmaf(sl[w], f[w], sum);
     }
     const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-    for (int d = tid; d < D; d += 32 * kJoinWarps) {
+    float * to = out + ((seq * g.n_tok + mine.token) * g.n_head + mine.head) * D;
+    for (int d = 32 * sub + lane; d < D; d += 32 * warps) {
         float o = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; w++) o = fmaf(so[w][d], f[w], o);
+        for (int w = 0; w < kJoinWarps; w++)
+            if (in[w]) o = fmaf(so[w][d], f[w], o);
         to[d] = o * inv;
     }
 }
@@ -976,13 +1015,22 @@ Geometry geometry(const b200_context * ctx, const b200_kv_cache * c, int64_t max
     // By items when the lengths that the table allows are short: the cluster (1 to 8 CTAs) is the largest that all items fit
     // on the GPU with at once. One launch instead of two, and no scan of the lengths, against CTAs with equal work. Measured
     // (F16, 16 and 8 heads of 128, lengths from a quarter of the table's width to all of it), by items and by positions: 1
-    // sequence of 512: 5.6 and 6.4 us, 4096: 10.5 and 8.4 (where the second launch costs the host as much again); 8 sequences of
-    // 1024: 8.3 and 11.2, 4096: 18.3 and 18.2; 64 sequences of 1024: 33.6 and 41.0, 2048: 64.0 and 65.2.
+    // sequence of 512: 5.5 and 6.4 us, 4096: 10.1 and 8.4 (where the second launch costs the host as much again); 8 sequences of
+    // 1024: 8.1 and 11.3, 4096: 17.4 and 17.5; 64 sequences of 1024: 33.3 and 37.0, 2048: 55 and 61, but 47 and 20 (4096)
+    // when one of them is long and the others short.
     const int64_t most = (max_pages * c->page_size + kChunk - 1) / kChunk;  // chunks of the longest sequence there can be
     g.cluster = 8;
     while (g.cluster > 1 && n_seq * g.items * g.cluster > g.ctas) g.cluster /= 2;
     if (most > kItemChunks * g.cluster || most > kItemMost) g.cluster = 0;
     if (g.ctas > most * n_seq * g.items) g.ctas = most > 0 ? most * n_seq * g.items : 1;
+    // The join has a unit for whatever there are fewer of, and as many warps to a row as make two CTAs per SM: a row of
+    // many partials wants many warps (131071 positions, 4 heads: 41 us with eight, 56 with one), but their CTAs take time to
+    // start (64 sequences of 512 to 4096, F16: 99.6 us with one warp, 117 with eight). By items alone, 256 sequences of 256 to
+    // 2048 would take 198 instead of 193 us, five tokens each 239 instead of 228.
+    g.by_item = n_seq * g.items < g.ctas;
+    g.units = g.by_item ? n_seq * g.items : g.ctas;
+    g.join_shift = 3;
+    while (g.join_shift > 0 && g.units * g.rows << g.join_shift > (int64_t) kJoinWarps * 2 * ctx->num_sms) g.join_shift--;
     return g;
 }
 
@@ -1012,7 +1060,7 @@ cudaError_t launch(const KvView & c, const Geometry & g, const float * q, int64_
     kv_attention_kernel<S><<<(unsigned) g.ctas, kThreads, S::kBytes, st>>>(c, g, q, ldq, scale, out, ws);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    cfg.gridDim = dim3((unsigned) (g.n_seq * g.items * g.rows), 1, 1);
+    cfg.gridDim = dim3((unsigned) ((g.units * g.rows << g.join_shift) / kJoinWarps), 1, 1);
     cfg.blockDim = dim3(32 * kJoinWarps, 1, 1);
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;

@@ -374,6 +374,35 @@ def test_attention_of_many_sequences(b200, ctx):
     Pool(b200, ctx, b200.F16, 1, 64, 16, lens, seed=20).fill().check_attention(2, 1)
 
 
+@pytest.mark.parametrize("qname,D,Hkv,group,n_tok", [("F16", 64, 3, 2, 1), ("Q8_0", 128, 3, 4, 3), ("F16", 256, 2, 1, 2)])
+@pytest.mark.parametrize("where", [0, 131, 299])
+def test_attention_of_more_items_than_ctas(b200, ctx, qname, D, Hkv, group, n_tok, where):
+    """Many short sequences, empty ones among them, and a long one that many CTAs share: a CTA ends items that others began,
+    takes some whole, and begins at most one that others end."""
+    import torch
+
+    lens = np.random.default_rng(23).integers(0, 100, 300).tolist()
+    lens[7] = lens[298] = 0
+    lens[where] = 4500
+    p = Pool(b200, ctx, getattr(b200, qname), Hkv, D, 16, lens, seed=23)
+    short = p.rng.normal(0, 1, (2, 300, 100, Hkv, D)).astype(np.float32)
+    row = p.rng.normal(0, 1, (2, 1, 4500, Hkv, D)).astype(np.float32)
+    ctx.kv_write(p.cache, cu(short[0]), cu(short[1]), p.table, p.lens_t)
+    ctx.kv_write(p.cache, cu(row[0]), cu(row[1]), cu(p.table_np[where:where + 1]), cu(np.array([4500], np.int32)))
+    q = p.rng.normal(0, 1.5, (300, n_tok, group * Hkv, D)).astype(np.float32)
+    got = ctx.kv_attention(p.cache, cu(q), p.table, p.lens_t, D ** -0.5, out=torch.full(q.shape, float("nan"), device="cuda"))
+    ctx.synchronize()
+    f = [a.cpu().numpy() for a in p.f]
+    keys, values = [], []
+    for s, n in enumerate(lens):
+        at = (p.table_np[s, np.arange(n) // 16], slice(None), np.arange(n) % 16)
+        for which, rows in ((0, keys), (1, values)):
+            x = f[which][at].astype(np.float64)
+            rows.append(x * np.repeat(f[2 + which][at].astype(np.float64), 32, -1) if qname == "Q8_0" else x)
+    want, tol = ref.attention(q, keys, values, lens, D ** -0.5)
+    assert (np.abs(got.cpu().numpy() - want) <= tol).all()
+
+
 @pytest.mark.parametrize("qname", ["F16", "Q8_0"])
 @pytest.mark.parametrize("width", [1, 2, 300])
 def test_attention_whatever_the_tables_width(b200, ctx, qname, width):
