@@ -84,9 +84,11 @@ __device__ __noinline__ double softmax_sum(const RouterParams & a, const float *
     return warp_sum_d(sum);
 }
 
-// The experts of one row: lane k gets the k-th chosen. For rows that float32 does not decide.
+// The experts of one row: lane k gets the k-th chosen. For rows that float32 does not decide. kept: the groups that stay, if
+// these at least are known (else 0).
 template <int EPL>
-__device__ __noinline__ int choose_exactly(const RouterParams & a, const float * __restrict__ logits, const float * __restrict__ bias, float top) {
+__device__ __noinline__ int choose_exactly(const RouterParams & a, const float * __restrict__ logits, const float * __restrict__ bias, float top,
+                                           unsigned kept) {
     const int lane = threadIdx.x & 31;
     unsigned long long key[EPL];  // 0: past the last expert, in a group that is not kept, or chosen
     {
@@ -114,7 +116,7 @@ __device__ __noinline__ int choose_exactly(const RouterParams & a, const float *
             if (key[i] == best) at = i * 32 + lane;
         return (int) __reduce_min_sync(kAll, at);
     };
-    if (a.n_group > 1) {
+    if (a.n_group > 1 && !kept) {
         unsigned long long mine = 0;  // lane g: group g's score
         for (int g = 0; g < a.n_group; g++) {
             unsigned long long best = 0;
@@ -137,13 +139,14 @@ __device__ __noinline__ int choose_exactly(const RouterParams & a, const float *
             }
             if (lane == g) mine = key_of(score == score ? score : -(double) INFINITY);
         }
-        unsigned kept = 0;
         for (int n = 0; n < a.topk_group; n++) {
             const unsigned long long best = warp_largest(mine);
             const int g = __ffs(__ballot_sync(kAll, mine == best)) - 1;
             kept |= 1u << g;
             if (lane == g) mine = 0;
         }
+    }
+    if (a.n_group > 1) {
 #pragma unroll
         for (int i = 0; i < EPL; i++)
             if (!(kept >> group_of(a, i * 32 + lane) & 1)) key[i] = 0;
@@ -236,11 +239,54 @@ __device__ __noinline__ int order_exactly(const RouterParams & a, const float * 
     return id;
 }
 
+// The groups that stay (a bit each) by scores in double, from the experts whose float32 scores may be among a group's first
+// group_top: those not below lane g's `least`. 0 where they are more than 32. Of 16384 random rows of 256 about one
+// comes here; choose_exactly takes some 7 us for its groups, and the call would wait for that row.
+__device__ __noinline__ unsigned groups_exactly(const RouterParams & a, const float * __restrict__ logits, const float * __restrict__ bias, float top,
+                                                const float * scores, float least, int * list) {
+    const int lane = threadIdx.x & 31;
+    int n = 0;
+    for (int e0 = 0; e0 < a.E; e0 += 32) {
+        const int e = e0 + lane, g = e < a.E ? group_of(a, e) : 0;
+        const float from = __shfl_sync(kAll, least, g);
+        const bool in = e < a.E && scores[e + g * (a.pitch - a.size)] >= from;
+        const unsigned who = __ballot_sync(kAll, in);
+        const int at = n + __popc(who & ((1u << lane) - 1));
+        if (in && at < 32) list[at] = e;
+        n += __popc(who);
+    }
+    if (n > 32) return 0;
+    __syncwarp();
+    const double sum = a.score == B200_ROUTER_SOFTMAX ? softmax_sum(a, logits, top) : 1.0;
+    double c = 0.0;
+    int group = -1;
+    if (lane < n) {
+        const int e = list[lane];
+        group = group_of(a, e);
+        c = term(a, logits[e], top);
+        if (a.score == B200_ROUTER_SOFTMAX) c /= sum;
+        if (bias) c += (double) bias[e];
+    }
+    __syncwarp();
+    double b1 = -INFINITY, b2 = -INFINITY;  // lane g: group g's largest
+    for (int j = 0; j < n; j++) {
+        const double o = __shfl_sync(kAll, c, j);
+        if (__shfl_sync(kAll, group, j) == lane) {
+            if (o > b1) b2 = b1, b1 = o;
+            else if (o > b2) b2 = o;
+        }
+    }
+    const double score = a.group_top == 2 && a.size > 1 ? b1 + b2 : b1;
+    int ahead = 0;
+    for (int g = 0; g < a.n_group; g++) ahead += before(__shfl_sync(kAll, score, g), g, score, lane);
+    return __ballot_sync(kAll, lane < a.n_group && ahead < a.topk_group);
+}
+
 // EPL: experts per lane (a power of two). BY_LOGIT: no bias and no groups. FULL: there are 32 EPL experts.
 template <int EPL, bool BY_LOGIT, bool FULL>
 __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a, const float * __restrict__ logits, const float * __restrict__ bias,
                                                                  int64_t T, int32_t * __restrict__ ids, float * __restrict__ w) {
-    extern __shared__ float shared[];  // groups: each warp's scores, [n_group][pitch]
+    extern __shared__ float shared[];  // groups: each warp's scores, [n_group][pitch], and a list of 32 experts
     constexpr unsigned kIndex = EPL - 1;  // a key's low bits give way to the expert's place in its lane, the first ones largest
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t t0 = (blockIdx.x * (int64_t) kWarps + warp) * a.rows;
@@ -262,6 +308,7 @@ __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a,
         unsigned key[EPL];
         float off = 0.0f;  // bound on the error of a score
         bool sure = true;
+        unsigned stay = 0;  // the groups that stay, once they are sure
         if constexpr (BY_LOGIT) {
 #pragma unroll
             for (int i = 0; i < EPL; i++) key[i] = i < mine ? key_of(x[i]) : 0;
@@ -306,7 +353,7 @@ __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a,
             off += 0x1.1p-24f * far;
             if (sure && a.n_group > 1) {
                 const int size = a.size;
-                float * scores = shared + warp * a.n_group * a.pitch;
+                float * scores = shared + warp * (a.n_group * a.pitch + 32);
                 int of[EPL];
 #pragma unroll
                 for (int i = 0; i < EPL; i++) {
@@ -332,14 +379,22 @@ __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a,
                     ahead += other > s || (other == s && n < lane);
                 }
                 const bool in = lane < a.n_group && ahead < a.topk_group;
-                const unsigned kept = __ballot_sync(kAll, in);
+                unsigned kept = __ballot_sync(kAll, in);
                 if (a.topk_group < a.n_group) {
                     const float low = value_of(__reduce_min_sync(kAll, in ? key_of(s) : kAll));
                     const float high = value_of(__reduce_max_sync(kAll, lane < a.n_group && !in ? key_of(s) : 0));
                     sure = low - high > 4.0f * off + 0x1p-22f * fmaxf(fabsf(low), fabsf(high));
+                    if (!sure) {
+                        // a group's first experts have at least its last one's true score, so float32 scores two errors below
+                        const float last = a.group_top == 2 && size > 1 ? b2 : b1;
+                        const float least = __shfl_sync(kAll, last, lane < a.n_group ? lane << a.lane_shift : 0) - 4.0f * off;
+                        const unsigned exact = groups_exactly(a, row, bias, top, scores, least, (int *) (scores + a.n_group * a.pitch));
+                        if (exact) kept = exact, sure = true;
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < EPL; i++) key[i] = kept >> of[i] & 1 ? key[i] : 0;
+                if (sure) stay = kept;
             }
         }
         int chosen = 0;  // lane k: the k-th expert
@@ -389,7 +444,7 @@ __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a,
         }
         if (!sure) {
             if constexpr (BY_LOGIT) chosen = choose_by_logit<EPL>(a, row);
-            else chosen = choose_exactly<EPL>(a, row, bias, top);
+            else chosen = choose_exactly<EPL>(a, row, bias, top, stay);
         }
         chosen = __shfl_sync(kAll, chosen, lane - r * a.seats);
         const double total = !a.renorm && softmax ? softmax_sum(a, row, top) : 0.0;
@@ -456,7 +511,7 @@ extern "C" b200_status b200_moe_router(b200_context * ctx, void * stream, const 
         a.inv = ((1u << 21) + a.size - 1) / a.size;  // e * (inv * size - 2^21) < 2^10 2^10, so the quotient is exact
         while (2 * a.lanes * a.n_group <= 32) a.lanes *= 2, a.lane_shift++;
         a.pitch = a.size + (a.lanes - a.size % 32 + 32) % 32;  // pitch mod 32 = lanes: lane l of a step reads bank l + const
-        smem = (size_t) kWarps * a.n_group * a.pitch * sizeof(float);  // at most 4 * (1024 + 32 * 31) * 4 B < 32 KB
+        smem = (size_t) kWarps * (a.n_group * a.pitch + 32) * sizeof(float);  // at most 4 * (1024 + 32 * 31 + 32) * 4 B = 32 KB
     }
     cudaStream_t st = stream ? (cudaStream_t) stream : ctx->stream;
     const unsigned grid = (unsigned) ((T + kWarps * a.rows - 1) / (kWarps * a.rows));

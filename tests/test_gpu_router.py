@@ -103,6 +103,19 @@ def test_scores_that_float32_cannot_tell_apart(ctx, score):
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("n_group,size,group_top", [(8, 32, 2), (8, 32, 1), (4, 5, 2), (32, 1, 2), (16, 64, 2)])
+@pytest.mark.parametrize("steps", [1.0, 2.0 ** -22])
+def test_groups_that_float32_cannot_tell_apart(ctx, score, n_group, size, group_top, steps):
+    """Each group has the same logits in another order, and biases that only double precision sees: their sums decide between
+    the groups. With logits that are `steps` apart a few experts of each group count, or all of them."""
+    rng = np.random.default_rng(5)
+    base = (rng.normal(0, 1, (40, 1)) + np.arange(size) * steps).astype(np.float32)
+    logits = np.concatenate([base[:, rng.permutation(size)] for _ in range(n_group)], 1)
+    bias = (rng.integers(-200, 200, n_group * size) * 2.0 ** -40).astype(np.float32)
+    check(ctx, logits, min(4, n_group // 2 * size), bias, score=score, n_group=n_group, topk_group=n_group // 2, group_top=group_top)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("biased", [False, True])
 @pytest.mark.parametrize("groups", [{}, dict(n_group=4, topk_group=2, group_top=2)])
 def test_infinities_nan_and_the_types_ends(ctx, score, biased, groups):
