@@ -11,7 +11,7 @@
 //    double; where groups are, or anything is not finite, the row is done again in double.
 // The weights of the chosen are double either way, one lane for each, of all the warp's rows at once. Reading the logits
 // takes 4 B per expert (2.7 us of HBM for 16384 rows of 256); the instructions decide the time. Measured on one B200, device
-// time: 16384 rows of 256, eight chosen, by logits 11 us, by sigmoid and bias 17 us, with four of eight groups kept 23 to 27 us
+// time: 16384 rows of 256, eight chosen, by logits 11 us, by sigmoid and bias 17 us, with four of eight groups kept 21 to 23 us
 // (in double throughout: 167 us); one row of 128 2.3 us, a launch.
 #include <cmath>
 
@@ -284,8 +284,9 @@ __device__ __noinline__ unsigned groups_exactly(const RouterParams & a, const fl
 
 // EPL: experts per lane (a power of two). BY_LOGIT: no bias and no groups. FULL: there are 32 EPL experts.
 template <int EPL, bool BY_LOGIT, bool FULL>
-__global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(RouterParams a, const float * __restrict__ logits, const float * __restrict__ bias,
-                                                                 int64_t T, int32_t * __restrict__ ids, float * __restrict__ w) {
+__global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(const __grid_constant__ RouterParams a, const float * __restrict__ logits,
+                                                                 const float * __restrict__ bias, int64_t T, int32_t * __restrict__ ids,
+                                                                 float * __restrict__ w) {
     extern __shared__ float shared[];  // groups: each warp's scores, [n_group][pitch], and a list of 32 experts
     constexpr unsigned kIndex = EPL - 1;  // a key's low bits give way to the expert's place in its lane, the first ones largest
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
