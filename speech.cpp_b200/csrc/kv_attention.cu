@@ -21,7 +21,8 @@
 // are swizzled as they are copied), and the scores' registers are the weights' fragment as they stand. Each warp copies its own
 // pieces of 16 positions into its own ring with cp.async, one or more ahead, so no warp waits for another before the end.
 // (Fragments loaded from HBM straight into registers need no copies, but what a warp has under way is then bound by its
-// registers: at its best that form took 105 us for F16 and 168 us for Q8_0, below; the ring took 103 and 142 us at once.)
+// registers: at its best that form took 105 us for F16 and 168 us for Q8_0, below; the ring took 103 and 142 us at once and
+// was refined from there.)
 //
 // Split. Sequences differ in length and there may be one of them. By positions: all (sequence, key/value head, row tile)
 // items are laid end to end in chunks of 64 positions, and each CTA takes an equal run of chunks; a CTA's four warps take
@@ -31,11 +32,11 @@
 // launch (geometry() has the rule and both sides' times).
 //
 // Measured on one B200, device time (a CUDA graph of calls on the same inputs), 16 heads on 8 of 128 unless said otherwise: 64
-// sequences of 512 to 4096 positions over F16 (612 MB) 104 us, 5.9 TB/s, bound by HBM; 32 of 2048 to 16384 over Q8_0 (658 MB)
-// 128 us, 5.1 TB/s, bound by the instructions that turn bytes into F16 and scale them (ALU pipe 48 % busy, matrix pipe 30 %,
-// some 490 instructions per 16 positions; on inputs that change from call to call, under the power limit, 147 us); one of
-// 131071 positions over Q8_0, 32 heads on 4, 41 us; one of 517 over F16 6.2 us, a chain of latencies: length, page number,
-// rows, two or three pieces, the cluster's join.
+// sequences of 512 to 4096 positions over F16 (612 MB) 100 to 103 us, 6.0 TB/s, bound by HBM; 32 of 2048 to 16384 over Q8_0
+// (658 MB) 123 us, 5.3 TB/s, bound by the instructions that turn bytes into F16 and scale them (ALU pipe 46 % busy, matrix pipe
+// 31 %, issue slots 60 %, some 500 instructions per 16 positions; on inputs that change from call to call, under the power limit,
+// 137 to 147 us); one of 131071 positions over Q8_0, 32 heads on 4, 40 us; one of 517 over F16 6.0 us, a chain of latencies:
+// length, page number, rows, two or three pieces, the cluster's join.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -153,9 +154,10 @@ struct Shape {
     static constexpr int kKeyWords = Q8 ? 2 : 4;           // a lane's words of a row's 32 dimensions
     static constexpr int kValueWords = Q8 ? 1 : kRun / 2;  // a lane's words of a row's group
     // A piece is 16 positions: its key rows, value rows, and their scales. A warp takes kSub pieces at a time (two of Q8_0 share
-    // the running maximum's and sum's arithmetic and one addition to o: 142 -> 134 us for the batch above), from a ring of
+    // the running maximum's and sum's arithmetic and one addition to o: 125.6 -> 123.2 us for the batch above), from a ring of
     // kStages such in shared memory; the ring's depth and the CTAs per SM fill its 227 KB and the registers. (F16, D = 128: two
-    // CTAs with three stages 103 us, three with two 106 us. Q8_0, D = 128: three with two 131 us, two with three 134 us.)
+    // CTAs with three stages 104.2 us, three with two 105.1. Q8_0, D = 128: three with two 122.7 us, two with three 123.9, and
+    // 128 sequences of 1024 to 4096 169 and 174 us, but the one of 131071 40.8 and 38.2.)
     static constexpr int kSub = Q8 && D <= 128 ? 2 : 1;
     static constexpr int kRowBytes = Q8 ? D : 2 * D;
     static constexpr int kScaleBytes = Q8 ? D / 16 : 0;    // of a row

@@ -8,8 +8,8 @@
 // launch latency for the rows of a decode step. A row's length and page number are a chain of dependent loads before its
 // first value, so many rows have to be under way: a warp or more per row, its threads walking the row's k then v values four
 // at a time with four such pieces in flight. Measured on one B200, device time, 8 heads of 128: 24 x 4001 rows of Q8_0 read as
-// float32 120 us, 5.7 TB/s (one CTA per row: 334 us); 1500 rows written as F16 4.7 us; 64 rows written as Q8_0 and read back
-// 5.4 us, two launches' latency.
+// float32 111 us, 6.2 TB/s (one CTA per row: 334 us); 1500 rows written as F16 4.1 us; 64 rows written as Q8_0 and read back
+// 5.6 us, two launches' latency.
 #include <cstdio>
 
 #include "kv.cuh"
@@ -260,8 +260,8 @@ __global__ void __launch_bounds__(512) kv_read_kernel(KvView c, RowSplit p, cons
 }
 
 // Threads per row: a power of two from 32 to 512, at most one per four values of k, such that all rows together come to
-// some 512 threads per SM. With more (2048 per SM) 1500 rows of 8 x 128 are written in 6.0 instead of 4.7 us and 1031 read in
-// 6.6 instead of 4.1: the threads' values are then not enough to keep their loads under way.
+// some 512 threads per SM. With more (2048 per SM) 1500 rows of 8 x 128 are written in 5.4 instead of 4.1 us and 1031 read in
+// 4.2 instead of 3.5: the threads' values are then not enough to keep their loads under way.
 RowSplit split_rows(const b200_context * ctx, const KvView & c, int64_t rows) {
     const int64_t fill = (int64_t) ctx->num_sms * 512, most = c.n_kv_head * c.head_dim / 4;
     int n = 32;

@@ -7,8 +7,8 @@
 //  - without bias and groups the keys are the logits, and rows with equal truncated neighbours are done again with whole keys;
 //  - otherwise scores are computed in float32 first, with a bound on their error, and the row is accepted if every
 //    comparison that decides (neighbours among the chosen and the next one, the last group kept and the first one left) is
-//    wider than that. Where neighbours are closer (some rows in a thousand) the few candidates are ordered by their scores in
-//    double; where groups are, or anything is not finite, the row is done again in double.
+//    wider than that. Where neighbours are closer (some rows in a thousand), or groups, the few candidates are ordered by their
+//    scores in double; where they are many, two lanes' keys are equal or anything is not finite, the row is done again in double.
 // The weights of the chosen are double either way, one lane for each, of all the warp's rows at once. Reading the logits
 // takes 4 B per expert (2.7 us of HBM for 16384 rows of 256); the instructions decide the time. Measured on one B200, device
 // time: 16384 rows of 256, eight chosen, by logits 11 us, by sigmoid and bias 17 us, with four of eight groups kept 21 to 23 us
