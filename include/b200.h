@@ -403,8 +403,9 @@ b200_status b200_kv_read(b200_context * ctx, void * stream, const b200_kv_cache 
  * -infinity) become zeros; what the cache holds past a row's last position does not reach it, NaN and infinities included.
  * Unlike B200_OP_FLASH_ATTN (which rounds q to F16 as ggml does), q and the weights enter with 22 bits and sums are float32;
  * weights below 2^-38 of a row's largest count as 0 in front of their values. A key or value that is not finite can make
- * every row that sees it NaN. workspace: device memory of b200_kv_attention_workspace bytes (256-byte aligned, contents arbitrary; NULL when that is 0), in use
- * until the call's work is done: calls that may overlap on the GPU need one each. */
+ * every row that sees it NaN. workspace: device memory of b200_kv_attention_workspace bytes (256-byte aligned, contents
+ * arbitrary; NULL when that is 0), in use until the call's work is done: calls that may overlap on the GPU need one each.
+ * table and lens must not change before then either. */
 size_t b200_kv_attention_workspace(b200_context * ctx, const b200_kv_cache * cache, int64_t max_pages, int64_t n_seq, int64_t n_tok,
                                    int64_t n_head);
 b200_status b200_kv_attention(b200_context * ctx, void * stream, const b200_kv_cache * cache, const int32_t * table, int64_t max_pages,
@@ -420,8 +421,8 @@ b200_status b200_kv_attention(b200_context * ctx, void * stream, const b200_kv_c
  *   and only the topk_group best groups' experts stay;
  *   ids [T][top_k] = the top_k largest c, largest first; w [T][top_k] = their p, divided by their sum (renorm), times scale.
  * p, c and their sums are double, rounded to float32 once in w; without bias and groups the experts are ordered by their
- * logits. Ties go to the lowest index. A NaN logit or c counts as -infinity, a logit of -infinity has p = 0, +infinity shares the softmax with
- * its equals; a sum of 0 gives weights 0.
+ * logits. Ties go to the lowest index. A NaN logit or c counts as -infinity, a logit of -infinity has p = 0, +infinity
+ * shares the softmax with its equals; a sum of 0 gives weights 0.
  * ------------------------------------------------------------------------------------------------------------ */
 enum { B200_ROUTER_SOFTMAX = 0, B200_ROUTER_SIGMOID = 1 };
 typedef struct b200_router {

@@ -857,8 +857,9 @@ __global__ void __launch_bounds__(kThreads, S::kCtas)
 // Joins the partials of the items that several CTAs worked on, and writes the zeros of empty sequences. A unit of work is an
 // item, or a CTA of the first kernel: the item that it begins and others end. A row has 2^join_shift warps (up to
 // kJoinWarps): each takes every so many-th partial, a lane D / 32 dimensions, and they join in shared memory.
+// (ws is not __restrict__: the first kernel may still write it until pdl_wait, so its loads are not those of constants.)
 template <int D, int ROWS>
-__global__ void __launch_bounds__(32 * kJoinWarps) kv_attention_join_kernel(KvView c, Geometry g, float * __restrict__ out, const float * __restrict__ ws) {
+__global__ void __launch_bounds__(32 * kJoinWarps) kv_attention_join_kernel(KvView c, Geometry g, float * __restrict__ out, const float * ws) {
     __shared__ int64_t red[kJoinWarps + 2], before[kJoinWarps];
     __shared__ float so[kJoinWarps][D], sm[kJoinWarps], sl[kJoinWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = 1 << g.join_shift;

@@ -403,6 +403,29 @@ def test_attention_of_more_items_than_ctas(b200, ctx, qname, D, Hkv, group, n_to
     assert (np.abs(got.cpu().numpy() - want) <= tol).all()
 
 
+@pytest.mark.parametrize("n_seq", [3, 300])
+@pytest.mark.parametrize("one", [0, 1, 4500])
+def test_a_batch_of_empty_places(b200, ctx, n_seq, one):
+    """Nothing to attend to but one sequence's positions, or nothing at all: zeros for every other row."""
+    import torch
+
+    lens = [0] * n_seq
+    lens[1] = one
+    p = Pool(b200, ctx, b200.F16, 3, 64, 16, lens, seed=24, width=300)
+    if one:
+        row = p.rng.normal(0, 1, (2, 1, one, 3, 64)).astype(np.float32)
+        ctx.kv_write(p.cache, cu(row[0]), cu(row[1]), cu(p.table_np[1:2]), cu(np.array([one], np.int32)))
+    q = p.rng.normal(0, 1.5, (n_seq, 1, 6, 64)).astype(np.float32)
+    got = ctx.kv_attention(p.cache, cu(q), p.table, p.lens_t, 0.125, out=torch.full(q.shape, float("nan"), device="cuda"))
+    ctx.synchronize()
+    got = got.cpu().numpy()
+    assert not got[[s for s in range(n_seq) if lens[s] == 0]].any()
+    if one:
+        k, v = p.rows(1)
+        want, tol = ref.attention(q[1:2], [k], [v], [one], 0.125)
+        assert (np.abs(got[1:2] - want) <= tol).all()
+
+
 @pytest.mark.parametrize("qname", ["F16", "Q8_0"])
 @pytest.mark.parametrize("width", [1, 2, 300])
 def test_attention_whatever_the_tables_width(b200, ctx, qname, width):
