@@ -141,6 +141,16 @@ def test_infinities_nan_and_the_types_ends(ctx, score, biased, groups):
         check(ctx, logits, 8, bias, score=score, renorm=renorm, **groups)
 
 
+@pytest.mark.parametrize("T,E,k,score,groups", [
+    (5003, 64, 4, "sigmoid", dict(n_group=8, topk_group=3, group_top=2)), (20001, 16, 1, "softmax", {}), (9000, 40, 3, "softmax", dict(n_group=5, topk_group=2)),
+    (2369, 32, 20, "sigmoid", {}),
+])
+def test_any_number_of_rows_per_warp(ctx, T, E, k, score, groups):
+    """A warp takes 1 to 32 / (a power of two from k) rows: three of eight, nine of 32, four of eight, one of one."""
+    rng = np.random.default_rng(T)
+    check(ctx, rng.normal(0, 2, (T, E)).astype(np.float32), k, rng.normal(0, 0.1, E).astype(np.float32), score=score, **groups)
+
+
 def test_many_rows_and_a_captured_call(ctx):
     import torch
 
