@@ -507,7 +507,7 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
             for (int u = 0; u < kSub; u++) top = fmaxf(top, fmaxf(fmaxf(s[y][u][0], s[y][u][1]), fmaxf(s[y][u][2], s[y][u][3])));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float m_new = fmaxf(m[y], top - kShift);
+            const float m_new = fmaxf(m[y], __fadd_ru(top, -kShift));  // rounded down, top - m could pass 14 where floats are 4 apart
             const float base = m_new == -INFINITY ? 0.0f : m_new;
             const float k = ex2(m[y] - base);
             keep[y] = make_float2(k, k);

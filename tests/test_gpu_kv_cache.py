@@ -450,6 +450,27 @@ def test_attention_with_scores_far_apart(b200, ctx, qname):
     p.check_attention(4, 1, q=q)  # the mean of the values
 
 
+@pytest.mark.parametrize("qname", ["F16", "Q8_0"])
+@pytest.mark.parametrize("width", [None, 300])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attention_with_large_equal_scores(b200, ctx, qname, width, sign):
+    """Equal scores of 2^20 to 2^31 (the distances between floats go from 1/8 to 256): the mean of the values, whatever they are."""
+    n, D = 200, 64
+    p = Pool(b200, ctx, getattr(b200, qname), 1, D, 16, [n], seed=25, width=width)
+    k = np.full((1, n, 1, D), 127.0, np.float32)  # the scale 1 in Q8_0
+    v = p.rng.normal(0, 1, (1, n, 1, D)).astype(np.float32)
+    ctx.kv_write(p.cache, cu(k), cu(v), p.table, p.lens_t)
+    ctx.synchronize()
+    values = p.rows(0)[1][:, 0]
+    # weights that are equal have 22 bits each, as have their products with a scale; a sum of 200, a division: below 2^-19
+    tol = np.abs(values).mean(0) * 2.0 ** -19
+    for power in range(20, 32):
+        for part in (1.0, 1.37, 1.999):
+            q = np.full((1, 1, 2, D), sign * part * 2.0 ** power / (127 * D), np.float32)
+            got = ctx.kv_attention(p.cache, cu(q), p.table, p.lens_t, 1.0).cpu().numpy()[0, 0]
+            assert (np.abs(got - values.mean(0)) <= tol).all(), (power, part)
+
+
 @pytest.mark.parametrize("n_tok", [1, 3])
 def test_values_that_a_weight_all_but_leaves_out(b200, ctx, n_tok):
     """In one piece of the cache lie values of 1e6 whose weights are some e^-40 and values of 1e-4 whose weights are most of
