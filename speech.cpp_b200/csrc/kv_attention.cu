@@ -1,10 +1,10 @@
 // kv_attention.cu — attention of a few new tokens per sequence over the paged key/value cache (b200_kv_attention).
 //
 // Mathematics. The rows of one key/value head (its group of query heads, times the call's tokens) share every key and value,
-// so they are taken eight (or twice eight) at a time: S = Q K^T and O = P V over 16 positions at a time, with a running maximum
-// and sum per row (o and l are rescaled by 2^(m_old - m_new) when a larger score appears; exponentials to base 2, their scale
-// folded into the scores'). Bytes decide: a position costs 4 D bytes (F16) or 2.125 D (Q8_0) of HBM and 4 D multiply-adds
-// per row, so the arithmetic has to cost next to nothing beside the stream of the cache.
+// so they are taken eight (or twice eight) at a time: S = Q K^T and O = P V over 16 positions at a time, with a running sum
+// per row, in units of 2^m: m follows the maximum of the positions at hand (o and l are rescaled by 2^(m_old - m_new);
+// exponentials to base 2, their scale folded into the scores'). Bytes decide: a position costs 4 D bytes (F16) or 2.125 D
+// (Q8_0) of HBM and 4 D multiply-adds per row, so the arithmetic has to cost next to nothing beside the stream of the cache.
 //
 // Float32 results from F16 matrix instructions. mma.m16n8k16 multiplies F16 exactly and adds in float32, but takes 16 rows
 // where there are at most eight: rows 0-7 of the tile hold the high half of the operand and rows 8-15 the low half (x = hi +
@@ -53,7 +53,8 @@ constexpr int kJoinWarps = 8;  // 2^3
 constexpr int kChunk = 64;       // positions of a chunk: one piece per warp
 constexpr int kItemChunks = 16;  // the work is cut by items up to this many chunks per CTA,
 constexpr int kItemMost = 64;    // and this many per sequence
-constexpr float kShift = 14;     // weights are held times 2^14, so that their low halves reach 2^-38 of the largest
+constexpr float kShift = 14;     // weights are held times 2^14, so that their low halves reach 2^-38 of a step's largest
+constexpr float kFall = 32;      // how far the unit of l and o may fall below the largest it was, in powers of two
 
 struct Geometry {
     int n_tok, n_head, group;
@@ -424,9 +425,9 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
 
     const int plain_end = min(p_end, all_see);  // steps that end here or before have all their positions, seen by every row
     float2 o[TILES][S::kGroups][S::kRun] = {};
-    float m[TILES], l[TILES];
+    float m[TILES], m_most[TILES], l[TILES];
 #pragma unroll
-    for (int y = 0; y < TILES; y++) m[y] = -INFINITY, l[y] = 0.0f;
+    for (int y = 0; y < TILES; y++) m[y] = m_most[y] = -INFINITY, l[y] = 0.0f;
     int stage = 0;
     for (int p0 = (int) c0 * kChunk + warp * 16 * kSub; p0 < p_end; p0 += kStep) {
         asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
@@ -497,7 +498,10 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                     }
         }
 
-        // ---- weights: m is the running maximum less kShift (-infinity before any score) ----
+        // ---- weights, in units of 2^m: m is the step's maximum, rounded up, less kShift (-infinity before any score) ----
+        // So what F16 cannot hold of a weight, or of its product with a scale, is small beside this step's largest, not only
+        // beside that of a position far away whose values may be 0. m stays within kFall of the largest it was, so that l and o
+        // do not leave float32's range, and is whole, so that going from one m to another is exact.
         float2 keep[TILES];
         uint32_t pf[TILES][kSub][4];  // the weights' fragments: hi, lo of positions 2 t, 2 t + 1, then of 2 t + 8, 2 t + 9
 #pragma unroll
@@ -507,7 +511,9 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
             for (int u = 0; u < kSub; u++) top = fmaxf(top, fmaxf(fmaxf(s[y][u][0], s[y][u][1]), fmaxf(s[y][u][2], s[y][u][3])));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float m_new = fmaxf(m[y], __fadd_ru(top, -kShift));  // rounded down, top - m could pass 14 where floats are 4 apart
+            const float own = __fadd_ru(ceilf(top), -kShift);  // rounded down, top - m could pass 14 where floats are 4 apart
+            m_most[y] = fmaxf(m_most[y], own);
+            const float m_new = fmaxf(own, m_most[y] - kFall);
             const float base = m_new == -INFINITY ? 0.0f : m_new;
             const float k = ex2(m[y] - base);
             keep[y] = make_float2(k, k);
@@ -582,9 +588,10 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                     }
                 }
             };
-            // Scales between 2^-14 and 2 (nearly always all of them) multiply the weights' halves in F16 pairs: the
-            // product's rounding error is exact in F16 and goes to the low half. The weights being up to 2^14 and the low
-            // halves reaching 2^-24, nothing overflows and what is lost is below 2^-24 of the largest weight's product.
+            // Scales between 2^-11 and 2 (nearly always all of them) multiply the weights' halves in F16 pairs: the product's
+            // rounding error is exact in F16 and goes to the low half. The largest weight being in (2^13, 2^14] and the low halves
+            // reaching 2^-24, nothing overflows, and products below 2^-27 of the largest weight times the least scale are lost.
+            // (Powers of two that bring each block's scales to 1 first would keep 2^-36, at 5 to 10 % of the time.)
             uint32_t low = vd[0][0][0], high = vd[0][0][0];
 #pragma unroll
             for (int u = 0; u < kSub; u++)
@@ -592,7 +599,7 @@ __device__ __forceinline__ void attend(const KvView & c, const Geometry & g, con
                 for (int i = 0; i < 2; i++)
 #pragma unroll
                     for (int b = 0; b < S::kBlocks; b++) low = __vminu2(low, vd[u][i][b]), high = __vmaxu2(high, vd[u][i][b]);
-            const bool plain = (low & 0xffffu) >= 0x0400u && low >= 0x04000000u && (high & 0xffffu) < 0x4000u && high < 0x40000000u;
+            const bool plain = (low & 0xffffu) >= 0x1000u && low >= 0x10000000u && (high & 0xffffu) < 0x4000u && high < 0x40000000u;
             if (__all_sync(0xffffffffu, plain)) {
                 auto go = [&](auto index) {
                     constexpr int b = decltype(index)::value;

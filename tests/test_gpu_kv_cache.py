@@ -485,6 +485,57 @@ def test_values_that_a_weight_all_but_leaves_out(b200, ctx, n_tok):
     p.check_attention(4, n_tok, scale=0.3125, q=q)  # scores of -40 beside +-0.35
 
 
+def lay_out(pool, s, which, numbers, scales):
+    """Sequence s's rows of a Q8_0 pool as they are given: whole numbers [n][Hkv][D] and scales [n][Hkv][D / 32]."""
+    import torch
+
+    pos = np.arange(numbers.shape[0])
+    page, slot = (torch.from_numpy(x).cuda() for x in (pool.table_np[s, pos // pool.page].astype(np.int64), pos % pool.page))
+    pool.f[which][page, :, slot] = cu(numbers.astype(np.int8))
+    pool.f[2 + which][page, :, slot] = cu(scales.astype(np.float16))
+
+
+@pytest.mark.parametrize("S,width", [(450, None), (450, 300), (1, None), (1, 300)])  # items of their own, or shared; by items, by positions
+@pytest.mark.parametrize("least,spread", [(2.0 ** -14, 0), (2.0 ** -11, 0), (2.0 ** -14, 14), (2.0 ** -11, 11)])
+@pytest.mark.parametrize("n,first", [(40, 3), (900, 500), (4700, 3), (4700, 2600)])
+@pytest.mark.parametrize("D,group", [(64, 2), (64, 12), (96, 2), (96, 9), (128, 2), (128, 16), (256, 2)])
+def test_a_tail_behind_one_position(b200, ctx, D, group, n, first, least, spread, S, width):
+    """One position takes all but e^-17 to e^-22 of the weights, and in the first block its values are 0: there the many small
+    weights are all there is. The values' scales are all the same, or go from there to 1. (All sequences are the same one, so
+    many that a warp takes a long run of its positions.)"""
+    rng = np.random.default_rng(n + D)
+    p = Pool(b200, ctx, b200.Q8_0, 1, D, 16, [n], seed=n, width=width)
+    blocks = D // 32
+    k, kd = np.full((n, 1, D), -127), np.zeros((n, 1, blocks))
+    kd[:] = rng.uniform(17, 22, (n, 1, 1)) / (127 * D)  # q is 1 in every dimension: scores of -17 to -22 beside 0
+    k[first], kd[first] = 0, 1.0
+    v = rng.integers(-127, 128, (n, 1, D))
+    vd = least * 2.0 ** (rng.uniform(0, spread, (n, 1, blocks)))
+    beside = slice(first, first + 1) if n < 100 else slice(first // 64 * 64, first // 64 * 64 + 64)
+    v[beside, 0, :32] = 0  # those that are taken at a time with the first one, too, where there are others
+    lay_out(p, 0, 0, k, kd)
+    lay_out(p, 0, 1, v, vd)
+    q = np.ones((S, 1, group, D), np.float32)
+    got = ctx.kv_attention(p.cache, cu(q), p.table.repeat(S, 1), p.lens_t.repeat(S), 1.0).cpu().numpy()[:, 0]
+    ctx.synchronize()
+    kk, vv = p.rows(0)
+    score = kk[:, 0].sum(-1)
+    w = np.exp(score - score.max())
+    w /= w.sum()
+    want, size = w @ vv[:, 0], w @ np.abs(vv[:, 0])
+    # A score is D / 32 exact blocks added up and two products more, each off by at most half a unit of 32 (2^-19), as are the
+    # two differences of base-2 logarithms that its weight is the exponential of: an error of delta in every score changes a
+    # weight by at most exp(2 delta) - 1. The weight meets up to four exponentials (2^-22 each), enters with 22 bits, as does
+    # its product with a scale, and is divided: below 2^-19. A warp takes at most 16 of every 64 positions, each 16 are
+    # added once, and up to 34 partial results are joined. F16 holds a weight and its product with a scale (at most 1) to 2^-39
+    # each of the largest weight, or twice that, that it is taken with: the first one's for 31 positions where these have
+    # values, the tail's for the others.
+    delta = (D / 32 + 4) * 2.0 ** -19
+    tol = size * (np.expm1(2 * delta) + 2.0 ** -19 + (n / 64 + 34) * 2.0 ** -24)
+    tol += 127 * 2.0 ** -38 * np.where((np.arange(D) < 32) & (n > 100), 0, 31) + n * 127 * 2.0 ** -37 * np.exp(-17)
+    assert (np.abs(got - want) <= tol).all(), f"off by {np.max(np.abs(got - want) / size):.3g} of the magnitudes, allowed {np.max(tol / size):.3g}"
+
+
 @pytest.mark.parametrize("width", [None, 300])
 def test_attention_does_not_see_what_lies_behind_a_row(b200, ctx, width):
     """Positions that later rows of the call see, but an earlier one does not, hold NaN and infinities: the earlier rows
