@@ -78,7 +78,8 @@ b200_status b200_context_create(int device, b200_context ** out);
 void b200_context_destroy(b200_context * ctx);
 /* The context's cudaStream_t. */
 void * b200_context_stream(b200_context * ctx);
-/* Waits for the stream; returns the first device-side error recorded since the last call (then clears it). */
+/* Waits for the stream; returns a device-side error recorded since the last call, if there is one (B200_ERR_TIMEOUT before
+ * B200_ERR_RANGE; the text names all kinds that were recorded), and clears what it returned. */
 b200_status b200_synchronize(b200_context * ctx);
 /* Text of the last error on this context ("" when none). */
 const char * b200_last_error(b200_context * ctx);

@@ -58,6 +58,9 @@ int64_t block_bytes(int t) {
     }
 }
 
+// The error word's bits to the (pinned) host word, and 0 in their place.
+__global__ void take_errors(unsigned * bits, unsigned * host) { *host = atomicExch(bits, 0); }
+
 // Grows the context's scratch to at least `bytes` (synchronizes the stream when it has to reallocate).
 b200_status ensure_scratch(b200_context * ctx, size_t bytes) {
     if (ctx->scratch_bytes >= bytes) return B200_OK;
@@ -332,16 +335,25 @@ b200_status b200_synchronize(b200_context * ctx) {
     if (!ctx) return fail(nullptr, B200_ERR_INVALID, "synchronize: NULL context");
     CK(ctx, cudaMemcpyAsync(ctx->host_err, ctx->dev_err, sizeof(unsigned), cudaMemcpyDeviceToHost, ctx->stream));
     CK(ctx, cudaStreamSynchronize(ctx->stream));
+    if (*ctx->host_err == 0) return B200_OK;
+    // Calls on other streams may still be setting bits: they are fetched and cleared in one step, so that each is reported once.
+    DeviceScope scope(ctx->device);
+    CK(ctx, scope.status);
+    take_errors<<<1, 1, 0, ctx->stream>>>(ctx->dev_err, ctx->host_err);
+    CK(ctx, cudaGetLastError());
+    CK(ctx, cudaStreamSynchronize(ctx->stream));
     const unsigned bits = *ctx->host_err;
-    if (bits) {
-        CK(ctx, cudaMemsetAsync(ctx->dev_err, 0, sizeof(unsigned), ctx->stream));
-        CK(ctx, cudaStreamSynchronize(ctx->stream));
-        if (bits & B200_DEVERR_TIMEOUT) return fail(ctx, B200_ERR_TIMEOUT, "a bounded device wait gave up");
-        if (bits & B200_DEVERR_EXPERT) return fail(ctx, B200_ERR_RANGE, "mul_mat_id: an expert id is outside [0, E)");
-        if (bits & B200_DEVERR_ROWS) return fail(ctx, B200_ERR_RANGE, "get_rows: a row id is outside the table");
-        return fail(ctx, B200_ERR_RANGE, "kv cache: a page number or a sequence length is outside its range");
-    }
-    return B200_OK;
+    static const struct {
+        unsigned bit;
+        const char * text;
+    } kinds[] = {{B200_DEVERR_TIMEOUT, "a bounded device wait gave up"},
+                 {B200_DEVERR_EXPERT, "mul_mat_id: an expert id is outside [0, E)"},
+                 {B200_DEVERR_ROWS, "get_rows: a row id is outside the table"},
+                 {B200_DEVERR_PAGE, "kv cache: a page number or a sequence length is outside its range"}};
+    std::string text;
+    for (const auto & k : kinds)
+        if (bits & k.bit) text += (text.empty() ? "" : "; ") + std::string(k.text);
+    return fail(ctx, bits & B200_DEVERR_TIMEOUT ? B200_ERR_TIMEOUT : B200_ERR_RANGE, text.c_str());
 }
 
 const char * b200_last_error(b200_context * ctx) { return ctx ? ctx->last_error.c_str() : g_error.c_str(); }

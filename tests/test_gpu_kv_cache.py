@@ -220,6 +220,35 @@ def test_bad_pages_and_lengths_are_reported_and_left_out(b200, ctx):
         p.data.copy_(before)
 
 
+def test_an_error_on_another_stream_is_reported_once(b200, ctx, oracle):
+    """A bad length on a side stream, recorded before, while or after the context reports an error of its own: whichever
+    report comes after it names it."""
+    import torch
+
+    p = Pool(b200, ctx, b200.F16, 1, 64, 16, [20], seed=26).fill()
+    q, out, bad = torch.ones(1, 1, 1, 64, device="cuda"), torch.empty(1, 1, 1, 64, device="cuda"), cu(np.array([-1], np.int32))
+    w = ctx.weight(b200.Q8_0, 64, 4, data=oracle.quantize(b200.Q8_0, np.ones((4, 64), np.float32)))
+    ids = cu(np.array([9], np.int32))
+    side = torch.cuda.Stream()
+    ctx.synchronize()
+    torch.cuda.synchronize()
+
+    def report():
+        return "" if ctx.L.b200_synchronize(ctx.h) == b200.OK else ctx.L.b200_last_error(ctx.h).decode()
+
+    for i in range(400):
+        ctx.get_rows(w, ids)
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(500 * i)  # up to some 100 us
+            ctx.kv_attention(p.cache, q, p.table, bad, 1.0, out=out)
+        first = report()
+        side.synchronize()
+        second = report()
+        assert "get_rows" in first and "get_rows" not in second, i
+        assert ("kv cache" in first) + ("kv cache" in second) == 1, i
+    ctx.free_weight(w)
+
+
 # ---- write and read ----------------------------------------------------------------------------------------------------
 
 
