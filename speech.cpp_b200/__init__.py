@@ -249,7 +249,6 @@ class Context:
     """One B200 device, one stream, a scratch pool (b200_context)."""
 
     _raw_stream = None
-    _on_torchs = False  # calls have run on torch's current stream since the last synchronize()
 
     def __init__(self, device=0):
         self.L = lib()
@@ -260,6 +259,7 @@ class Context:
             raise B200Error(s, self.L.b200_last_error(None).decode())
         self.h = h
         self._children = weakref.WeakSet()  # decoders built on this context: closed before it
+        self._used = set()  # torch's streams (their handles) that calls have run on since the last synchronize()
 
     def check(self, status):
         if status != OK:
@@ -275,11 +275,17 @@ class Context:
         return torch.cuda.ExternalStream(self.stream_handle, device=torch.device("cuda", self.device))
 
     def synchronize(self):
-        """Waits for the context's stream and, after calls that ran on torch's current stream, for that one; raises the first
-        error that a kernel recorded."""
-        if self._on_torchs:
-            self._sync_in()
-            self._on_torchs = False
+        """Waits for the context's stream and for the calls that ran on torch's (for the whole device where these were others
+        than the current one, which may be gone by now); raises an error that a kernel recorded. Replays of a captured graph
+        are the caller's to wait for first."""
+        if self._used:
+            import torch
+
+            if self._used == {self._torch_handle()}:
+                self._sync_in()
+            else:
+                torch.cuda.synchronize(self.device)
+            self._used.clear()
         self.check(self.L.b200_synchronize(self.h))
 
     def close(self):
@@ -443,16 +449,22 @@ class Context:
     # -- paged key/value cache and expert router (torch CUDA tensors; run on torch's current stream) ------------------
     # A decode step calls these once per layer, so their checks read each attribute of a tensor once and build texts only for
     # an error.
-    def _stream(self):
+    def _torch_handle(self):
         """torch's current stream of this device as a cudaStream_t (the default stream as cudaStreamLegacy, since NULL
-        means the context's own stream). These calls use nothing of the context's stream, so they run in torch's order."""
+        means the context's own stream)."""
         if self._raw_stream is None:
             import torch
 
             # the handle alone, where torch has it: a Stream object costs a microsecond more per call
             self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
-        self._on_torchs = True
         return self._raw_stream(self.device) or 1
+
+    def _stream(self):
+        """The stream that a call runs on: torch's current one. These calls use nothing of the context's stream, so they run in
+        torch's order."""
+        handle = self._torch_handle()
+        self._used.add(handle)
+        return handle
 
     def _refuse(self, t, what, wanted):
         if not t.is_cuda or t.get_device() != self.device:

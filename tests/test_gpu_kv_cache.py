@@ -666,6 +666,30 @@ def test_calls_run_on_torchs_current_stream(b200, ctx, lens):
     assert torch.equal(out, want[0])
 
 
+@pytest.mark.parametrize("others", [1, 2])
+def test_synchronize_waits_for_the_streams_that_calls_ran_on(b200, ctx, others):
+    """Calls on side streams, checked outside of these: their work is done and their errors are raised, once."""
+    import torch
+
+    p = Pool(b200, ctx, b200.F16, 1, 64, 16, [20], seed=27).fill()
+    q, bad = torch.ones(1, 1, 1, 64, device="cuda"), cu(np.array([-1], np.int32))
+    outs = [torch.ones(1, 1, 1, 64, device="cuda") for _ in range(others)]
+    ctx.synchronize()
+    for rep in range(3):
+        streams = [torch.cuda.Stream() for _ in range(others)]
+        for st, out in zip(streams, outs):
+            out.fill_(1.0)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(st):
+                torch.cuda._sleep(10_000_000)  # some 5 ms
+                ctx.kv_attention(p.cache, q, p.table, bad, 1.0, out=out)
+        with pytest.raises(b200.B200Error, match="kv cache"):
+            ctx.synchronize()
+        assert all(st.query() for st in streams)
+        assert not any(out.any() for out in outs)
+        ctx.synchronize()
+
+
 def test_the_first_call_of_a_context_may_be_captured(b200):
     import torch
 
