@@ -585,6 +585,78 @@ def test_attention_does_not_see_what_lies_behind_a_row(b200, ctx, width):
     ctx.synchronize()
 
 
+@pytest.mark.parametrize("qname", ["F16", "Q8_0"])
+@pytest.mark.parametrize("D,H", [(64, 4), (64, 8), (96, 8), (128, 4), (128, 8), (256, 8)])  # eight rows of a key/value head, or sixteen
+@pytest.mark.parametrize("width", [None, 300])
+def test_rows_before_a_position_that_is_not_finite(b200, ctx, qname, D, H, width):
+    """A key or value (in Q8_0: its scale) that only the later half of the call's rows see is NaN or infinite: the earlier
+    rows have what they have without it."""
+    import torch
+
+    p = Pool(b200, ctx, getattr(b200, qname), 2, D, 16, [50, 17, 135], seed=28, width=width).fill()
+    q = p.rng.normal(0, 1, (3, 4, H, D)).astype(np.float32)
+    kv = [p.rows(s) for s in range(3)]
+    want, tol = ref.attention(q[:, :2], [k[:-2] for k, _ in kv], [v[:-2] for _, v in kv], [n - 2 for n in p.lens], 0.1)
+    first = 0 if qname == "F16" else 2
+    for which, value in ((0, float("nan")), (0, float("inf")), (1, float("nan")), (1, float("inf"))):
+        keep = p.data.clone()
+        for s, n in enumerate(p.lens):
+            p.f[first + which][p.table_np[s, (n - 2) // 16], :, (n - 2) % 16] = value  # rows 2 and 3 see it
+        got = ctx.kv_attention(p.cache, cu(q), p.table, p.lens_t, 0.1)
+        assert (np.abs(got[:, :2].cpu().numpy() - want) <= tol).all()
+        if which == 1 or np.isnan(value):
+            assert not torch.isfinite(got[:, 2:]).all(-1).any()
+        p.data.copy_(keep)
+    ctx.synchronize()
+
+
+@pytest.mark.parametrize("D,Hkv,group,page,n_tok,lens", [(64, 2, 2, 16, 1, [300]), (64, 1, 5, 48, 3, [200, 31]), (96, 2, 1, 16, 1, [100, 700]),
+                                                         (96, 1, 16, 32, 1, [333]), (128, 1, 4, 16, 4, [260, 5]), (256, 2, 2, 32, 2, [90, 400])])
+@pytest.mark.parametrize("width", [None, 300])
+def test_value_scales_of_any_size(b200, ctx, D, Hkv, group, page, n_tok, lens, width):
+    """Blocks whose scales lie below 2^-14, above 2, in between and across these ends."""
+    p = Pool(b200, ctx, b200.Q8_0, Hkv, D, page, lens, seed=29, width=width)
+    n = max(lens)
+    k = p.rng.normal(0, 1, (len(lens), n, Hkv, D)).astype(np.float32)
+    blocks = np.resize([2.0 ** -16, 2.0 ** 12, 1.0, 2.0 ** -7, 2.0 ** 7, 2.0 ** -20], (Hkv * D // 32,)).reshape(Hkv, D // 32).repeat(32, -1)
+    v = (p.rng.normal(0, 1, (len(lens), n, Hkv, D)) * 2.0 ** p.rng.integers(-2, 3, (len(lens), n, Hkv, 1)) * blocks).astype(np.float32)
+    ctx.kv_write(p.cache, cu(k), cu(v), p.table, p.lens_t)
+    p.check_attention(Hkv * group, n_tok)
+
+
+@pytest.mark.parametrize("qname", ["F16", "Q8_0"])
+def test_a_prefix_read_back_for_a_prompts_block(b200, ctx, qname):
+    """The rows of one request taken out as F16 and attended to by FLASH_ATTN: the 30 newest of 77 positions, of which the 16
+    newest are what kv_attention gives for them."""
+    import torch
+
+    n, n_q, H, Hkv, D, scale = 77, 30, 4, 2, 64, 0.125
+    p = Pool(b200, ctx, getattr(b200, qname), Hkv, D, 16, [n], seed=30).fill()
+    k, v = ctx.kv_read(p.cache, p.table, p.lens_t, n_tok=n, dtype=torch.float16)
+    q = p.rng.normal(0, 1, (n_q, H, D)).astype(np.float16).astype(np.float32)  # FLASH_ATTN rounds q to F16
+    mask = np.where(np.arange(n)[None] <= n - n_q + np.arange(n_q)[:, None], 0.0, -np.inf).astype(np.float16)
+    out, qd, md = torch.full((n_q, H, D), float("nan"), device="cuda"), cu(q), cu(mask)
+    g = b200.Graph(ctx)
+    g.add(b200.OP_FLASH_ATTN, out, src=[g.add(t=t) for t in (qd.permute(1, 0, 2), k[0].permute(1, 0, 2), v[0].permute(1, 0, 2), md)],
+          params=[g.fbits(scale)])
+    g.compute()
+    newest = ctx.kv_attention(p.cache, qd[None, -16:].contiguous(), p.table, p.lens_t, scale)
+    ctx.synchronize()
+    kk, vv = (x[0].cpu().numpy().astype(np.float64) for x in (k, v))
+    for which, x in enumerate(p.rows(0)):  # the rows are the cache's, rounded once
+        assert np.array_equal((kk, vv)[which], x.astype(np.float32).astype(np.float16).astype(np.float64))
+    s = np.einsum("qhd,jhd->qhj", q.astype(np.float64), kk.repeat(H // Hkv, 1)) * scale + mask[:, None].astype(np.float64)
+    w = np.exp(s - s.max(-1, keepdims=True))
+    w /= w.sum(-1, keepdims=True)
+    want, size = (np.einsum("qhj,jhd->qhd", w, x.repeat(H // Hkv, 1)) for x in (vv, np.abs(vv)))
+    # a score is rounded twice, its difference to the maximum and its exponential once, a product with a value and the result once
+    delta = 4 * 2.0 ** -24 * np.abs(np.where(np.isfinite(s), s, 0)).max()
+    assert (np.abs(out.cpu().numpy() - want) <= size * (np.expm1(2 * delta) + 2.0 ** -22)).all()
+    got = newest[0].cpu().numpy()
+    want, tol = ref.attention(q[None, -16:], [p.rows(0)[0]], [p.rows(0)[1]], [n], scale)
+    assert (np.abs(got - want[0]) <= tol[0]).all()
+
+
 def test_non_finite_queries_stay_in_their_rows(b200, ctx):
     import torch
 
