@@ -406,9 +406,10 @@ b200_status b200_kv_read(b200_context * ctx, void * stream, const b200_kv_cache 
  * Weights are held against the largest one among the 16 or 32 positions that are taken at a time: below 2^-16 of it they have
  * fewer bits, and below 2^-38 they count as 0 in front of their values. Over Q8_0 the same goes for the products of weights
  * and values' scales against the largest weight times the block's largest scale: below 2^-10 and 2^-32 of it for scales of
- * 2^-6, at the worst (2^-11) below 2^-5 and 2^-27. A key or value that is not finite can make every row that sees it NaN. workspace: device memory of b200_kv_attention_workspace bytes (256-byte aligned, contents
- * arbitrary; NULL when that is 0), in use until the call's work is done: calls that may overlap on the GPU need one each.
- * table and lens must not change before then either. */
+ * 2^-6, at the worst (2^-13) below 2^-3 and 2^-25. A key or value that is not finite can make every row that sees it NaN.
+ * workspace: device memory of b200_kv_attention_workspace bytes (256-byte aligned, contents arbitrary; NULL when that is 0),
+ * in use until the call's work is done: calls that may overlap on the GPU need one each. table and lens must not change
+ * before then either. */
 size_t b200_kv_attention_workspace(b200_context * ctx, const b200_kv_cache * cache, int64_t max_pages, int64_t n_seq, int64_t n_tok,
                                    int64_t n_head);
 b200_status b200_kv_attention(b200_context * ctx, void * stream, const b200_kv_cache * cache, const int32_t * table, int64_t max_pages,

@@ -525,7 +525,7 @@ def lay_out(pool, s, which, numbers, scales):
 
 
 @pytest.mark.parametrize("S,width", [(450, None), (450, 300), (1, None), (1, 300)])  # items of their own, or shared; by items, by positions
-@pytest.mark.parametrize("least,spread", [(2.0 ** -14, 0), (2.0 ** -11, 0), (2.0 ** -14, 14), (2.0 ** -11, 11)])
+@pytest.mark.parametrize("least,spread", [(2.0 ** -14, 0), (2.0 ** -13, 0), (2.0 ** -11, 0), (2.0 ** -14, 14), (2.0 ** -13, 13), (2.0 ** -11, 11)])
 @pytest.mark.parametrize("n,first", [(40, 3), (900, 500), (4700, 3), (4700, 2600)])
 @pytest.mark.parametrize("D,group", [(64, 2), (64, 12), (96, 2), (96, 9), (128, 2), (128, 16), (256, 2)])
 def test_a_tail_behind_one_position(b200, ctx, D, group, n, first, least, spread, S, width):
