@@ -16,6 +16,31 @@
 
 using namespace b200;
 
+namespace {
+
+// Bytes of the arrays k (and v) and of the scales of k (and v); false when the cache is not one that is supported.
+bool kv_sizes(int type, int64_t heads, int64_t dim, int64_t page, int64_t pages, int64_t * values, int64_t * scales) {
+    if (type != B200_TYPE_F16 && type != B200_TYPE_Q8_0) return false;
+    if (dim != 64 && dim != 96 && dim != 128 && dim != 256) return false;
+    if (heads <= 0 || heads > 65535 || page <= 0 || page % 16 || page > 4096 || pages <= 0 || pages > INT32_MAX) return false;
+    const int64_t rows = heads * page;  // at most 2^28
+    if (pages > ((int64_t) 1 << 52) / (rows * dim)) return false;
+    *values = pages * rows * dim * (type == B200_TYPE_F16 ? 2 : 1);
+    *scales = type == B200_TYPE_F16 ? 0 : pages * rows * (dim / 32) * 2;
+    return true;
+}
+
+// Where the arrays k, v, k scales and v scales start, and the bytes of all.
+struct KvLayout {
+    int64_t off[4], bytes;
+    KvLayout(int64_t values, int64_t scales)
+        : off{0, align256(values), 2 * align256(values), 2 * align256(values) + align256(scales)}, bytes(2 * align256(values) + 2 * align256(scales)) {}
+};
+
+bool aligned(const void * p, size_t to) { return ((uintptr_t) p & (to - 1)) == 0; }
+
+}  // namespace
+
 namespace b200 {
 
 b200_status kv_fail(b200_context * ctx, b200_status s, const char * what, const char * why) {
@@ -32,8 +57,12 @@ b200_status kv_cuda(b200_context * ctx, cudaError_t e, const char * what) {
 b200_status kv_checked_view(b200_context * ctx, const char * what, const b200_kv_cache * c, const int32_t * table, int64_t max_pages,
                             const int32_t * lens, int64_t n_seq, int64_t n_tok, KvView * out) {
     if (!ctx) return kv_fail(ctx, B200_ERR_INVALID, what, "NULL context");
-    const size_t need = c ? b200_kv_cache_nbytes(c->type, c->n_kv_head, c->head_dim, c->page_size, c->n_pages) : 0;
-    if (!need || !c->data || c->nbytes < need) return kv_fail(ctx, B200_ERR_INVALID, what, "not a cache");
+    int64_t values, scales;
+    if (!c || !kv_sizes(c->type, c->n_kv_head, c->head_dim, c->page_size, c->n_pages, &values, &scales))
+        return kv_fail(ctx, B200_ERR_INVALID, what, "not a cache");
+    const KvLayout layout(values, scales);
+    if (!c->data || !aligned(c->data, 16) || c->nbytes < (size_t) layout.bytes || std::memcmp(c->field_off, layout.off, sizeof layout.off) != 0)
+        return kv_fail(ctx, B200_ERR_INVALID, what, "not a cache");
     if (c->device != ctx->device) return kv_fail(ctx, B200_ERR_INVALID, what, "the cache lies on another device than the context");
     if (n_seq < 0 || n_tok < 0 || max_pages < 0) return kv_fail(ctx, B200_ERR_INVALID, what, "a negative size");
     if (n_seq > 0 && n_tok > 0 && (!lens || (max_pages > 0 && !table) || ((uintptr_t) lens & 3) || ((uintptr_t) table & 3)))
@@ -60,18 +89,6 @@ b200_status kv_checked_view(b200_context * ctx, const char * what, const b200_kv
 }  // namespace b200
 
 namespace {
-
-// Bytes of the arrays k (and v) and of the scales of k (and v); false when the cache is not one that is supported.
-bool kv_sizes(int type, int64_t heads, int64_t dim, int64_t page, int64_t pages, int64_t * values, int64_t * scales) {
-    if (type != B200_TYPE_F16 && type != B200_TYPE_Q8_0) return false;
-    if (dim != 64 && dim != 96 && dim != 128 && dim != 256) return false;
-    if (heads <= 0 || heads > 65535 || page <= 0 || page % 16 || page > 4096 || pages <= 0 || pages > INT32_MAX) return false;
-    const int64_t rows = heads * page;  // at most 2^28
-    if (pages > ((int64_t) 1 << 52) / (rows * dim)) return false;
-    *values = pages * rows * dim * (type == B200_TYPE_F16 ? 2 : 1);
-    *scales = type == B200_TYPE_F16 ? 0 : pages * rows * (dim / 32) * 2;
-    return true;
-}
 
 // Four float32 values at p (16-byte aligned when VEC).
 template <bool VEC>
@@ -287,8 +304,6 @@ void with_dim(int D, F f) {
     }
 }
 
-bool aligned(const void * p, size_t to) { return ((uintptr_t) p & (to - 1)) == 0; }
-
 }  // namespace
 
 extern "C" {
@@ -296,7 +311,7 @@ extern "C" {
 size_t b200_kv_cache_nbytes(int type, int64_t n_kv_head, int64_t head_dim, int64_t page_size, int64_t n_pages) {
     int64_t values, scales;
     if (!kv_sizes(type, n_kv_head, head_dim, page_size, n_pages, &values, &scales)) return 0;
-    return (size_t) (2 * align256(values) + 2 * align256(scales));
+    return (size_t) KvLayout(values, scales).bytes;
 }
 
 b200_status b200_kv_cache_view(b200_context * ctx, int type, int64_t n_kv_head, int64_t head_dim, int64_t page_size, int64_t n_pages,
@@ -309,7 +324,8 @@ b200_status b200_kv_cache_view(b200_context * ctx, int type, int64_t n_kv_head, 
         return kv_fail(ctx, B200_ERR_UNSUPPORTED, "kv_cache_view",
                        "needs F16 or Q8_0, head_dim 64, 96, 128 or 256, page_size a multiple of 16 up to 4096");
     if (!aligned(data, 16)) return kv_fail(ctx, B200_ERR_INVALID, "kv_cache_view", "data is not 16-byte aligned");
-    const size_t need = b200_kv_cache_nbytes(type, n_kv_head, head_dim, page_size, n_pages);
+    const KvLayout layout(values, scales);
+    const size_t need = (size_t) layout.bytes;
     if (nbytes < need) return kv_fail(ctx, B200_ERR_INVALID, "kv_cache_view", "too few bytes");
     out->type = type;
     out->device = ctx->device;
@@ -319,9 +335,7 @@ b200_status b200_kv_cache_view(b200_context * ctx, int type, int64_t n_kv_head, 
     out->n_pages = n_pages;
     out->data = data;
     out->nbytes = need;
-    out->field_off[1] = align256(values);
-    out->field_off[2] = 2 * align256(values);
-    out->field_off[3] = 2 * align256(values) + align256(scales);
+    std::memcpy(out->field_off, layout.off, sizeof layout.off);
     return B200_OK;
 }
 

@@ -178,6 +178,29 @@ def test_refusals(b200, ctx):
     ctx.synchronize()
 
 
+@pytest.mark.parametrize("qname", ["F16", "Q8_0"])
+def test_caches_that_are_not_laid_out_as_documented_are_refused(b200, ctx, qname):
+    """Arrays that the struct places elsewhere, or memory that is not aligned, would be read past their ends or misaligned."""
+    import torch
+
+    cache = ctx.kv_cache(getattr(b200, qname), 2, 64, 16, 4)
+    table, lens, x = cu(np.zeros((1, 2), np.int32)), cu(np.array([1], np.int32)), torch.zeros(1, 1, 2, 64, device="cuda").data_ptr()
+    kinds = [("data", cache.s.data + 8), ("data", cache.s.data + 1), ("data", 0), ("nbytes", cache.s.nbytes - 1)]
+    kinds += [(i, cache.s.field_off[i] + by) for i in range(4) for by in (-256, -16, 1, 16, 1 << 40)]
+    for name, value in kinds:
+        bad = b200.KvCacheStruct.from_buffer_copy(cache.s)
+        if name in ("data", "nbytes"):
+            setattr(bad, name, value)
+        else:
+            bad.field_off[name] = value
+        call = (ctx.h, None, ctypes.byref(bad), table.data_ptr(), 2, lens.data_ptr())
+        assert ctx.L.b200_kv_write(*call, 1, 1, x, 128, x, 128) == b200.ERR_INVALID
+        assert ctx.L.b200_kv_read(*call, None, 1, 1, b200.F32, x, x) == b200.ERR_INVALID
+        assert ctx.L.b200_kv_attention(*call, 1, 1, 2, x, 128, 1.0, x, None, 0) == b200.ERR_INVALID
+    cache.close()
+    ctx.synchronize()
+
+
 def test_bad_pages_and_lengths_are_reported_and_left_out(b200, ctx):
     import torch
 
