@@ -13,7 +13,9 @@
 // values are whole numbers and exact in F16; their scales stay outside: a key block's multiplies its partial score, a value
 // block's multiplies the weight's two halves. An instruction's own accumulation truncates, which over thousands of positions
 // would add up: at most two are chained, and their sum is added to the float32 result with a rounded addition. (Errors
-// against 64 bits: 2e-7 to 4e-7 of the result, a plain float32 computation's being 4e-7 to 2e-6.)
+// against 64 bits over rows of 1 to 131071 positions: 1.5e-7 to 6.2e-7 of the result, a plain float32 computation's being
+// 2.9e-7 to 2.1e-6.) What F16 drops is what is small beside the positions taken with it: m, the unit of the weights, goes down
+// again where the scores do.
 //
 // Operands. The k index of S = Q K^T may run through a row's dimensions in any order that both operands share, and the n index
 // of O = P V through any order that the output is written back in. They are chosen such that a lane's fragment is 16 (F16
@@ -32,11 +34,12 @@
 // launch (geometry() has the rule and both sides' times).
 //
 // Measured on one B200, device time (a CUDA graph of calls on the same inputs), 16 heads on 8 of 128 unless said otherwise: 64
-// sequences of 512 to 4096 positions over F16 (612 MB) 100 to 103 us, 6.0 TB/s, bound by HBM; 32 of 2048 to 16384 over Q8_0
+// sequences of 512 to 4096 positions over F16 (612 MB) 99 to 103 us, 6.0 TB/s, bound by HBM; 32 of 2048 to 16384 over Q8_0
 // (658 MB) 123 us, 5.3 TB/s, bound by the instructions that turn bytes into F16 and scale them (ALU pipe 46 % busy, matrix pipe
 // 31 %, issue slots 60 %, some 500 instructions per 16 positions; on inputs that change from call to call, under the power limit,
-// 137 to 147 us); one of 131071 positions over Q8_0, 32 heads on 4, 40 us; one of 517 over F16 6.0 us, a chain of latencies:
-// length, page number, rows, two or three pieces, the cluster's join.
+// 135 to 147 us; 64 of 512 to 4096 76 us, 128 of 128 to 1024 48 us, where the bytes alone are 50 and 25); one of 131071 positions
+// over Q8_0, 32 heads on 4, 40 to 42 us; one of 517 over F16 6.0 us, a chain of latencies: length, page number, rows, two or
+// three pieces, the cluster's join.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -1025,10 +1028,11 @@ Geometry geometry(const b200_context * ctx, const b200_kv_cache * c, int64_t max
     g.n_seq = n_seq;
     // By items when the lengths that the table allows are short: the cluster (1 to 8 CTAs) is the largest that all items fit
     // on the GPU with at once. One launch instead of two, and no scan of the lengths, against CTAs with equal work. Measured
-    // (F16, 16 and 8 heads of 128, lengths from a quarter of the table's width to all of it), by items and by positions: 1
-    // sequence of 512: 5.5 and 6.4 us, 4096: 10.1 and 8.4 (where the second launch costs the host as much again); 8 sequences of
-    // 1024: 8.1 and 11.3, 4096: 17.4 and 17.5; 64 sequences of 1024: 33.3 and 37.0, 2048: 55 and 61, but 47 and 20 (4096)
-    // when one of them is long and the others short.
+    // (F16, 16 and 8 heads of 128, lengths from an eighth of the table's width to all of it), by items and by positions: 1
+    // sequence of 512: 5.5 and 6.2 us, 4096: 10.3 and 8.4 (where the second launch costs the host as much again; a captured graph
+    // does not pay that); 8 sequences of 1024: 8.8 and 11.0, 4096: 18.3 and 16.2; 64 of 1024: 35.6 and 37.4; 128 of 1024 over
+    // Q8_0 48 and 58. The host does not know the lengths, so where few are long the choice loses: one of 1024 among 63 short ones
+    // 15.2 and 12.9, among 511 79 and 52. With wider tables that would be 46 and 16 (one of 4096 among 63).
     const int64_t most = (max_pages * c->page_size + kChunk - 1) / kChunk;  // chunks of the longest sequence there can be
     g.cluster = 8;
     while (g.cluster > 1 && n_seq * g.items * g.cluster > g.ctas) g.cluster /= 2;

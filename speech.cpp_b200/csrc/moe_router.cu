@@ -7,12 +7,19 @@
 //  - without bias and groups the keys are the logits, and rows with equal truncated neighbours are done again with whole keys;
 //  - otherwise scores are computed in float32 first, with a bound on their error, and the row is accepted if every
 //    comparison that decides (neighbours among the chosen and the next one, the last group kept and the first one left) is
-//    wider than that. Where neighbours are closer (some rows in a thousand), or groups, the few candidates are ordered by their
-//    scores in double; where they are many, two lanes' keys are equal or anything is not finite, the row is done again in double.
+//    wider than that. Where neighbours are closer (some rows in a thousand of random ones), or groups, the few candidates are
+//    ordered by their scores in double; where they are many, two lanes' keys are equal or anything is not finite, the row is
+//    done again in double.
 // The weights of the chosen are double either way, one lane for each, of all the warp's rows at once. Reading the logits
 // takes 4 B per expert (2.7 us of HBM for 16384 rows of 256); the instructions decide the time. Measured on one B200, device
-// time: 16384 rows of 256, eight chosen, by logits 11 us, by sigmoid and bias 17 us, with four of eight groups kept 21 to 23 us
-// (in double throughout: 167 us); one row of 128 2.3 us, a launch.
+// time: 16384 rows of 256, eight chosen, by logits 11 us, by sigmoid and bias 16 us, by softmax and bias 19, with four of eight
+// groups kept 22 to 23 us (in double throughout: 167 us); one row of 128 2.3 us, a launch. What takes longer:
+//  - softmax without renorm: an exponential in double for every expert (21 us by logits, 33 with a bias);
+//  - many equal logits (16-bit ones, by logits 20 us; with groups and no bias 50 us);
+//  - an infinite logit or bias where there is a bias or groups (a masked logit, an expert switched off): every such row is done
+//    in double (52 to 56 us, with groups 96);
+//  - 32 of more than 32 experts, as the round that shows the next one to be apart has no lane: every row is done again (65 us by
+//    logits, 31 of 256 taking 24; 121 us with a bias).
 #include <cmath>
 
 #include "kv.cuh"
@@ -317,8 +324,8 @@ __global__ void __launch_bounds__(32 * kWarps) moe_router_kernel(const __grid_co
             // float32 scores; `off` bounds the error of each. __expf(-d) is within 2 + 1.173 d units of its last place, so within
             // 2^-22 absolutely. A sigmoid of x has p (1 - p) (2 + 1.173 |x|) < 0.63 times 2^-23 of that, half of one from the
             // rounded sum and two units (2^-23) from the quotient: below 2^-21. A softmax's sum adds up to 32 terms per lane and
-            // five times over the warp (37 roundings, below 2^-18.7) of terms that are off by some 2^-20.7 of the sum at most:
-            // below 2^-17 of the largest term. The sum with the bias rounds once more.
+            // five times over the warp (37 roundings, below 2^-18.7) of terms that are off by 2^-20.1 of the sum at most (1024 terms,
+            // all but one some 5.5 below the largest logit): below 2^-17 of the largest term. The sum with the bias rounds once more.
             float c[EPL], far = 0.0f, flaw = 0.0f;  // flaw: NaN where a logit or a score is NaN or infinite
             if (softmax) {
                 float sum = 0.0f;
