@@ -425,9 +425,9 @@ b200_status b200_kv_attention(b200_context * ctx, void * stream, const b200_kv_c
  *   and only the topk_group best groups' experts stay;
  *   ids [T][top_k] = the top_k largest c, largest first; w [T][top_k] = their p, divided by their sum (renorm), times scale.
  * p, c and their sums are double, rounded to float32 once in w; without bias and groups the experts are ordered by their
- * logits. Ties (in double) go to the lowest index. Infinite logits or biases, many equal logits, softmax without renorm and a
- * top_k of 32 take two to six times as long as other calls. A NaN logit or c counts as -infinity, a logit of -infinity has p = 0, +infinity
- * shares the softmax with its equals; a sum of 0 gives weights 0.
+ * logits. Ties (in double) go to the lowest index. Many equal logits, softmax without renorm, a top_k of 32 of more experts and,
+ * with a bias or groups, infinite logits or biases take two to six times as long as other calls. A NaN logit or c counts as
+ * -infinity, a logit of -infinity has p = 0, +infinity shares the softmax with its equals; a sum of 0 gives weights 0.
  * ------------------------------------------------------------------------------------------------------------ */
 enum { B200_ROUTER_SOFTMAX = 0, B200_ROUTER_SIGMOID = 1 };
 typedef struct b200_router {
